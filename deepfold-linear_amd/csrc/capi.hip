@@ -104,6 +104,16 @@ int hip_fail(hipError_t e, const char* what) {
   return (int)e;
 }
 
+}  // namespace
+
+// The same error text for the entry points of capi_window.hip.
+namespace dfl {
+int capi_fail(const char* message) { return fail("%s", message); }
+int capi_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+}  // namespace dfl
+
+namespace {
+
 // Exchange tags carry a 20-bit call salt (common.h).  The counter behind it is
 // 64-bit: its bits above the salt count the salt's wrap-arounds ("epochs").  A
 // workspace first used in one epoch and used again in a later one could hold a

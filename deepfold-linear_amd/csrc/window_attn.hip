@@ -1,0 +1,154 @@
+// Attention over a sliding window and a few first tokens, forward.
+//
+// Query i stands at position t = i + N - M; it sees the keys t - window < j <= t (both
+// directions: |t - j| < window) and the keys j < n_sink (causal: j <= t).
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp2(y_ij - m_i),
+//   y_ij = log2(e) (scale q_i.k_j + table[bucket(j - t)])
+// A workgroup owns 128 queries of one head, a wave 32 of them; the keys it can see stream
+// through LDS once, with the running reference m_i and sum in registers.
+#include "window_engine.h"
+#include "window_stage.h"
+
+namespace dfl {
+
+template <typename T, int DP, bool FAST, bool REL>
+__global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
+  using E = WinEng<T, DP>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  T* sk = reinterpret_cast<T*>(smem);
+  T* sv = sk + E::TILE;
+  unsigned* smask = reinterpret_cast<unsigned*>(sv + E::TILE);  // one bit a key of the tile: inside and unmasked
+  float* lut = reinterpret_cast<float*>(smask + 4);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h32 = lane >> 5;
+
+  const int G = a.H / a.Hk, nqt = (a.M + WIN_RES - 1) / WIN_RES;
+  int x = xcd_order(blockIdx.x, gridDim.x);
+  const int g = x % G;
+  x /= G;
+  const int qt = x % nqt, bhk = x / nqt, b = bhk / a.Hk, hk = bhk % a.Hk, h = hk * G + g;
+  const int shift = a.N - a.M;  // position of query 0
+  const T* kb = reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh;
+  const T* vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh;
+  const float* mask = a.mask ? a.mask + (size_t)b * a.N : nullptr;
+  const WinVis vis(a);
+  if (REL) build_rel_lut(a, h, lut, nullptr);
+
+  const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
+  const bool row_ok = i < a.M && (!mask || mask[t] != 0.f);
+  typename E::Frag qf;
+  E::template load_frag<FAST>(
+      qf, row_ok ? reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh + (size_t)i * a.qsn : nullptr, a.d, lane);
+  const float sc = a.scale * LOG2E;
+  float m = NEG_BIG, l = 0.f;
+  f32x16 acc[E::NT] = {};
+
+  const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
+  for (int it = 0; it < kt.total; ++it) {
+    const int j0 = kt.tile(it) * E::BK;
+    __syncthreads();
+    stage_tile<T, DP, FAST>(sk, kb, a.ksn, sv, vb, a.vsn, smask, j0, a.N, a.d, mask);
+    __syncthreads();
+#pragma unroll
+    for (int sub = 0; sub < E::NSUB; ++sub) {
+      const int js = j0 + 32 * sub;
+      const bool sinks = js < vis.n_sink && (!vis.causal || js <= t0 + 31);
+      if (vis.none_near(t0, js) && !sinks) continue;
+      f32x16 y = E::row_product(sk, 32 * sub, qf, lane);
+      if (REL) {
+        const int far = rel_far(a.rel, t0, js);
+        if (far >= 0) {
+          const float c = lut[far];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, c);
+        } else {
+          const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, p[-acc_row(r, 0)]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] *= sc;
+      }
+      const unsigned bits = smask[sub];
+      if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
+        const unsigned mine = bits >> (4 * h32);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = js + acc_row(r, h32);
+          y[r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[r] : -INFINITY;
+        }
+      }
+      float mx = y[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, y[r]);
+      mx = fmaxf(xor32_pair(mx, true), m);
+      const float al = fast_exp2(m - mx);
+      m = mx;
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        y[r] = fast_exp2(y[r] - m);
+        s += y[r];
+      }
+      l = l * al + s;
+#pragma unroll
+      for (int n = 0; n < E::NT; ++n) acc[n] *= al;
+      typename E::Prob p;
+      E::to_operand(y, p);
+      E::column_product(sv, 32 * sub, p, acc, lane);
+    }
+  }
+  l = xor32_pair(l, false);
+  const bool some = row_ok && l > 0.f;
+  const float inv = some ? 1.f / l : 0.f;
+  if (i < a.M) {
+    const size_t row = ((size_t)b * a.H + h) * a.M + i;
+    if (a.lse && h32 == 0) a.lse[row] = some ? m + fast_log2(l) : LSE_EMPTY;
+    T* o = reinterpret_cast<T*>(a.o) + row * a.d;
+#pragma unroll
+    for (int n = 0; n < E::NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int c = 32 * n + acc_row(r, h32);
+        if (c < a.d) o[c] = from_f32<T>(some ? acc[n][r] * inv : 0.f);
+      }
+  }
+}
+
+// 16-byte loads: aligned rows of whole chunks.
+template <typename T> static bool win_fast(const WinArgs& a, bool bwd) {
+  auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
+  auto st = [](long long s) { return ((s * (long long)sizeof(T)) & 15) == 0; };
+  bool ok = (a.d * sizeof(T)) % 16 == 0 && al(a.q) && al(a.k) && al(a.v);
+  ok = ok && st(a.qsb) && st(a.qsh) && st(a.qsn) && st(a.ksb) && st(a.ksh) && st(a.ksn) && st(a.vsb) && st(a.vsh) &&
+       st(a.vsn);
+  if (bwd) ok = ok && al(a.o) && al(a.go);
+  return ok;
+}
+bool window_fast(const WinArgs& a, bool bf16_in, bool bwd) {
+  return bf16_in ? win_fast<bf16>(a, bwd) : win_fast<float>(a, bwd);
+}
+
+template <typename T, int DP, bool FAST, bool REL>
+static hipError_t fwd_launch(const WinArgs& a, hipStream_t s) {
+  using E = WinEng<T, DP>;
+  const size_t lds = 2 * E::TILE * sizeof(T) + 16 + (REL ? rel_lut_size(a.rel) * 4 : 0);
+  auto kern = window_fwd_kernel<T, DP, FAST, REL>;
+  const hipError_t attr = set_lds_limit((const void*)kern, lds);
+  if (attr != hipSuccess) return attr;
+  const int nqt = (a.M + WIN_RES - 1) / WIN_RES;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(nqt * a.B * a.H)), dim3(WIN_NT), lds, s, a);
+  return hipGetLastError();
+}
+template <typename T, int DP> static hipError_t fwd_pick(const WinArgs& a, hipStream_t s) {
+  const bool fast = win_fast<T>(a, false);
+  if (a.table) return fast ? fwd_launch<T, DP, true, true>(a, s) : fwd_launch<T, DP, false, true>(a, s);
+  return fast ? fwd_launch<T, DP, true, false>(a, s) : fwd_launch<T, DP, false, false>(a, s);
+}
+hipError_t launch_window_fwd(const WinArgs& a, bool bf16_in, int DP, hipStream_t s) {
+  if (bf16_in)
+    return DP == 32 ? fwd_pick<bf16, 32>(a, s) : DP == 64 ? fwd_pick<bf16, 64>(a, s) : fwd_pick<bf16, 128>(a, s);
+  return DP == 32 ? fwd_pick<float, 32>(a, s) : DP == 64 ? fwd_pick<float, 64>(a, s) : fwd_pick<float, 128>(a, s);
+}
+
+}  // namespace dfl

@@ -1,0 +1,210 @@
+// Building blocks of the window attention kernels: 32x32 MFMA tiles over LDS tiles of
+// 16-byte chunks.
+//
+// Every product is one of two kinds.
+//  * row product: D[m][n] = sum_c A[m][c] R[n][c]; A rows from an LDS tile (one 16-byte chunk
+//    a lane), R the wave's 32 resident rows, kept in registers (Frag).  bf16 takes
+//    32x32x16 instructions (lane: row l % 32, columns 8 (l / 32) ..), fp32 four 32x32x2 a
+//    chunk; both operands use the same column order, so any order gives the product.
+//  * column product: O[c][n] += sum_m A[m][c] P[m][n] with P in the accumulator layout
+//    (lane: n = l % 32, register r: m = 8 (r / 4) + 4 (l / 32) + r % 4).  As the B operand
+//    the registers 8 s .. 8 s + 7 hold, in lane half h, the rows 16 s + 4 h + {0..3} and
+//    16 s + 8 + 4 h + {0..3}; the A operand takes the same rows of the LDS tile
+//    transposed, two ds_read_b64_tr_b16 (fp32: one 32-bit read a register).
+// So scores are kept transposed (keys x queries) in the query-resident passes and queries x
+// keys in the key-resident one: a softmax row never leaves its lane pair (l, l ^ 32), and
+// probabilities go from accumulator to operand without passing through LDS.
+//
+// An LDS tile has rows of DP elements without padding; the 16-byte chunk c of row r lies at
+// position c ^ f(r).  f sends 16 consecutive rows to 16 different positions of the 256-byte
+// bank period (row reads of 16 bytes) and 4 consecutive rows to different 64-byte quarters
+// (the transposing reads take 64 bytes of 4 rows at once), so neither read has conflicts.
+#pragma once
+#include "common.h"
+#include "window_args.h"
+
+namespace dfl {
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
+
+constexpr int WIN_NT = 256;  // threads of a workgroup: 4 waves of 32 resident rows each
+constexpr int WIN_RES = 128;
+
+template <typename T, int DP> struct WinEng {
+  static constexpr int VEC = 16 / (int)sizeof(T);  // elements of a chunk
+  static constexpr int NCH = DP / VEC;             // chunks of a row
+  static constexpr int STEPS = NCH / 2;            // chunk pairs: steps of a row product
+  static constexpr int NT = DP / 32;               // 32-column tiles of a column product
+  static constexpr int BK = (sizeof(T) == 4 && DP == 128) ? 32 : 64;  // streamed rows of an LDS tile
+  static constexpr int NSUB = BK / 32;
+  static constexpr int TILE = BK * DP;  // elements
+  struct Frag { u32x4 v[STEPS]; };
+
+  __device__ static __forceinline__ int swz(int r, int c) {
+    if (NCH >= 16) return c ^ (((r & 3) << 2) | ((r >> 2) & 3));
+    if (NCH == 8) return c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
+    return c ^ ((r >> 2) & 3);
+  }
+  __device__ static __forceinline__ u32x4* chunk(T* tile, int r, int c) {
+    return reinterpret_cast<u32x4*>(tile + r * DP + swz(r, c) * VEC);
+  }
+
+  // Chunk c of a global row (null: zeros); columns from d on are zero.  FAST: 16-byte
+  // aligned rows and d a multiple of VEC.
+  template <bool FAST> __device__ static __forceinline__ u32x4 load(const T* row, int c, int d) {
+    u32x4 x = {0u, 0u, 0u, 0u};
+    if (!row) return x;
+    if (FAST) {
+      if (c * VEC < d) x = *reinterpret_cast<const u32x4*>(row + c * VEC);
+    } else {
+      T e[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) e[i] = c * VEC + i < d ? row[c * VEC + i] : from_f32<T>(0.f);
+      __builtin_memcpy(&x, e, 16);
+    }
+    return x;
+  }
+  // The wave's resident rows: lane l takes row l % 32 (its own `row`; null: zeros).
+  template <bool FAST> __device__ static __forceinline__ void load_frag(Frag& f, const T* row, int d, int lane) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) f.v[s] = load<FAST>(row, 2 * s + (lane >> 5), d);
+  }
+  __device__ static __forceinline__ f32x16 step(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 x, y;
+      __builtin_memcpy(&x, &a, 16);
+      __builtin_memcpy(&y, &b, 16);
+      c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    }
+    return c;
+  }
+  // rows r0 .. r0 + 31 of the tile times the resident rows
+  __device__ static __forceinline__ f32x16 row_product(T* tile, int r0, const Frag& f, int lane) {
+    f32x16 c = {};
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) c = step(*chunk(tile, r0 + (lane & 31), 2 * s + (lane >> 5)), f.v[s], c);
+    return c;
+  }
+  // B operands of a column product
+  struct Prob {
+    bf16x8 h[sizeof(T) == 2 ? 2 : 1];
+    f32x16 f;
+  };
+  // bf16: probabilities and score gradients are rounded to bf16 here, as their products' other operand is;
+  // the sums stay in fp32
+  __device__ static __forceinline__ void to_operand(const f32x16& p, Prob& o) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o.h[r / 8][r % 8] = (bf16)p[r];
+    } else {
+      o.f = p;
+    }
+  }
+  // acc[t] += (columns 32 t .. of rows r0 .. r0 + 31 of the tile)^T P
+  __device__ static __forceinline__ void column_product(T* tile, int r0, const Prob& p, f32x16 (&acc)[NT], int lane) {
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4* lptr;
+      const int h = lane >> 5, q = (lane >> 4) & 1, i = (lane & 15) >> 2, e = lane & 3;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          // chunk of columns 32 t + 16 q + 4 e ..: 8 bytes of it
+          const int c = 4 * t + 2 * q + (e >> 1), ra = r0 + 16 * s + 4 * h + i, rb = ra + 8;
+          T* pa = tile + ra * DP + swz(ra, c) * VEC + 4 * (e & 1);
+          T* pb = tile + rb * DP + swz(rb, c) * VEC + 4 * (e & 1);
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)pa);
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)pb);
+          bf16x8 a;
+          __builtin_memcpy(&a, &lo, 8);
+          __builtin_memcpy(reinterpret_cast<char*>(&a) + 8, &hi, 8);
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.h[s], acc[t], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = r0 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int col = 32 * t + (lane & 31);
+          const float a = tile[row * DP + swz(row, col / VEC) * VEC + col % VEC];
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p.f[r], acc[t], 0, 0, 0);
+        }
+      }
+    }
+  }
+};
+
+// Row of register r in lane half h of an accumulator tile.
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
+
+// Chunk-wise work order: workgroup w of n takes logical position x(w) such that each XCD (w mod 8) works on
+// one contiguous part: neighbouring tiles, which read the same keys, share its L2.
+__device__ __forceinline__ int xcd_order(int w, int n) {
+  const int per = n >> 3, rem = n & 7, x = w & 7;
+  return x * per + min(x, rem) + (w >> 3);
+}
+
+// Visibility of key j to the query at position t, without the mask.
+struct WinVis {
+  int off, n_sink, causal;
+  unsigned range;
+  __device__ __forceinline__ explicit WinVis(const WinArgs& a) {
+    const int w = min(a.window, a.N);
+    off = a.causal ? 0 : w - 1;
+    range = (unsigned)(a.causal ? w : 2 * w - 1);
+    n_sink = a.n_sink;
+    causal = a.causal;
+  }
+  __device__ __forceinline__ bool near(int t, int j) const { return (unsigned)(t - j + off) < range; }
+  __device__ __forceinline__ bool first(int t, int j) const { return (j < n_sink) & ((causal == 0) | (j <= t)); }
+  // (combined with & and |: a chain of branches around single elements of an accumulator loses some of the writes
+  // to them in this compiler)
+  __device__ __forceinline__ bool sees(int t, int j) const { return near(t, j) | first(t, j); }
+  // all of the 32 x 32 pairs with queries from t0 and keys from j0 on / none of them
+  __device__ __forceinline__ bool all_near(int t0, int j0) const { return near(t0, j0 + 31) && near(t0 + 31, j0); }
+  __device__ __forceinline__ bool none_near(int t0, int j0) const {
+    return t0 + 31 - j0 + off < 0 || t0 - (j0 + 31) + off >= (int)range;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Bias lookup in LDS: lut[x] for the distance x = t - j + base(), in units of log2.  REL_PAD
+// entries more than the table's range on both sides hold its end values, so that a 32 x 32
+// tile any pair of which is inside the range needs no clamp.
+constexpr int REL_PAD = 64;
+__host__ __device__ inline int rel_lut_size(const RelSpec& r) {
+  return ((r.both ? 2 * r.dist() + 1 : r.dist() + 1) + 2 * REL_PAD + 3) & ~3;
+}
+__device__ __forceinline__ int rel_lut_base(const RelSpec& r) { return (r.both ? r.dist() : 0) + REL_PAD; }
+// bucket of rel = j - t
+__device__ __forceinline__ int rel_bucket(const RelSpec& r, int rel) {
+  const int mag = r.both ? abs(rel) : max(-rel, 0);
+  int b = 0;
+  for (int k = 0; k < r.n; ++k) b += r.edge[k] <= mag;
+  return b + ((r.both && rel > 0) ? r.n + 1 : 0);
+}
+__device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, float* lut, uint8_t* bucket) {
+  const int n = rel_lut_size(a.rel), base = rel_lut_base(a.rel);
+  const float* row = a.table + (size_t)h * a.rel.buckets();
+  for (int x = threadIdx.x; x < n; x += blockDim.x) {
+    const int b = rel_bucket(a.rel, base - x);
+    lut[x] = row[b] * LOG2E;
+    if (bucket) bucket[x] = (uint8_t)b;
+  }
+}
+// Where every distance t - j of a 32 x 32 tile lies beyond the table's range: the index of its one value, else -1.
+__device__ __forceinline__ int rel_far(const RelSpec& r, int t0, int j0) {
+  const int dist = r.dist();
+  if (t0 - (j0 + 31) >= dist) return rel_lut_base(r) + dist;
+  if (r.both && j0 - (t0 + 31) > dist) return rel_lut_base(r) - dist - 1;
+  return -1;
+}
+
+}  // namespace dfl

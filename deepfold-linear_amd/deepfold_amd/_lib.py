@@ -216,6 +216,68 @@ class CoordUpdateParams(ctypes.Structure):
     ]
 
 
+class WindowAttnParams(ctypes.Structure):
+    """Mirror of ``dfl_window_attn_params``."""
+
+    _fields_ = [
+        ("dtype", I32),
+        ("q", P), ("k", P), ("v", P),
+        ("q_stride_b", I64), ("q_stride_h", I64), ("q_stride_n", I64),
+        ("k_stride_b", I64), ("k_stride_h", I64), ("k_stride_n", I64),
+        ("v_stride_b", I64), ("v_stride_h", I64), ("v_stride_n", I64),
+        ("mask", P), ("rel_table", P), ("rel_edges", P), ("n_edges", I32),
+        ("B", I32), ("H", I32), ("Hk", I32), ("M", I32), ("N", I32), ("d", I32),
+        ("window", I32), ("n_sink", I32), ("causal", I32), ("scale", F32),
+        ("o", P), ("lse", P),
+        ("grad_o", P), ("dq", P), ("dk", P), ("dv", P), ("drel_table", P),
+    ]
+
+
+class WindowCacheFillParams(ctypes.Structure):
+    """Mirror of ``dfl_window_cache_fill_params``."""
+
+    _fields_ = [
+        ("dtype", I32),
+        ("k", P), ("v", P),
+        ("k_stride_b", I64), ("k_stride_h", I64), ("k_stride_n", I64),
+        ("v_stride_b", I64), ("v_stride_h", I64), ("v_stride_n", I64),
+        ("lengths", P), ("k_cache", P), ("v_cache", P),
+        ("kc_stride_b", I64), ("kc_stride_h", I64), ("kc_stride_n", I64),
+        ("vc_stride_b", I64), ("vc_stride_h", I64), ("vc_stride_n", I64),
+        ("B", I32), ("Hk", I32), ("N", I32), ("d", I32), ("window", I32), ("n_sink", I32),
+    ]
+
+
+class WindowDecodeParams(ctypes.Structure):
+    """Mirror of ``dfl_window_decode_params``."""
+
+    _fields_ = [
+        ("dtype", I32),
+        ("q", P), ("k", P), ("v", P),
+        ("q_stride_b", I64), ("q_stride_h", I64),
+        ("k_stride_b", I64), ("k_stride_h", I64),
+        ("v_stride_b", I64), ("v_stride_h", I64),
+        ("k_cache", P), ("v_cache", P),
+        ("kc_stride_b", I64), ("kc_stride_h", I64), ("kc_stride_n", I64),
+        ("vc_stride_b", I64), ("vc_stride_h", I64), ("vc_stride_n", I64),
+        ("lengths", P), ("rel_table", P), ("rel_edges", P), ("n_edges", I32),
+        ("B", I32), ("H", I32), ("Hk", I32), ("d", I32), ("window", I32), ("n_sink", I32), ("scale", F32),
+        ("o", P),
+    ]
+
+
+class RelBiasParams(ctypes.Structure):
+    """Mirror of ``dfl_rel_bias_params``."""
+
+    _fields_ = [
+        ("dtype", I32),
+        ("rel_table", P), ("rel_edges", P), ("n_edges", I32), ("rel_both", I32),
+        ("q_pos", P), ("k_pos", P),
+        ("B", I32), ("H", I32), ("M", I32), ("N", I32),
+        ("out", P), ("grad_out", P), ("drel_table", P),
+    ]
+
+
 DFL_ATTN_BIAS_NONE = 0
 DFL_ATTN_BIAS_BINS = 1
 DFL_ATTN_BIAS_DENSE = 2
@@ -261,6 +323,15 @@ SIGNATURES = [
     ("dfl_coord_update_workspace_size", ctypes.c_size_t, [I32, I32]),
     ("dfl_coord_update_fwd", I32, [ctypes.POINTER(CoordUpdateParams), P]),
     ("dfl_coord_update_bwd", I32, [ctypes.POINTER(CoordUpdateParams), P, ctypes.c_size_t, P]),
+    ("dfl_window_attn_workspace_size", ctypes.c_size_t, [I32] * 10),
+    ("dfl_window_attn_fwd", I32, [ctypes.POINTER(WindowAttnParams), P]),
+    ("dfl_window_attn_bwd", I32, [ctypes.POINTER(WindowAttnParams), P, ctypes.c_size_t, P]),
+    ("dfl_window_cache_fill", I32, [ctypes.POINTER(WindowCacheFillParams), P]),
+    ("dfl_window_decode_workspace_size", ctypes.c_size_t, [I32] * 6),
+    ("dfl_window_decode", I32, [ctypes.POINTER(WindowDecodeParams), P, ctypes.c_size_t, P]),
+    ("dfl_rel_bias_workspace_size", ctypes.c_size_t, [I32] * 6),
+    ("dfl_rel_bias_fwd", I32, [ctypes.POINTER(RelBiasParams), P]),
+    ("dfl_rel_bias_bwd", I32, [ctypes.POINTER(RelBiasParams), P, ctypes.c_size_t, P]),
 ]
 
 
@@ -310,6 +381,25 @@ def require_gpu(*tensors) -> torch.device:
     if dev is None:
         raise RuntimeError("deepfold_amd: no tensor inputs")
     return dev
+
+
+class on_device:
+    """Makes ``device`` current for a launch (a stream belongs to its device) where it is not already."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+        return False
 
 
 _ws_cache: dict = {}

@@ -35,6 +35,8 @@
 
 #include <stddef.h>
 
+#include "dfl_window.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -666,6 +668,26 @@ typedef struct dfl_coord_update_params {
 size_t dfl_coord_update_workspace_size(int C, int H);
 int dfl_coord_update_fwd(const dfl_coord_update_params* p, void* stream);
 int dfl_coord_update_bwd(const dfl_coord_update_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over a sliding window and a few first tokens, its rolling cache and
+ * single-token form, and the relative position bias: parameter blocks and semantics
+ * in dfl_window.h.  (The reference has no counterpart.)  Head dims up to 128; all may be
+ * captured into a graph: no state outlives a call, and a workspace needs no clearing.
+ */
+/* Bytes of backward workspace. */
+size_t dfl_window_attn_workspace_size(int B, int H, int Hk, int M, int N, int d, int window, int n_sink, int causal,
+                                      int n_edges);
+/* lse (B,H,M): base-2 log of the row sums, 1e30 on empty rows; NULL if no backward follows. */
+int dfl_window_attn_fwd(const dfl_window_attn_params* p, void* stream);
+int dfl_window_attn_bwd(const dfl_window_attn_params* p, void* workspace, size_t workspace_bytes, void* stream);
+int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream);
+size_t dfl_window_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink);
+int dfl_window_decode(const dfl_window_decode_params* p, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of backward workspace; the forward uses none. */
+size_t dfl_rel_bias_workspace_size(int B, int H, int M, int N, int n_edges, int rel_both);
+int dfl_rel_bias_fwd(const dfl_rel_bias_params* p, void* stream);
+int dfl_rel_bias_bwd(const dfl_rel_bias_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
