@@ -11,13 +11,17 @@
 
 namespace dfl {
 
+// A row's reference moves only when a score exceeds it by this much (log2): the weights stay below 2^8, the output
+// rows are rescaled once or twice a row instead of once a tile.
+constexpr float WIN_SLACK = 8.f;
+
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
+__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) window_fwd_kernel(WinArgs a) {
   using E = WinEng<T, DP>;
   extern __shared__ __align__(16) unsigned char smem[];
-  T* sk = reinterpret_cast<T*>(smem);
-  T* sv = sk + E::TILE;
-  unsigned* smask = reinterpret_cast<unsigned*>(sv + E::TILE);  // one bit a key of the tile: inside and unmasked
+  T* sk = reinterpret_cast<T*>(smem);  // [2] key tiles, [2] value tiles
+  T* sv = sk + 2 * E::TILE;
+  unsigned* smask = reinterpret_cast<unsigned*>(sv + 2 * E::TILE);  // [2] one bit a key of the tile: inside and unmasked
   float* lut = reinterpret_cast<float*>(smask + 4);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h32 = lane >> 5;
 
@@ -31,6 +35,10 @@ __global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
   const T* vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh;
   const float* mask = a.mask ? a.mask + (size_t)b * a.N : nullptr;
   const WinVis vis(a);
+
+  const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
+  KeyStage<T, DP, FAST> st;
+  st.load(kb, a.ksn, vb, a.vsn, kt.tile(0) * E::BK, a.N, a.d, mask);
   if (REL) build_rel_lut(a, h, lut, nullptr);
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
@@ -42,61 +50,75 @@ __global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
   float m = NEG_BIG, l = 0.f;
   f32x16 acc[E::NT] = {};
 
-  const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
+  st.store(sk, sv, smask);
+  __syncthreads();
   for (int it = 0; it < kt.total; ++it) {
-    const int j0 = kt.tile(it) * E::BK;
-    __syncthreads();
-    stage_tile<T, DP, FAST>(sk, kb, a.ksn, sv, vb, a.vsn, smask, j0, a.N, a.d, mask);
-    __syncthreads();
+    const int j0 = kt.tile(it) * E::BK, buf = it & 1;
+    const bool more = it + 1 < kt.total;
+    if (more) st.load(kb, a.ksn, vb, a.vsn, kt.tile(it + 1) * E::BK, a.N, a.d, mask);
+    bool none = true;
 #pragma unroll
-    for (int sub = 0; sub < E::NSUB; ++sub) {
-      const int js = j0 + 32 * sub;
-      const bool sinks = js < vis.n_sink && (!vis.causal || js <= t0 + 31);
-      if (vis.none_near(t0, js) && !sinks) continue;
-      f32x16 y = E::row_product(sk, 32 * sub, qf, lane);
-      if (REL) {
-        const int far = rel_far(a.rel, t0, js);
-        if (far >= 0) {
-          const float c = lut[far];
+    for (int sub = 0; sub < E::NSUB; ++sub) none &= vis.none(t0, j0 + 32 * sub);
+    if (!none) {
+      T* tk = sk + buf * E::TILE;
+      f32x16 y[E::NSUB];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, c);
+      for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < E::NSUB; ++sub) {
+        const int js = j0 + 32 * sub;
+        if (REL) {
+          const int far = rel_far(a.rel, t0, js);
+          if (far >= 0) {
+            const float c = lut[far];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[sub][r] = __builtin_fmaf(y[sub][r], sc, c);
+          } else {
+            const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[sub][r] = __builtin_fmaf(y[sub][r], sc, p[-acc_row(r, 0)]);
+          }
         } else {
-          const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, p[-acc_row(r, 0)]);
+          for (int r = 0; r < 16; ++r) y[sub][r] *= sc;
         }
-      } else {
+        const unsigned bits = smask[2 * buf + sub];
+        if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
+          const unsigned mine = bits >> (4 * h32);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] *= sc;
+          for (int r = 0; r < 16; ++r) {
+            const int j = js + acc_row(r, h32);
+            y[sub][r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[sub][r] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[sub][r]);
       }
-      const unsigned bits = smask[sub];
-      if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
-        const unsigned mine = bits >> (4 * h32);
+      mx = xor32_pair(mx, true);
+      if (__any(mx > m + WIN_SLACK)) {
+        const float to = fmaxf(mx, m), al = fast_exp2(m - to);
+        m = to;
+        l *= al;
+#pragma unroll
+        for (int n = 0; n < E::NT; ++n) acc[n] *= al;
+      }
+#pragma unroll
+      for (int sub = 0; sub < E::NSUB; ++sub) {
+        float s = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int j = js + acc_row(r, h32);
-          y[r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[r] : -INFINITY;
+          y[sub][r] = fast_exp2(y[sub][r] - m);
+          s += y[sub][r];
         }
+        l += s;
+        typename E::Prob p;
+        E::to_operand(y[sub], p);
+        E::column_product(sv + buf * E::TILE, 32 * sub, p, acc, lane);
       }
-      float mx = y[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, y[r]);
-      mx = fmaxf(xor32_pair(mx, true), m);
-      const float al = fast_exp2(m - mx);
-      m = mx;
-      float s = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        y[r] = fast_exp2(y[r] - m);
-        s += y[r];
-      }
-      l = l * al + s;
-#pragma unroll
-      for (int n = 0; n < E::NT; ++n) acc[n] *= al;
-      typename E::Prob p;
-      E::to_operand(y, p);
-      E::column_product(sv, 32 * sub, p, acc, lane);
     }
+    if (more) st.store(sk + (buf ^ 1) * E::TILE, sv + (buf ^ 1) * E::TILE, smask + 2 * (buf ^ 1));
+    __syncthreads();
   }
   l = xor32_pair(l, false);
   const bool some = row_ok && l > 0.f;
@@ -108,9 +130,11 @@ __global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
 #pragma unroll
     for (int n = 0; n < E::NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int c = 32 * n + acc_row(r, h32);
-        if (c < a.d) o[c] = from_f32<T>(some ? acc[n][r] * inv : 0.f);
+      for (int r = 0; r < 16; r += 4) {
+        f32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = some ? acc[n][r + e] * inv : 0.f;
+        store4<T, FAST>(o, 32 * n + acc_row(r, h32), a.d, w);
       }
   }
 }
@@ -119,10 +143,10 @@ __global__ void __launch_bounds__(WIN_NT) window_fwd_kernel(WinArgs a) {
 template <typename T> static bool win_fast(const WinArgs& a, bool bwd) {
   auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
   auto st = [](long long s) { return ((s * (long long)sizeof(T)) & 15) == 0; };
-  bool ok = (a.d * sizeof(T)) % 16 == 0 && al(a.q) && al(a.k) && al(a.v);
+  bool ok = (a.d * sizeof(T)) % 16 == 0 && al(a.q) && al(a.k) && al(a.v) && al(a.o);
   ok = ok && st(a.qsb) && st(a.qsh) && st(a.qsn) && st(a.ksb) && st(a.ksh) && st(a.ksn) && st(a.vsb) && st(a.vsh) &&
        st(a.vsn);
-  if (bwd) ok = ok && al(a.o) && al(a.go);
+  if (bwd) ok = ok && al(a.go) && al(a.dq) && al(a.dk) && al(a.dv);
   return ok;
 }
 bool window_fast(const WinArgs& a, bool bf16_in, bool bwd) {
@@ -132,7 +156,7 @@ bool window_fast(const WinArgs& a, bool bf16_in, bool bwd) {
 template <typename T, int DP, bool FAST, bool REL>
 static hipError_t fwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
-  const size_t lds = 2 * E::TILE * sizeof(T) + 16 + (REL ? rel_lut_size(a.rel) * 4 : 0);
+  const size_t lds = 4 * E::TILE * sizeof(T) + 16 + (REL ? rel_lut_size(a.rel) * 4 : 0);
   auto kern = window_fwd_kernel<T, DP, FAST, REL>;
   const hipError_t attr = set_lds_limit((const void*)kern, lds);
   if (attr != hipSuccess) return attr;

@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
 
   const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
   float D = 0.f, f = 1.f;
+  KeyStage<T, DP, FAST> st;
 
   // p and dp of one 32 x 32 pair of the staged tile; false where the wave sees nothing of it
   auto pair = [&](int sub, int j0, f32x16& y, f32x16& dp) -> bool {
@@ -116,7 +117,8 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
     for (int it = 0; it < kt.total; ++it) {
       const int j0 = kt.tile(it) * E::BK;
       __syncthreads();
-      stage_tile<T, DP, FAST>(sk, kb, a.ksn, sv, vb, a.vsn, smask, j0, a.N, a.d, mask);
+      st.load(kb, a.ksn, vb, a.vsn, j0, a.N, a.d, mask);
+      st.store(sk, sv, smask);
       __syncthreads();
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
@@ -151,7 +153,8 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   for (int it = 0; it < kt.total; ++it) {
     const int j0 = kt.tile(it) * E::BK;
     __syncthreads();
-    stage_tile<T, DP, FAST>(sk, kb, a.ksn, sv, vb, a.vsn, smask, j0, a.N, a.d, mask);
+    st.load(kb, a.ksn, vb, a.vsn, j0, a.N, a.d, mask);
+      st.store(sk, sv, smask);
     __syncthreads();
 #pragma unroll
     for (int sub = 0; sub < E::NSUB; ++sub) {
@@ -250,6 +253,7 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     ihi = min(a.M, k1 - vis.off + (int)vis.range - shift);
   }
   f32x16 dk[E::NT] = {}, dv[E::NT] = {};
+  RowStage<T, DP, FAST> sq_st, sg_st;
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
     if (REL) {
@@ -261,8 +265,10 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     const T* gb = reinterpret_cast<const T*>(a.go) + row0 * a.d;
     for (int i0 = ilo; i0 < ihi; i0 += E::BK) {
       __syncthreads();
-      stage_rows<T, DP, FAST>(sq, qb, a.qsn, i0, a.M, a.d, mask ? mask + shift : nullptr);
-      stage_rows<T, DP, FAST>(sg, gb, a.d, i0, a.M, a.d, mask ? mask + shift : nullptr);
+      sq_st.load(qb, a.qsn, i0, a.M, a.d, mask ? mask + shift : nullptr);
+      sg_st.load(gb, a.d, i0, a.M, a.d, mask ? mask + shift : nullptr);
+      sq_st.store(sq);
+      sg_st.store(sg);
       if ((int)threadIdx.x < E::BK) {
         const int i = i0 + threadIdx.x;
         const bool ok = i < ihi && (!mask || mask[shift + i] != 0.f);

@@ -172,6 +172,9 @@ struct WinVis {
   __device__ __forceinline__ bool none_near(int t0, int j0) const {
     return t0 + 31 - j0 + off < 0 || t0 - (j0 + 31) + off >= (int)range;
   }
+  __device__ __forceinline__ bool none(int t0, int j0) const {
+    return none_near(t0, j0) & !((j0 < n_sink) & ((causal == 0) | (j0 <= t0 + 31)));
+  }
 };
 
 // ---------------------------------------------------------------------------
