@@ -75,6 +75,10 @@ int check_heads(int dtype, int B, int H, int Hk, int d) {
   if (d <= 0 || d > 128) return fail("head dim d=%d outside [1, 128]", d);
   return 0;
 }
+// The running reference is a maximum of scaled scores, taken before the scale.
+int check_scale(float scale) {
+  return scale >= 1e-30f && scale <= 1e30f ? 0 : fail("scale=%g outside [1e-30, 1e30]", (double)scale);
+}
 int check_window(int window, int n_sink) {
   if (window < 1) return fail("window=%d must be positive", window);
   if (n_sink < 0 || n_sink > MAX_SINK) return fail("n_sink=%d outside [0, %d]", n_sink, MAX_SINK);
@@ -114,6 +118,7 @@ int check_attn(const dfl_window_attn_params* p, bool bwd) {
   if (p->M <= 0 || p->N <= 0 || p->M > p->N || p->N > MAX_N)
     return fail("M=%d, N=%d: need 0 < M <= N <= %lld", p->M, p->N, MAX_N);
   if ((((long long)p->N + RES - 1) / RES + 1) * p->B * p->H >= (1ll << 31)) return fail("too many rows");
+  if (int rc = check_scale(p->scale)) return rc;
   if (!p->q || !p->k || !p->v || !p->o) return fail("required pointer is NULL");
   if (!p->rel_table != (p->n_edges == 0)) return fail("rel_table and rel_edges must be given together");
   if (int rc = check_rel(p->rel_edges, p->n_edges, !p->causal)) return rc;
@@ -251,6 +256,7 @@ int dfl_window_decode(const dfl_window_decode_params* p, void* workspace, size_t
     if (int rc = check_heads(p->dtype, p->B, p->H, p->Hk, p->d)) return rc;
     if (int rc = check_window(p->window, p->n_sink)) return rc;
     if (p->window > MAX_N) return fail("window=%d above %lld", p->window, MAX_N);
+    if (int rc = check_scale(p->scale)) return rc;
     if (!p->q || !p->k || !p->v || !p->k_cache || !p->v_cache || !p->lengths || !p->o)
       return fail("required pointer is NULL");
     if (!p->rel_table != (p->n_edges == 0)) return fail("rel_table and rel_edges must be given together");

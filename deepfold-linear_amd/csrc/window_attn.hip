@@ -61,27 +61,27 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
     for (int sub = 0; sub < E::NSUB; ++sub) none &= vis.none(t0, j0 + 32 * sub);
     if (!none) {
       T* tk = sk + buf * E::TILE;
+      // log2 of the weights: ya y + yc; a table entry per pair goes into y itself
       f32x16 y[E::NSUB];
+      float ya[E::NSUB], yc[E::NSUB];
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
-      float mx = -INFINITY;
+      float mx = NEG_BIG;
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
         const int js = j0 + 32 * sub;
+        ya[sub] = sc;
+        yc[sub] = 0.f;
         if (REL) {
           const int far = rel_far(a.rel, t0, js);
           if (far >= 0) {
-            const float c = lut[far];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) y[sub][r] = __builtin_fmaf(y[sub][r], sc, c);
+            yc[sub] = lut[far];
           } else {
             const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
 #pragma unroll
             for (int r = 0; r < 16; ++r) y[sub][r] = __builtin_fmaf(y[sub][r], sc, p[-acc_row(r, 0)]);
+            ya[sub] = 1.f;
           }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) y[sub][r] *= sc;
         }
         const unsigned bits = smask[2 * buf + sub];
         if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
@@ -92,8 +92,10 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             y[sub][r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[sub][r] : -INFINITY;
           }
         }
+        float top = y[sub][0];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, y[sub][r]);
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, y[sub][r]);
+        mx = fmaxf(mx, __builtin_fmaf(top, ya[sub], yc[sub]));
       }
       mx = xor32_pair(mx, true);
       if (__any(mx > m + WIN_SLACK)) {
@@ -105,10 +107,11 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       }
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
+        const float c = yc[sub] - m;
         float s = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          y[sub][r] = fast_exp2(y[sub][r] - m);
+          y[sub][r] = fast_exp2(__builtin_fmaf(y[sub][r], ya[sub], c));
           s += y[sub][r];
         }
         l += s;

@@ -21,28 +21,51 @@ struct KeyTiles {
 };
 
 // Rows j0 .. j0 + BK - 1 of one operand on their way to LDS: issued as loads into registers before the product of
-// the tile in front, written after it.  Rows outside [0, N) or masked are zero there (their values may be NaN).
+// the tile in front, written after it.  Rows outside [0, N) or masked, and columns from d on, are zero there (what lies
+// in masked rows may be NaN).  A tile inside [0, N) without mask and of full width needs neither clamps nor selects.
 template <typename T, int DP, bool FAST> struct RowStage {
   using E = WinEng<T, DP>;
   static constexpr int PER = E::BK * E::NCH / WIN_NT;  // chunks of a thread
+  static constexpr int STEP = WIN_NT / E::NCH;         // rows between them
   u32x4 v[PER];
-  unsigned ok;  // a bit a chunk
+  unsigned ok;  // a bit a chunk: keep it
   __device__ __forceinline__ void load(const T* base, long long stride, int j0, int N, int d, const float* mask) {
-    ok = 0;
+    const int r = threadIdx.x / E::NCH, c = threadIdx.x % E::NCH;
+    if (FAST && !mask && j0 + E::BK <= N && d == DP) {
+      const T* p = base + j0 * stride + (r * stride + c * E::VEC);
+#pragma unroll
+      for (int n = 0; n < PER; ++n) v[n] = *reinterpret_cast<const u32x4*>(p + n * STEP * stride);
+      ok = ~0u;
+      return;
+    }
+    unsigned bits = 0;
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
-      const int e = threadIdx.x + n * WIN_NT, r = e / E::NCH, j = j0 + r, at = min(j, N - 1);
-      v[n] = E::template load<FAST>(base + (size_t)at * stride, e % E::NCH, d);
-      ok |= (unsigned)((j < N) & (!mask || mask[at] != 0.f)) << n;
+      const int j = j0 + r + n * STEP, at = min(j, N - 1);
+      const T* row = base + at * stride;
+      if (FAST) {  // a chunk behind the row's end reads the row's first one
+        v[n] = *reinterpret_cast<const u32x4*>(row + (c * E::VEC < d ? c * E::VEC : 0));
+        bits |= (unsigned)((j < N) & (c * E::VEC < d)) << n;
+      } else {
+        v[n] = E::template load<false>(row, c, d);
+        bits |= (unsigned)(j < N) << n;
+      }
     }
+    if (mask) {
+#pragma unroll
+      for (int n = 0; n < PER; ++n) bits &= ~((unsigned)(mask[min(j0 + r + n * STEP, N - 1)] == 0.f) << n);
+    }
+    ok = bits;
   }
-  __device__ __forceinline__ void store(T* tile) const {
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int e = threadIdx.x + n * WIN_NT;
+  __device__ __forceinline__ void store(T* tile) {
+    const int r = threadIdx.x / E::NCH, c = threadIdx.x % E::NCH;
+    if (__any(ok != ~0u)) {
       const u32x4 zero = {0u, 0u, 0u, 0u};
-      *E::chunk(tile, e / E::NCH, e % E::NCH) = (ok >> n) & 1u ? v[n] : zero;
+#pragma unroll
+      for (int n = 0; n < PER; ++n) v[n] = (ok >> n) & 1u ? v[n] : zero;
     }
+#pragma unroll
+    for (int n = 0; n < PER; ++n) *E::chunk(tile, r + n * STEP, c) = v[n];
   }
 };
 
@@ -55,13 +78,15 @@ template <typename T, int DP, bool FAST> struct KeyStage {
                                        const float* mask) {
     k.load(kb, ksn, j0, N, d, mask);
     v.load(vb, vsn, j0, N, d, mask);
-    if (threadIdx.x < 64) {
-      const int j = j0 + threadIdx.x;
-      const bool in = ((int)threadIdx.x < E::BK) & (j < N);
+    if (mask || j0 + E::BK > N) {
+      const int lane = threadIdx.x & 63, j = j0 + lane;
+      const bool in = (lane < E::BK) & (j < N);
       bits = __ballot(in && (!mask || mask[in ? j : 0] != 0.f));
+    } else {
+      bits = ~0ull;
     }
   }
-  __device__ __forceinline__ void store(T* sk, T* sv, unsigned* smask) const {
+  __device__ __forceinline__ void store(T* sk, T* sv, unsigned* smask) {
     k.store(sk);
     v.store(sv);
     if (threadIdx.x == 0) {

@@ -44,6 +44,15 @@ def _check_window(what, window, n_sink):
         raise ValueError(f"{what}: n_sink={n_sink} outside [0, {MAX_SINK}]")
 
 
+def _scale(what, scale, d):
+    if scale is None:
+        return 1.0 / math.sqrt(d)
+    scale = float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{what}: scale={scale} outside [1e-30, 1e30]")
+    return scale
+
+
 def _fwd_params(dt, q, k, v, mask, tab, arr, window, n_sink, causal, scale, o, lse):
     B, H, M, d = q.shape
     return _lib.WindowAttnParams(
@@ -134,7 +143,7 @@ def flash_window_attn(
     h // (H // Hk)), M <= N, D <= 128, any strides.  mask (B,N) or (N,), 0 = masked: a masked key reaches nothing,
     whatever its values, and rows of masked queries are zero, as is a row that sees no key.  (A key that only the
     window hides is ordinary data: a NaN or infinity in its V may reach queries nearby.)  ``scale`` defaults to
-    D ** -0.5.  ``rel_table`` with ``rel_edges``: scores get table[h, bucket(j - t)], see ``rel_pos_bias``, whose
+    D ** -0.5 and is positive.  ``rel_table`` with ``rel_edges``: scores get table[h, bucket(j - t)], see ``rel_pos_bias``, whose
     ``bidirectional`` is ``not causal`` here; an entry of -inf (or below -1e30) takes its keys out.
 
     Returns O with the shape and dtype of Q; gradients to Q, K, V and rel_table."""
@@ -161,7 +170,7 @@ def flash_window_attn(
     if (rel_table is None) != (rel_edges is None):
         raise ValueError("flash_window_attn: give rel_table and rel_edges together")
     arr = None if rel_table is None else edge_array(rel_table, rel_edges, H, not causal)
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    scale = _scale("flash_window_attn", scale, d)
     if not (Q.is_floating_point() and K.is_floating_point() and V.is_floating_point()):
         raise TypeError("flash_window_attn: Q, K, V must be floating point")
     if B == 0 or H == 0 or M == 0:
@@ -302,7 +311,7 @@ def window_decode_attn(
         *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
         *k_cache.stride()[:3], *v_cache.stride()[:3], at.data_ptr(), _lib.ptr(tab),
         None if arr is None else ctypes.addressof(arr), 0 if arr is None else len(arr), B, H, Hk, d, window, n_sink,
-        1.0 / math.sqrt(d) if scale is None else float(scale), o.data_ptr())
+        _scale(what, scale, d), o.data_ptr())
     with _lib.on_device(dev):
         rc = _lib.timed_launch(what, dev, lambda: lib.dfl_window_decode(
             ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))

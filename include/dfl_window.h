@@ -20,7 +20,7 @@
  * t - window < j <= t (causal = 0: |t - j| < window) or j < n_sink (causal: and j <= t),
  * and mask[b,j] != 0; rows with mask[b,t] = 0, or that see nothing, are zero.  The table's
  * direction is that of the attention: rel_both = !causal.  A table entry of -inf
- * (or below about -1e30) takes its keys out. */
+ * (or below about -1e30) takes its keys out.  scale is positive (1e-30 to 1e30). */
 typedef struct dfl_window_attn_params {
   int dtype;
   const void* q;

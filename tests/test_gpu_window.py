@@ -112,7 +112,9 @@ def test_one_key_rows_have_no_score_gradient():
             x = [leaf(rnd(2, 4, N, 64, seed=s, dtype=dtype)) for s in (1, 2, 3)]
             t = leaf(rnd(4, len(EDGES) + 1, seed=5))
             o = flash_window_attn(*x, window=window, rel_table=t, rel_edges=EDGES)
-            assert torch.equal(o, x[2])
+            # the weight and its sum are one number near 1: bf16 weights are rounded to 1, fp32 keeps the roundings
+            # of their product and quotient
+            assert ((o - x[2]).abs() <= (0 if dtype == BF else 4 * ref.U32) * x[2].abs()).all()
             dq, dk, dv, dt = torch.autograd.grad(o, [*x, t], torch.ones_like(o) * 0.37)
             assert not dq.any() and not dk.any() and not dt.any()
 

@@ -154,6 +154,9 @@ def test_refusals_of_arguments():
             (TypeError, lambda: att(q.int(), k.int(), k.int(), window=4)),
             (ValueError, lambda: att(torch.zeros(1, 1, 1, 129), torch.zeros(1, 1, 1, 129), torch.zeros(1, 1, 1, 129),
                                      window=4)),
+            (ValueError, lambda: att(q, k, k, window=4, scale=-1.0)),
+            (ValueError, lambda: att(q, k, k, window=4, scale=0)),
+            (ValueError, lambda: att(q, k, k, window=4, scale=math.nan)),
             (RuntimeError, lambda: att(q, k, k, window=4)),
             (ValueError, lambda: df.rel_pos_bias(t6, (1, 2, 3), 4)),
             (ValueError, lambda: df.rel_pos_bias(t6, (1, 2), 0)),
@@ -238,7 +241,7 @@ def test_c_entries_refuse():
     good = dict(dtype=_lib.DFL_BF16, q=fake, k=fake, v=fake, B=1, H=4, Hk=2, M=8, N=8, d=64, window=4, n_sink=0, causal=1,
                 scale=1.0, o=fake)
     for bad, text in ((dict(dtype=7), "dtype"), (dict(Hk=3), "multiple"), (dict(d=129), "head dim"), (dict(M=9), "M <= N"),
-                      (dict(window=0), "window"), (dict(n_sink=129), "n_sink"), (dict(q=None), "NULL"),
+                      (dict(window=0), "window"), (dict(n_sink=129), "n_sink"), (dict(q=None), "NULL"), (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale"),
                       (dict(rel_table=fake), "together"),
                       (dict(rel_table=fake, rel_edges=ctypes.addressof(flat), n_edges=2), "ascend"),
                       (dict(N=1 << 29, M=1), "M <= N")):
