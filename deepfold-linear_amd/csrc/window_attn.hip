@@ -9,6 +9,8 @@
 #include "window_engine.h"
 #include "window_stage.h"
 
+#include <type_traits>
+
 namespace dfl {
 
 // A row's reference moves only when a score exceeds it by this much (log2): the weights stay below 2^8, the output
@@ -21,9 +23,9 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   extern __shared__ __align__(16) unsigned char smem[];
   T* sk = reinterpret_cast<T*>(smem);  // [2] key tiles, [2] value tiles
   T* sv = sk + 2 * E::TILE;
-  unsigned* smask = reinterpret_cast<unsigned*>(sv + 2 * E::TILE);  // [2] one bit a key of the tile: inside and unmasked
-  float* lut = reinterpret_cast<float*>(smask + 4);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h32 = lane >> 5;
+  float* lut = reinterpret_cast<float*>(sv + 2 * E::TILE);
+  const int lane = threadIdx.x & 63, h32 = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
 
   const int G = a.H / a.Hk, nqt = (a.M + WIN_RES - 1) / WIN_RES;
   int x = xcd_order(blockIdx.x, gridDim.x);
@@ -37,8 +39,10 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   const WinVis vis(a);
 
   const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
-  KeyStage<T, DP, FAST> st;
-  st.load(kb, a.ksn, vb, a.vsn, kt.tile(0) * E::BK, a.N, a.d, mask);
+  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
+  lk.issue(sk, kt.tile(0) * E::BK);
+  lv.issue(sv, kt.tile(0) * E::BK);
+  uint64_t bits = row_bits<E::BK>(kt.tile(0) * E::BK, a.N, mask);
   if (REL) build_rel_lut(a, h, lut, nullptr);
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
@@ -50,28 +54,23 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   float m = NEG_BIG, l = 0.f;
   f32x16 acc[E::NT] = {};
 
-  st.store(sk, sv, smask);
-  __syncthreads();
-  for (int it = 0; it < kt.total; ++it) {
-    const int j0 = kt.tile(it) * E::BK, buf = it & 1;
-    const bool more = it + 1 < kt.total;
-    if (more) st.load(kb, a.ksn, vb, a.vsn, kt.tile(it + 1) * E::BK, a.N, a.d, mask);
-    bool none = true;
+  // One key tile for the wave.  WHOLE: every pair is visible and the table gives them one value, cst: no test and no
+  // branch between the products, so that the weights of one half are formed while the matrix unit works on the other.
+  constexpr uint64_t KEYS = E::BK == 64 ? ~0ull : (1ull << E::BK) - 1;  // all keys of a tile inside and unmasked
+  auto tile = [&](auto whole, int j0, T* tk, T* tv, uint64_t keys, float cst) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    // log2 of the weights: ya y + yc; a table entry per pair goes into y itself
+    f32x16 y[E::NSUB];
+    float ya[E::NSUB], yc[E::NSUB];
 #pragma unroll
-    for (int sub = 0; sub < E::NSUB; ++sub) none &= vis.none(t0, j0 + 32 * sub);
-    if (!none) {
-      T* tk = sk + buf * E::TILE;
-      // log2 of the weights: ya y + yc; a table entry per pair goes into y itself
-      f32x16 y[E::NSUB];
-      float ya[E::NSUB], yc[E::NSUB];
+    for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
+    float mx = NEG_BIG;
 #pragma unroll
-      for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
-      float mx = NEG_BIG;
-#pragma unroll
-      for (int sub = 0; sub < E::NSUB; ++sub) {
-        const int js = j0 + 32 * sub;
-        ya[sub] = sc;
-        yc[sub] = 0.f;
+    for (int sub = 0; sub < E::NSUB; ++sub) {
+      const int js = j0 + 32 * sub;
+      ya[sub] = sc;
+      yc[sub] = WHOLE ? cst : 0.f;
+      if (!WHOLE) {
         if (REL) {
           const int far = rel_far(a.rel, t0, js);
           if (far >= 0) {
@@ -83,7 +82,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             ya[sub] = 1.f;
           }
         }
-        const unsigned bits = smask[2 * buf + sub];
+        const unsigned bits = (unsigned)(keys >> (32 * sub));
         if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
           const unsigned mine = bits >> (4 * h32);
 #pragma unroll
@@ -92,36 +91,57 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             y[sub][r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[sub][r] : -INFINITY;
           }
         }
-        float top = y[sub][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, y[sub][r]);
-        mx = fmaxf(mx, __builtin_fmaf(top, ya[sub], yc[sub]));
       }
-      mx = xor32_pair(mx, true);
-      if (__any(mx > m + WIN_SLACK)) {
-        const float to = fmaxf(mx, m), al = fast_exp2(m - to);
-        m = to;
-        l *= al;
+      float top = y[sub][0];
 #pragma unroll
-        for (int n = 0; n < E::NT; ++n) acc[n] *= al;
-      }
-#pragma unroll
-      for (int sub = 0; sub < E::NSUB; ++sub) {
-        const float c = yc[sub] - m;
-        float s = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          y[sub][r] = fast_exp2(__builtin_fmaf(y[sub][r], ya[sub], c));
-          s += y[sub][r];
-        }
-        l += s;
-        typename E::Prob p;
-        E::to_operand(y[sub], p);
-        E::column_product(sv + buf * E::TILE, 32 * sub, p, acc, lane);
-      }
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, y[sub][r]);
+      mx = fmaxf(mx, __builtin_fmaf(top, ya[sub], yc[sub]));
     }
-    if (more) st.store(sk + (buf ^ 1) * E::TILE, sv + (buf ^ 1) * E::TILE, smask + 2 * (buf ^ 1));
-    __syncthreads();
+    mx = xor32_pair(mx, true);
+    if (__any(mx > m + WIN_SLACK)) {
+      const float to = fmaxf(mx, m), al = fast_exp2(m - to);
+      m = to;
+      l *= al;
+#pragma unroll
+      for (int n = 0; n < E::NT; ++n) acc[n] *= al;
+    }
+#pragma unroll
+    for (int sub = 0; sub < E::NSUB; ++sub) {
+      const float c = yc[sub] - m;
+      float s = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        y[sub][r] = fast_exp2(__builtin_fmaf(y[sub][r], ya[sub], c));
+        s += y[sub][r];
+      }
+      l += s;
+      typename E::Prob p;
+      E::to_operand(y[sub], p);
+      E::column_product(tv, 32 * sub, p, acc, lane);
+    }
+  };
+
+  for (int it = 0; it < kt.total; ++it) {
+    const int j0 = kt.tile(it) * E::BK, buf = it & 1;
+    T *tk = sk + buf * E::TILE, *tv = sv + buf * E::TILE;
+    __syncthreads();  // this tile's loads are done, and the other buffer's products
+    const uint64_t now = bits;
+    if (now != KEYS) {
+      clear_rows<T, DP>(tk, now);
+      clear_rows<T, DP>(tv, now);
+      __syncthreads();
+    }
+    if (it + 1 < kt.total) {
+      const int j1 = kt.tile(it + 1) * E::BK;
+      lk.issue(sk + (buf ^ 1) * E::TILE, j1);
+      lv.issue(sv + (buf ^ 1) * E::TILE, j1);
+      bits = row_bits<E::BK>(j1, a.N, mask);
+    }
+    const int far = REL ? rel_far(a.rel, t0, j0, E::BK) : 0;
+    if ((now == KEYS) & vis.all_near(t0, j0, E::BK) & (far >= 0))
+      tile(std::true_type(), j0, tk, tv, now, REL ? lut[far] : 0.f);
+    else if ((now != 0) & !vis.none(t0, j0, E::BK))
+      tile(std::false_type(), j0, tk, tv, now, 0.f);
   }
   l = xor32_pair(l, false);
   const bool some = row_ok && l > 0.f;
@@ -159,7 +179,7 @@ bool window_fast(const WinArgs& a, bool bf16_in, bool bwd) {
 template <typename T, int DP, bool FAST, bool REL>
 static hipError_t fwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
-  const size_t lds = 4 * E::TILE * sizeof(T) + 16 + (REL ? rel_lut_size(a.rel) * 4 : 0);
+  const size_t lds = 4 * E::TILE * sizeof(T) + (REL ? rel_lut_size(a.rel) * 4 : 0);
   auto kern = window_fwd_kernel<T, DP, FAST, REL>;
   const hipError_t attr = set_lds_limit((const void*)kern, lds);
   if (attr != hipSuccess) return attr;

@@ -40,13 +40,13 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   T* sk = reinterpret_cast<T*>(smem);
   T* sv = sk + E::TILE;
-  unsigned* smask = reinterpret_cast<unsigned*>(sv + E::TILE);
-  float* lut = reinterpret_cast<float*>(smask + 4);
+  float* lut = reinterpret_cast<float*>(sv + E::TILE);
   // sums by bucket, a column for each thread: every address has one writer
   float* hist = lut + (REL ? rel_lut_size(a.rel) : 0);
   const bool tab = REL && a.dtable;
   uint8_t* lutb = reinterpret_cast<uint8_t*>(hist + (tab ? a.rel.buckets() * WIN_NT : 0));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h32 = lane >> 5;
+  const int lane = threadIdx.x & 63, h32 = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
 
   const int G = a.H / a.Hk, nqt = (a.M + WIN_RES - 1) / WIN_RES;
   int x = xcd_order(blockIdx.x, gridDim.x);
@@ -74,8 +74,21 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
 
   const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
   float D = 0.f, f = 1.f;
-  KeyStage<T, DP, FAST> st;
+  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
 
+  uint64_t bits = 0;
+  auto stage = [&](int j0) {
+    __syncthreads();
+    lk.issue(sk, j0);
+    lv.issue(sv, j0);
+    bits = row_bits<E::BK>(j0, a.N, mask);
+    __syncthreads();
+    if (bits != (E::BK == 64 ? ~0ull : (1ull << E::BK) - 1)) {
+      clear_rows<T, DP>(sk, bits);
+      clear_rows<T, DP>(sv, bits);
+      __syncthreads();
+    }
+  };
   // p and dp of one 32 x 32 pair of the staged tile; false where the wave sees nothing of it
   auto pair = [&](int sub, int j0, f32x16& y, f32x16& dp) -> bool {
     const int js = j0 + 32 * sub;
@@ -98,9 +111,9 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, -lse);
     }
-    const unsigned bits = smask[sub];
-    if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
-      const unsigned mine = bits >> (4 * h32);
+    const unsigned keys = (unsigned)(bits >> (32 * sub));
+    if (keys != 0xffffffffu || !vis.all_near(t0, js)) {
+      const unsigned mine = keys >> (4 * h32);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int j = js + acc_row(r, h32);
@@ -116,10 +129,7 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
     float sum = 0.f, sdp = 0.f, top = 0.f;
     for (int it = 0; it < kt.total; ++it) {
       const int j0 = kt.tile(it) * E::BK;
-      __syncthreads();
-      st.load(kb, a.ksn, vb, a.vsn, j0, a.N, a.d, mask);
-      st.store(sk, sv, smask);
-      __syncthreads();
+      stage(j0);
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
         f32x16 p, dp;
@@ -152,10 +162,7 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   float far_past = 0.f, far_next = 0.f;
   for (int it = 0; it < kt.total; ++it) {
     const int j0 = kt.tile(it) * E::BK;
-    __syncthreads();
-    st.load(kb, a.ksn, vb, a.vsn, j0, a.N, a.d, mask);
-      st.store(sk, sv, smask);
-    __syncthreads();
+    stage(j0);
 #pragma unroll
     for (int sub = 0; sub < E::NSUB; ++sub) {
       f32x16 p, dp;
@@ -216,7 +223,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
   T* sg = sq + E::TILE;
   float* srow = reinterpret_cast<float*>(sg + E::TILE);  // [3][BK]: lse, D, factor
   float* lut = srow + 3 * E::BK;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h32 = lane >> 5;
+  const int lane = threadIdx.x & 63, h32 = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
   const int G = a.H / a.Hk, shift = a.N - a.M;
   const WinVis vis(a);
 
@@ -253,7 +261,6 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     ihi = min(a.M, k1 - vis.off + (int)vis.range - shift);
   }
   f32x16 dk[E::NT] = {}, dv[E::NT] = {};
-  RowStage<T, DP, FAST> sq_st, sg_st;
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
     if (REL) {
@@ -263,12 +270,12 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh;
     const size_t row0 = ((size_t)b * a.H + h) * a.M;
     const T* gb = reinterpret_cast<const T*>(a.go) + row0 * a.d;
+    const RowLoader<T, DP, FAST> lq(qb, a.qsn, a.M, a.d), lg(gb, a.d, a.M, a.d);
     for (int i0 = ilo; i0 < ihi; i0 += E::BK) {
       __syncthreads();
-      sq_st.load(qb, a.qsn, i0, a.M, a.d, mask ? mask + shift : nullptr);
-      sg_st.load(gb, a.d, i0, a.M, a.d, mask ? mask + shift : nullptr);
-      sq_st.store(sq);
-      sg_st.store(sg);
+      lq.issue(sq, i0);
+      lg.issue(sg, i0);
+      const uint64_t bits = row_bits<E::BK>(i0, a.M, mask ? mask + shift : nullptr);
       if ((int)threadIdx.x < E::BK) {
         const int i = i0 + threadIdx.x;
         const bool ok = i < ihi && (!mask || mask[shift + i] != 0.f);
@@ -277,6 +284,11 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
         srow[2 * E::BK + threadIdx.x] = ok ? a.rowd[2 * (row0 + i) + 1] : 0.f;
       }
       __syncthreads();
+      if (bits != (E::BK == 64 ? ~0ull : (1ull << E::BK) - 1)) {
+        clear_rows<T, DP>(sq, bits);
+        clear_rows<T, DP>(sg, bits);
+        __syncthreads();
+      }
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
         const int t0 = i0 + 32 * sub + shift;
@@ -413,7 +425,7 @@ static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
   const size_t tiles = 2 * E::TILE * sizeof(T), lutn = REL ? rel_lut_size(a.rel) : 0;
   const bool tab = REL && a.dtable;
-  const size_t lq = tiles + 16 + lutn * 4 + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0);
+  const size_t lq = tiles + lutn * 4 + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0);
   // the first tokens' reduction takes 64 DP floats over the tiles
   const size_t lkv = std::max(tiles + 3 * E::BK * 4 + lutn * 4, (size_t)64 * DP * 4);
   auto kq = window_bwd_q_kernel<T, DP, FAST, REL>;

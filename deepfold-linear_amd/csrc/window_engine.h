@@ -167,13 +167,15 @@ struct WinVis {
   // (combined with & and |: a chain of branches around single elements of an accumulator loses some of the writes
   // to them in this compiler)
   __device__ __forceinline__ bool sees(int t, int j) const { return near(t, j) | first(t, j); }
-  // all of the 32 x 32 pairs with queries from t0 and keys from j0 on / none of them
-  __device__ __forceinline__ bool all_near(int t0, int j0) const { return near(t0, j0 + 31) && near(t0 + 31, j0); }
-  __device__ __forceinline__ bool none_near(int t0, int j0) const {
-    return t0 + 31 - j0 + off < 0 || t0 - (j0 + 31) + off >= (int)range;
+  // all / none of the pairs of 32 queries from t0 and n keys from j0 on
+  __device__ __forceinline__ bool all_near(int t0, int j0, int n = 32) const {
+    return near(t0, j0 + n - 1) & near(t0 + 31, j0);
   }
-  __device__ __forceinline__ bool none(int t0, int j0) const {
-    return none_near(t0, j0) & !((j0 < n_sink) & ((causal == 0) | (j0 <= t0 + 31)));
+  __device__ __forceinline__ bool none_near(int t0, int j0, int n = 32) const {
+    return (t0 + 31 - j0 + off < 0) | (t0 - (j0 + n - 1) + off >= (int)range);
+  }
+  __device__ __forceinline__ bool none(int t0, int j0, int n = 32) const {
+    return none_near(t0, j0, n) & !((j0 < n_sink) & ((causal == 0) | (j0 <= t0 + 31)));
   }
 };
 
@@ -202,10 +204,10 @@ __device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, float* lu
     if (bucket) bucket[x] = (uint8_t)b;
   }
 }
-// Where every distance t - j of a 32 x 32 tile lies beyond the table's range: the index of its one value, else -1.
-__device__ __forceinline__ int rel_far(const RelSpec& r, int t0, int j0) {
+// Where every distance t - j of 32 queries and n keys lies beyond the table's range: the index of its one value, else -1.
+__device__ __forceinline__ int rel_far(const RelSpec& r, int t0, int j0, int n = 32) {
   const int dist = r.dist();
-  if (t0 - (j0 + 31) >= dist) return rel_lut_base(r) + dist;
+  if (t0 - (j0 + n - 1) >= dist) return rel_lut_base(r) + dist;
   if (r.both && j0 - (t0 + 31) > dist) return rel_lut_base(r) - dist - 1;
   return -1;
 }

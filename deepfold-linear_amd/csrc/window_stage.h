@@ -20,81 +20,60 @@ struct KeyTiles {
   __device__ __forceinline__ int tile(int it) const { return it < pre ? it : b0 + it - pre; }
 };
 
-// Rows j0 .. j0 + BK - 1 of one operand on their way to LDS: issued as loads into registers before the product of
-// the tile in front, written after it.  Rows outside [0, N) or masked, and columns from d on, are zero there (what lies
-// in masked rows may be NaN).  A tile inside [0, N) without mask and of full width needs neither clamps nor selects.
-template <typename T, int DP, bool FAST> struct RowStage {
+// Brings tiles of BK rows of one operand to LDS.  FAST: asynchronous 16-byte loads straight into LDS (no registers
+// between, in flight until the next barrier); the swizzle is on the global side, each lane fetching the chunk that
+// belongs where its 16 bytes land.  Rows from N on repeat the last one and chunks from column d on the row's first,
+// so that every address is inside: clear_rows() zeroes such rows before use, and columns from d on meet zero columns
+// of the resident operand or end in columns that are not written.  Else: element loads, zeros outside.
+template <typename T, int DP, bool FAST> struct RowLoader {
   using E = WinEng<T, DP>;
   static constexpr int PER = E::BK * E::NCH / WIN_NT;  // chunks of a thread
   static constexpr int STEP = WIN_NT / E::NCH;         // rows between them
-  u32x4 v[PER];
-  unsigned ok;  // a bit a chunk: keep it
-  __device__ __forceinline__ void load(const T* base, long long stride, int j0, int N, int d, const float* mask) {
-    const int r = threadIdx.x / E::NCH, c = threadIdx.x % E::NCH;
-    if (FAST && !mask && j0 + E::BK <= N && d == DP) {
-      const T* p = base + j0 * stride + (r * stride + c * E::VEC);
+  const T* base;
+  long long stride;
+  int N, d;
+  __device__ __forceinline__ RowLoader(const T* b, long long s, int n, int dim) : base(b), stride(s), N(n), d(dim) {}
+  __device__ __forceinline__ void issue(T* tile, int j0) const {
+    const int r = threadIdx.x / E::NCH, pos = threadIdx.x % E::NCH;
+    if constexpr (FAST) {
+      typedef __attribute__((address_space(3))) unsigned* lptr;
+      typedef const __attribute__((address_space(1))) unsigned* gptr;
+      T* to = tile + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u) * E::VEC;
+      const bool inside = j0 + E::BK <= N;
+      const T* p = base + j0 * stride;
 #pragma unroll
-      for (int n = 0; n < PER; ++n) v[n] = *reinterpret_cast<const u32x4*>(p + n * STEP * stride);
-      ok = ~0u;
-      return;
-    }
-    unsigned bits = 0;
+      for (int n = 0; n < PER; ++n) {
+        const int row = r + n * STEP, c = E::swz(row, pos) * E::VEC;
+        const long long at = inside ? row : min(row, N - 1 - j0);
+        __builtin_amdgcn_global_load_lds((gptr)(p + at * stride + (c < d ? c : 0)), (lptr)(to + n * WIN_NT * E::VEC), 16, 0,
+                                         0);
+      }
+    } else {
 #pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int j = j0 + r + n * STEP, at = min(j, N - 1);
-      const T* row = base + at * stride;
-      if (FAST) {  // a chunk behind the row's end reads the row's first one
-        v[n] = *reinterpret_cast<const u32x4*>(row + (c * E::VEC < d ? c * E::VEC : 0));
-        bits |= (unsigned)((j < N) & (c * E::VEC < d)) << n;
-      } else {
-        v[n] = E::template load<false>(row, c, d);
-        bits |= (unsigned)(j < N) << n;
+      for (int n = 0; n < PER; ++n) {
+        const int row = r + n * STEP, j = j0 + row;
+        *E::chunk(tile, row, pos) = E::template load<false>(j < N ? base + j * stride : nullptr, pos, d);
       }
     }
-    if (mask) {
-#pragma unroll
-      for (int n = 0; n < PER; ++n) bits &= ~((unsigned)(mask[min(j0 + r + n * STEP, N - 1)] == 0.f) << n);
-    }
-    ok = bits;
-  }
-  __device__ __forceinline__ void store(T* tile) {
-    const int r = threadIdx.x / E::NCH, c = threadIdx.x % E::NCH;
-    if (__any(ok != ~0u)) {
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int n = 0; n < PER; ++n) v[n] = (ok >> n) & 1u ? v[n] : zero;
-    }
-#pragma unroll
-    for (int n = 0; n < PER; ++n) *E::chunk(tile, r + n * STEP, c) = v[n];
   }
 };
 
-// One key tile: K, V and the bits of its keys that are inside and unmasked (the first wave's).
-template <typename T, int DP, bool FAST> struct KeyStage {
+// Zeroes the rows of a staged tile whose bit is clear: outside the sequence or masked, where NaN may lie.
+template <typename T, int DP> __device__ __forceinline__ void clear_rows(T* tile, uint64_t bits) {
   using E = WinEng<T, DP>;
-  RowStage<T, DP, FAST> k, v;
-  uint64_t bits;
-  __device__ __forceinline__ void load(const T* kb, long long ksn, const T* vb, long long vsn, int j0, int N, int d,
-                                       const float* mask) {
-    k.load(kb, ksn, j0, N, d, mask);
-    v.load(vb, vsn, j0, N, d, mask);
-    if (mask || j0 + E::BK > N) {
-      const int lane = threadIdx.x & 63, j = j0 + lane;
-      const bool in = (lane < E::BK) & (j < N);
-      bits = __ballot(in && (!mask || mask[in ? j : 0] != 0.f));
-    } else {
-      bits = ~0ull;
-    }
-  }
-  __device__ __forceinline__ void store(T* sk, T* sv, unsigned* smask) {
-    k.store(sk);
-    v.store(sv);
-    if (threadIdx.x == 0) {
-      smask[0] = (unsigned)bits;
-      smask[1] = (unsigned)(bits >> 32);
-    }
-  }
-};
+  const u32x4 zero = {0u, 0u, 0u, 0u};
+  for (int e = threadIdx.x; e < E::BK * E::NCH; e += WIN_NT)
+    if (!((bits >> (e / E::NCH)) & 1u)) *reinterpret_cast<u32x4*>(tile + e * E::VEC) = zero;
+}
+
+// One bit for each of the BK rows from j0 on: inside [0, N) and unmasked.  The same in every wave.
+template <int BK> __device__ __forceinline__ uint64_t row_bits(int j0, int N, const float* mask) {
+  constexpr uint64_t all = BK == 64 ? ~0ull : (1ull << BK) - 1;
+  if (!mask && j0 + BK <= N) return all;
+  const int lane = threadIdx.x & 63, j = j0 + lane;
+  const bool in = (lane < BK) & (j < N);
+  return __ballot(in && (!mask || mask[in ? j : 0] != 0.f));
+}
 
 // Four consecutive columns c .. c + 3 of a result row of d columns.
 template <typename T, bool FAST> __device__ __forceinline__ void store4(T* row, int c, int d, f32x4 x) {
