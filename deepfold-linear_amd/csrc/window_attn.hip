@@ -9,8 +9,6 @@
 #include "window_engine.h"
 #include "window_stage.h"
 
-#include <type_traits>
-
 namespace dfl {
 
 // A row's reference moves only when a score exceeds it by this much (log2): the weights stay below 2^8, the output
@@ -54,27 +52,41 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   float m = NEG_BIG, l = 0.f;
   f32x16 acc[E::NT] = {};
 
-  // One key tile for the wave.  WHOLE: every pair is visible and the table gives them one value, cst: no test and no
-  // branch between the products, so that the weights of one half are formed while the matrix unit works on the other.
   constexpr uint64_t KEYS = E::BK == 64 ? ~0ull : (1ull << E::BK) - 1;  // all keys of a tile inside and unmasked
-  auto tile = [&](auto whole, int j0, T* tk, T* tv, uint64_t keys, float cst) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    // log2 of the weights: ya y + yc; a table entry per pair goes into y itself
+  for (int it = 0; it < kt.total; ++it) {
+    const int j0 = kt.tile(it) * E::BK, buf = it & 1;
+    T *tk = sk + buf * E::TILE, *tv = sv + buf * E::TILE;
+    __syncthreads();  // this tile's loads are done, and the other buffer's products
+    const uint64_t now = bits;
+    if (now != KEYS) {
+      clear_rows<T, DP>(tk, now);
+      clear_rows<T, DP>(tv, now);
+      __syncthreads();
+    }
+    if (it + 1 < kt.total) {
+      const int j1 = kt.tile(it + 1) * E::BK;
+      lk.issue(sk + (buf ^ 1) * E::TILE, j1);
+      lv.issue(sv + (buf ^ 1) * E::TILE, j1);
+      bits = row_bits<E::BK>(j1, a.N, mask);
+    }
+    if ((now == 0) | vis.none(t0, j0, E::BK)) continue;
     f32x16 y[E::NSUB];
-    float ya[E::NSUB], yc[E::NSUB];
 #pragma unroll
     for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
-    float mx = NEG_BIG;
+    // log2 of the weights: ya y + yc.  A tile all of whose pairs are visible and get one table value needs no test a
+    // pair; else a table value a pair goes into y itself, and what is not visible becomes -inf.
+    float ya[E::NSUB], yc[E::NSUB];
+    const int far = REL ? rel_far(a.rel, t0, j0, E::BK) : 0;
 #pragma unroll
-    for (int sub = 0; sub < E::NSUB; ++sub) {
-      const int js = j0 + 32 * sub;
-      ya[sub] = sc;
-      yc[sub] = WHOLE ? cst : 0.f;
-      if (!WHOLE) {
-        if (REL) {
-          const int far = rel_far(a.rel, t0, js);
-          if (far >= 0) {
-            yc[sub] = lut[far];
+    for (int sub = 0; sub < E::NSUB; ++sub) ya[sub] = sc, yc[sub] = REL && far >= 0 ? lut[far] : 0.f;
+    if ((now != KEYS) | !vis.all_near(t0, j0, E::BK) | (far < 0)) {
+#pragma unroll
+      for (int sub = 0; sub < E::NSUB; ++sub) {
+        const int js = j0 + 32 * sub;
+        if (REL && far < 0) {
+          const int one = rel_far(a.rel, t0, js);
+          if (one >= 0) {
+            yc[sub] = lut[one];
           } else {
             const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
 #pragma unroll
@@ -82,9 +94,9 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             ya[sub] = 1.f;
           }
         }
-        const unsigned bits = (unsigned)(keys >> (32 * sub));
-        if (bits != 0xffffffffu || !vis.all_near(t0, js)) {
-          const unsigned mine = bits >> (4 * h32);
+        const unsigned keys = (unsigned)(now >> (32 * sub));
+        if (keys != 0xffffffffu || !vis.all_near(t0, js)) {
+          const unsigned mine = keys >> (4 * h32);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int j = js + acc_row(r, h32);
@@ -92,6 +104,10 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
           }
         }
       }
+    }
+    float mx = NEG_BIG;
+#pragma unroll
+    for (int sub = 0; sub < E::NSUB; ++sub) {
       float top = y[sub][0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, y[sub][r]);
@@ -119,29 +135,6 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       E::to_operand(y[sub], p);
       E::column_product(tv, 32 * sub, p, acc, lane);
     }
-  };
-
-  for (int it = 0; it < kt.total; ++it) {
-    const int j0 = kt.tile(it) * E::BK, buf = it & 1;
-    T *tk = sk + buf * E::TILE, *tv = sv + buf * E::TILE;
-    __syncthreads();  // this tile's loads are done, and the other buffer's products
-    const uint64_t now = bits;
-    if (now != KEYS) {
-      clear_rows<T, DP>(tk, now);
-      clear_rows<T, DP>(tv, now);
-      __syncthreads();
-    }
-    if (it + 1 < kt.total) {
-      const int j1 = kt.tile(it + 1) * E::BK;
-      lk.issue(sk + (buf ^ 1) * E::TILE, j1);
-      lv.issue(sv + (buf ^ 1) * E::TILE, j1);
-      bits = row_bits<E::BK>(j1, a.N, mask);
-    }
-    const int far = REL ? rel_far(a.rel, t0, j0, E::BK) : 0;
-    if ((now == KEYS) & vis.all_near(t0, j0, E::BK) & (far >= 0))
-      tile(std::true_type(), j0, tk, tv, now, REL ? lut[far] : 0.f);
-    else if ((now != 0) & !vis.none(t0, j0, E::BK))
-      tile(std::false_type(), j0, tk, tv, now, 0.f);
   }
   l = xor32_pair(l, false);
   const bool some = row_ok && l > 0.f;

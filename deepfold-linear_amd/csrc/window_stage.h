@@ -30,23 +30,35 @@ template <typename T, int DP, bool FAST> struct RowLoader {
   static constexpr int PER = E::BK * E::NCH / WIN_NT;  // chunks of a thread
   static constexpr int STEP = WIN_NT / E::NCH;         // rows between them
   const T* base;
+  const T* mine;  // this thread's chunk of row 0 .. of the tile at row 0
   long long stride;
   int N, d;
-  __device__ __forceinline__ RowLoader(const T* b, long long s, int n, int dim) : base(b), stride(s), N(n), d(dim) {}
+  __device__ __forceinline__ static int column(int row, int pos, int d) {
+    const int c = E::swz(row, pos) * E::VEC;
+    return c < d ? c : 0;
+  }
+  __device__ __forceinline__ RowLoader(const T* b, long long s, int n, int dim) : base(b), stride(s), N(n), d(dim) {
+    const int r = threadIdx.x / E::NCH;
+    mine = base + r * stride + column(r, threadIdx.x % E::NCH, d);
+  }
   __device__ __forceinline__ void issue(T* tile, int j0) const {
     const int r = threadIdx.x / E::NCH, pos = threadIdx.x % E::NCH;
     if constexpr (FAST) {
       typedef __attribute__((address_space(3))) unsigned* lptr;
       typedef const __attribute__((address_space(1))) unsigned* gptr;
       T* to = tile + __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u) * E::VEC;
-      const bool inside = j0 + E::BK <= N;
-      const T* p = base + j0 * stride;
+      if (STEP % 16 == 0 && j0 + E::BK <= N) {  // one column for all of the thread's rows
 #pragma unroll
-      for (int n = 0; n < PER; ++n) {
-        const int row = r + n * STEP, c = E::swz(row, pos) * E::VEC;
-        const long long at = inside ? row : min(row, N - 1 - j0);
-        __builtin_amdgcn_global_load_lds((gptr)(p + at * stride + (c < d ? c : 0)), (lptr)(to + n * WIN_NT * E::VEC), 16, 0,
-                                         0);
+        for (int n = 0; n < PER; ++n)
+          __builtin_amdgcn_global_load_lds((gptr)(mine + (j0 + n * STEP) * stride), (lptr)(to + n * WIN_NT * E::VEC), 16, 0,
+                                           0);
+      } else {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+          const int row = r + n * STEP;
+          __builtin_amdgcn_global_load_lds((gptr)(base + min(j0 + row, N - 1) * stride + column(row, pos, d)),
+                                           (lptr)(to + n * WIN_NT * E::VEC), 16, 0, 0);
+        }
       }
     } else {
 #pragma unroll
