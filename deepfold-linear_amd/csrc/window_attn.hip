@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
   lk.issue(sk, kt.tile(0) * E::BK);
   lv.issue(sv, kt.tile(0) * E::BK);
-  uint64_t bits = row_bits<E::BK>(kt.tile(0) * E::BK, a.N, mask);
+  RowBits<E::BK> rb(mask, a.N);
+  rb.fetch(kt.tile(0) * E::BK);
   if (REL) build_rel_lut(a, h, lut, nullptr);
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
@@ -52,12 +53,13 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   float m = NEG_BIG, l = 0.f;
   f32x16 acc[E::NT] = {};
 
-  constexpr uint64_t KEYS = E::BK == 64 ? ~0ull : (1ull << E::BK) - 1;  // all keys of a tile inside and unmasked
+  constexpr uint64_t KEYS = RowBits<E::BK>::ALL;  // all keys of a tile inside and unmasked
   for (int it = 0; it < kt.total; ++it) {
     const int j0 = kt.tile(it) * E::BK, buf = it & 1;
     T *tk = sk + buf * E::TILE, *tv = sv + buf * E::TILE;
-    __syncthreads();  // this tile's loads are done, and the other buffer's products
-    const uint64_t now = bits;
+    lds_loads_done();
+    __syncthreads();  // this tile is there, and the other buffer's products are done
+    const uint64_t now = rb.get();
     if (now != KEYS) {
       clear_rows<T, DP>(tk, now);
       clear_rows<T, DP>(tv, now);
@@ -67,7 +69,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       const int j1 = kt.tile(it + 1) * E::BK;
       lk.issue(sk + (buf ^ 1) * E::TILE, j1);
       lv.issue(sv + (buf ^ 1) * E::TILE, j1);
-      bits = row_bits<E::BK>(j1, a.N, mask);
+      rb.fetch(j1);
     }
     if ((now == 0) | vis.none(t0, j0, E::BK)) continue;
     f32x16 y[E::NSUB];

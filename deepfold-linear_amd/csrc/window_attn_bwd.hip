@@ -81,9 +81,12 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
     __syncthreads();
     lk.issue(sk, j0);
     lv.issue(sv, j0);
-    bits = row_bits<E::BK>(j0, a.N, mask);
+    RowBits<E::BK> rb(mask, a.N);
+    rb.fetch(j0);
+    lds_loads_done();
     __syncthreads();
-    if (bits != (E::BK == 64 ? ~0ull : (1ull << E::BK) - 1)) {
+    bits = rb.get();
+    if (bits != RowBits<E::BK>::ALL) {
       clear_rows<T, DP>(sk, bits);
       clear_rows<T, DP>(sv, bits);
       __syncthreads();
@@ -275,7 +278,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
       __syncthreads();
       lq.issue(sq, i0);
       lg.issue(sg, i0);
-      const uint64_t bits = row_bits<E::BK>(i0, a.M, mask ? mask + shift : nullptr);
+      RowBits<E::BK> rb(mask ? mask + shift : nullptr, a.M);
+      rb.fetch(i0);
       if ((int)threadIdx.x < E::BK) {
         const int i = i0 + threadIdx.x;
         const bool ok = i < ihi && (!mask || mask[shift + i] != 0.f);
@@ -283,8 +287,10 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
         srow[E::BK + threadIdx.x] = ok ? a.rowd[2 * (row0 + i)] : 0.f;
         srow[2 * E::BK + threadIdx.x] = ok ? a.rowd[2 * (row0 + i) + 1] : 0.f;
       }
+      lds_loads_done();
       __syncthreads();
-      if (bits != (E::BK == 64 ? ~0ull : (1ull << E::BK) - 1)) {
+      const uint64_t bits = rb.get();
+      if (bits != RowBits<E::BK>::ALL) {
         clear_rows<T, DP>(sq, bits);
         clear_rows<T, DP>(sg, bits);
         __syncthreads();

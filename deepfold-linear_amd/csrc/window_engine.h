@@ -89,6 +89,15 @@ template <typename T, int DP> struct WinEng {
     f32x16 c = {};
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) c = step(*chunk(tile, r0 + (lane & 31), 2 * s + (lane >> 5)), f.v[s], c);
+    // a few LDS reads ahead of the products (the scheduler would rather save their registers and wait for each)
+    constexpr int AHEAD = STEPS < 4 ? STEPS : 4, PER = sizeof(T) == 2 ? 1 : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int s = AHEAD; s < STEPS; ++s) {
+      __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * PER, 0);
     return c;
   }
   // B operands of a column product
