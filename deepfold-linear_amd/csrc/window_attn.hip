@@ -22,6 +22,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   T* sk = reinterpret_cast<T*>(smem);  // [2] key tiles, [2] value tiles
   T* sv = sk + 2 * E::TILE;
   float* lut = reinterpret_cast<float*>(sv + 2 * E::TILE);
+  int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
 
@@ -42,7 +43,11 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   lv.issue(sv, kt.tile(0) * E::BK);
   RowBits<E::BK> rb(mask, a.N);
   rb.fetch(kt.tile(0) * E::BK);
-  if (REL) build_rel_lut(a, h, lut, nullptr);
+  if (REL) {
+    stage_edges(a.rel, edge);
+    __syncthreads();
+    build_rel_lut(a, h, edge, lut, nullptr);
+  }
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
   const bool row_ok = i < a.M && (!mask || mask[t] != 0.f);
@@ -174,7 +179,7 @@ bool window_fast(const WinArgs& a, bool bf16_in, bool bwd) {
 template <typename T, int DP, bool FAST, bool REL>
 static hipError_t fwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
-  const size_t lds = 4 * E::TILE * sizeof(T) + (REL ? rel_lut_size(a.rel) * 4 : 0);
+  const size_t lds = 4 * E::TILE * sizeof(T) + (REL ? (rel_lut_size(a.rel) + REL_EDGES) * 4 : 0);
   auto kern = window_fwd_kernel<T, DP, FAST, REL>;
   const hipError_t attr = set_lds_limit((const void*)kern, lds);
   if (attr != hipSuccess) return attr;

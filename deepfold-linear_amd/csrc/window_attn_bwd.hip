@@ -35,14 +35,15 @@ __device__ __forceinline__ float frag_dot(const typename WinEng<T, DP>::Frag& x,
 }
 
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
+__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) window_bwd_q_kernel(WinArgs a, int n_buf) {
   using E = WinEng<T, DP>;
   extern __shared__ __align__(16) unsigned char smem[];
-  T* sk = reinterpret_cast<T*>(smem);
-  T* sv = sk + E::TILE;
-  float* lut = reinterpret_cast<float*>(sv + E::TILE);
+  T* sk = reinterpret_cast<T*>(smem);  // [n_buf] key tiles, [n_buf] value tiles
+  T* sv = sk + n_buf * E::TILE;
+  float* lut = reinterpret_cast<float*>(sv + n_buf * E::TILE);
+  int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
   // sums by bucket, a column for each thread: every address has one writer
-  float* hist = lut + (REL ? rel_lut_size(a.rel) : 0);
+  float* hist = reinterpret_cast<float*>(edge + (REL ? REL_EDGES : 0));
   const bool tab = REL && a.dtable;
   uint8_t* lutb = reinterpret_cast<uint8_t*>(hist + (tab ? a.rel.buckets() * WIN_NT : 0));
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
@@ -58,7 +59,23 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   const T* vb = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh;
   const float* mask = a.mask ? a.mask + (size_t)b * a.N : nullptr;
   const WinVis vis(a);
-  if (REL) build_rel_lut(a, h, lut, tab ? lutb : nullptr);
+  const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
+  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
+  RowBits<E::BK> rb(mask, a.N);
+  constexpr uint64_t KEYS = RowBits<E::BK>::ALL;
+  // Two buffers, the next tile on its way during this one's products; one where a large table's sums take their room.
+  auto issue = [&](int it, int buf) {
+    const int j0 = kt.tile(it) * E::BK;
+    lk.issue(sk + buf * E::TILE, j0);
+    lv.issue(sv + buf * E::TILE, j0);
+    rb.fetch(j0);
+  };
+  if (n_buf > 1) issue(0, 0);
+  if (REL) {
+    stage_edges(a.rel, edge);
+    __syncthreads();
+    build_rel_lut(a, h, edge, lut, tab ? lutb : nullptr);
+  }
   if (tab)
     for (int n = 0; n < a.rel.buckets(); ++n) hist[n * WIN_NT + threadIdx.x] = 0.f;
 
@@ -71,90 +88,84 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   E::template load_frag<FAST>(gf, row_ok ? reinterpret_cast<const T*>(a.go) + row * a.d : nullptr, a.d, lane);
   const float sc = a.scale * LOG2E;
   const float lse = row_ok ? a.lse[row] : LSE_EMPTY;
-
-  const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
+  const bool exact = kt.total * E::BK <= WIN_EXACT_KEYS;
   float D = 0.f, f = 1.f;
-  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
+  if (!exact) {
+    typename E::Frag of;
+    E::template load_frag<FAST>(of, row_ok ? reinterpret_cast<const T*>(a.o) + row * a.d : nullptr, a.d, lane);
+    D = frag_dot<T, DP>(of, gf);
+  }
 
-  uint64_t bits = 0;
-  auto stage = [&](int j0) {
-    __syncthreads();
-    lk.issue(sk, j0);
-    lv.issue(sv, j0);
-    RowBits<E::BK> rb(mask, a.N);
-    rb.fetch(j0);
-    lds_loads_done();
-    __syncthreads();
-    bits = rb.get();
-    if (bits != RowBits<E::BK>::ALL) {
-      clear_rows<T, DP>(sk, bits);
-      clear_rows<T, DP>(sv, bits);
-      __syncthreads();
-    }
-  };
-  // p and dp of one 32 x 32 pair of the staged tile; false where the wave sees nothing of it
-  auto pair = [&](int sub, int j0, f32x16& y, f32x16& dp) -> bool {
-    const int js = j0 + 32 * sub;
-    const bool sinks = js < vis.n_sink && (!vis.causal || js <= t0 + 31);
-    if (vis.none_near(t0, js) && !sinks) return false;
-    y = E::row_product(sk, 32 * sub, qf, lane);
-    dp = E::row_product(sv, 32 * sub, gf, lane);
-    if (REL) {
-      const int far = rel_far(a.rel, t0, js);
-      if (far >= 0) {
-        const float c = lut[far] - lse;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, c);
-      } else {
-        const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, p[-acc_row(r, 0)]) - lse;
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, -lse);
-    }
-    const unsigned keys = (unsigned)(bits >> (32 * sub));
-    if (keys != 0xffffffffu || !vis.all_near(t0, js)) {
-      const unsigned mine = keys >> (4 * h32);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = js + acc_row(r, h32);
-        y[r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[r] : -INFINITY;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] = fast_exp2(y[r]);
-    return true;
-  };
-
-  if (kt.total * E::BK <= WIN_EXACT_KEYS) {
-    float sum = 0.f, sdp = 0.f, top = 0.f;
-    for (int it = 0; it < kt.total; ++it) {
+  // body(p, dp, js) for every 32 x 32 pair that the wave sees something of; `buf`: where the first tile is or goes
+  auto sweep = [&](auto body, int& buf, bool again) {
+    for (int it = 0; it < kt.total; ++it, buf ^= n_buf - 1) {
       const int j0 = kt.tile(it) * E::BK;
-      stage(j0);
+      T *tk = sk + buf * E::TILE, *tv = sv + buf * E::TILE;
+      if (n_buf == 1) {
+        __syncthreads();
+        issue(it, 0);
+      }
+      lds_loads_done();
+      __syncthreads();  // this tile is there, and the other buffer's products are done
+      const uint64_t now = rb.get();
+      if (now != KEYS) {
+        clear_rows<T, DP>(tk, now);
+        clear_rows<T, DP>(tv, now);
+        __syncthreads();
+      }
+      if (n_buf > 1 && (it + 1 < kt.total || again)) issue(it + 1 < kt.total ? it + 1 : 0, buf ^ 1);
+      if (now == 0) continue;
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
-        f32x16 p, dp;
-        if (!pair(sub, j0, p, dp)) continue;
+        const int js = j0 + 32 * sub;
+        if (vis.none(t0, js)) continue;
+        f32x16 y = E::row_product(tk, 32 * sub, qf, lane);
+        f32x16 dp = E::row_product(tv, 32 * sub, gf, lane);
+        const int far = REL ? rel_far(a.rel, t0, js) : 0;
+        if (REL && far < 0) {
+          const float* p = lut + rel_lut_base(a.rel) + t - js - 4 * h32;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sum += p[r];
-          sdp = __builtin_fmaf(p[r], dp[r], sdp);
-          top = fmaxf(top, p[r]);
+          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, p[-acc_row(r, 0)]) - lse;
+        } else {
+          const float c = REL ? lut[far] - lse : -lse;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(y[r], sc, c);
         }
+        const unsigned keys = (unsigned)(now >> (32 * sub));
+        if (keys != 0xffffffffu || !vis.all_near(t0, js)) {
+          const unsigned mine = keys >> (4 * h32);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = js + acc_row(r, h32);
+            y[r] = (((mine >> acc_row(r, 0)) & 1u) != 0u) & vis.sees(t, j) ? y[r] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] = fast_exp2(y[r]);
+        body(y, dp, js, far, tk, sub);
       }
     }
+  };
+
+  int buf = 0;
+  if (exact) {
+    float sum = 0.f, sdp = 0.f, top = 0.f;
+    sweep(
+        [&](const f32x16& p, const f32x16& dp, int, int, T*, int) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            sum += p[r];
+            sdp = __builtin_fmaf(p[r], dp[r], sdp);
+            top = fmaxf(top, p[r]);
+          }
+        },
+        buf, true);
     sum = xor32_pair(sum, false);
     sdp = xor32_pair(sdp, false);
     top = xor32_pair(top, true);
     // a row that one key takes whole has no score gradient; its rounding errors are none either
     f = (sum > 0.f && top == sum) ? 0.f : 1.f;
     D = (sum > 0.f && f != 0.f) ? sdp / sum : 0.f;
-  } else {
-    typename E::Frag of;
-    E::template load_frag<FAST>(of, row_ok ? reinterpret_cast<const T*>(a.o) + row * a.d : nullptr, a.d, lane);
-    D = frag_dot<T, DP>(of, gf);
   }
   if (i < a.M && h32 == 0) {
     a.rowd[2 * row] = D;
@@ -163,44 +174,40 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
 
   f32x16 acc[E::NT] = {};
   float far_past = 0.f, far_next = 0.f;
-  for (int it = 0; it < kt.total; ++it) {
-    const int j0 = kt.tile(it) * E::BK;
-    stage(j0);
+  sweep(
+      [&](f32x16& p, const f32x16& dp, int js, int far, T* tk, int sub) {
 #pragma unroll
-    for (int sub = 0; sub < E::NSUB; ++sub) {
-      f32x16 p, dp;
-      if (!pair(sub, j0, p, dp)) continue;
+        for (int r = 0; r < 16; ++r) p[r] *= __builtin_fmaf(dp[r], f, -D);
+        if (tab) {
+          if (far >= 0) {
+            float s = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] *= __builtin_fmaf(dp[r], f, -D);
-      if (tab) {
-        const int js = j0 + 32 * sub, far = rel_far(a.rel, t0, js);
-        if (far >= 0) {
-          float s = 0.f;
+            for (int r = 0; r < 16; ++r) s += p[r];
+            if (far > rel_lut_base(a.rel)) far_past += s;
+            else far_next += s;
+          } else {
+            const uint8_t* lb = lutb + rel_lut_base(a.rel) + t - js - 4 * h32;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s += p[r];
-          if (far > rel_lut_base(a.rel)) far_past += s;
-          else far_next += s;
-        } else {
-          const uint8_t* lb = lutb + rel_lut_base(a.rel) + t - js - 4 * h32;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            __hip_atomic_fetch_add(hist + lb[-acc_row(r, 0)] * WIN_NT + threadIdx.x, p[r], __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int r = 0; r < 16; ++r)
+              __hip_atomic_fetch_add(hist + lb[-acc_row(r, 0)] * WIN_NT + threadIdx.x, p[r], __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+          }
         }
-      }
-      typename E::Prob o;
-      E::to_operand(p, o);
-      E::column_product(sk, 32 * sub, o, acc, lane);
-    }
-  }
+        typename E::Prob o;
+        E::to_operand(p, o);
+        E::column_product(tk, 32 * sub, o, acc, lane);
+      },
+      buf, false);
   if (i < a.M) {
     T* dq = reinterpret_cast<T*>(a.dq) + row * a.d;
 #pragma unroll
     for (int n = 0; n < E::NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int c = 32 * n + acc_row(r, h32);
-        if (c < a.d) dq[c] = from_f32<T>(acc[n][r] * a.scale);
+      for (int r = 0; r < 16; r += 4) {
+        f32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = acc[n][r + e] * a.scale;
+        store4<T, FAST>(dq, 32 * n + acc_row(r, h32), a.d, w);
       }
   }
   if (tab) {
@@ -217,18 +224,25 @@ __global__ void __launch_bounds__(WIN_NT) window_bwd_q_kernel(WinArgs a) {
   }
 }
 
-// Key-resident pass.  SINK: 32 of the first tokens' keys against a chunk of the queries outside their band, a
-// wave 32 of the staged queries at a time; else 128 keys against the queries of their band, a wave 32 of the keys.
+// Key-resident pass: 64 keys of a (sample, key head) against the queries of their band, 64 staged queries at a time;
+// a wave has 32 of the keys (wave & 1) and 32 of the staged queries (wave >> 1), so that twice as many workgroups share
+// the keys as with 32 keys a wave each, and the two halves of a key's sum meet in LDS at the end.
+// SINK: 32 of the first tokens' keys against a chunk of the queries outside their band.
+constexpr int WIN_KEYS = 64;
+
 template <typename T, int DP, bool FAST, bool REL, bool SINK>
 __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* smem) {
   using E = WinEng<T, DP>;
-  T* sq = reinterpret_cast<T*>(smem);
-  T* sg = sq + E::TILE;
-  float* srow = reinterpret_cast<float*>(sg + E::TILE);  // [3][BK]: lse, D, factor
-  float* lut = srow + 3 * E::BK;
+  constexpr int NB = 64 / E::BK;  // LDS tiles of the engine's size in 64 rows
+  constexpr int TILE = 64 * DP;
+  T* sq = reinterpret_cast<T*>(smem);  // [2] query tiles, [2] tiles of their output's gradient
+  T* sg = sq + 2 * TILE;
+  float* srow = reinterpret_cast<float*>(sg + 2 * TILE);  // [2][3][64]: lse, D, factor
+  float* lut = srow + 2 * 3 * 64;
+  int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
-  const int G = a.H / a.Hk, shift = a.N - a.M;
+  const int G = a.H / a.Hk, shift = a.N - a.M, half = wave >> 1;
   const WinVis vis(a);
 
   int bhk, j0, c = 0;
@@ -239,19 +253,12 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     j0 = 32 * (x % ngrp);
     bhk = x / ngrp;
   } else {
-    const int nkt = (a.N + WIN_RES - 1) / WIN_RES;
-    j0 = (x % nkt) * WIN_RES + wave * 32;
+    const int nkt = (a.N + WIN_KEYS - 1) / WIN_KEYS;
+    j0 = (x % nkt) * WIN_KEYS + (wave & 1) * 32;
     bhk = x / nkt;
   }
   const int b = bhk / a.Hk, hk = bhk % a.Hk, j = j0 + (lane & 31);
   const float* mask = a.mask ? a.mask + (size_t)b * a.N : nullptr;
-  const bool key_ok = j < (SINK ? min(a.n_sink, a.N) : a.N) && (!mask || mask[j] != 0.f);
-  typename E::Frag kf, vf;
-  E::template load_frag<FAST>(
-      kf, key_ok ? reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + (size_t)j * a.ksn : nullptr, a.d, lane);
-  E::template load_frag<FAST>(
-      vf, key_ok ? reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + (size_t)j * a.vsn : nullptr, a.d, lane);
-  const float sc = a.scale * LOG2E;
 
   int ilo, ihi;  // queries [ilo, ihi)
   if (SINK) {
@@ -259,137 +266,160 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     ilo = first + c * a.chunk;
     ihi = min(a.M, ilo + a.chunk);
   } else {
-    const int k0 = j0 - wave * 32, k1 = min(a.N, k0 + WIN_RES) - 1;
+    const int k0 = j0 - (wave & 1) * 32, k1 = min(a.N, k0 + WIN_KEYS) - 1;
     ilo = max(0, k0 - vis.off - shift);
     ihi = min(a.M, k1 - vis.off + (int)vis.range - shift);
   }
-  f32x16 dk[E::NT] = {}, dv[E::NT] = {};
-  for (int g = 0; g < G; ++g) {
-    const int h = hk * G + g;
-    if (REL) {
-      __syncthreads();
-      build_rel_lut(a, h, lut, nullptr);
-    }
-    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh;
+  const int nt = ihi > ilo ? (ihi - ilo + 63) / 64 : 0, total = G * nt;
+  RowBits<64> rb(mask ? mask + shift : nullptr, a.M);
+  float r_lse, r_d, r_f;  // of the next tile's row threadIdx.x
+  auto issue = [&](int it, int buf) {
+    const int h = hk * G + it / nt, i0 = ilo + it % nt * 64;
     const size_t row0 = ((size_t)b * a.H + h) * a.M;
-    const T* gb = reinterpret_cast<const T*>(a.go) + row0 * a.d;
-    const RowLoader<T, DP, FAST> lq(qb, a.qsn, a.M, a.d), lg(gb, a.d, a.M, a.d);
-    for (int i0 = ilo; i0 < ihi; i0 += E::BK) {
-      __syncthreads();
-      lq.issue(sq, i0);
-      lg.issue(sg, i0);
-      RowBits<E::BK> rb(mask ? mask + shift : nullptr, a.M);
-      rb.fetch(i0);
-      if ((int)threadIdx.x < E::BK) {
-        const int i = i0 + threadIdx.x;
-        const bool ok = i < ihi && (!mask || mask[shift + i] != 0.f);
-        srow[threadIdx.x] = ok ? a.lse[row0 + i] : LSE_EMPTY;
-        srow[E::BK + threadIdx.x] = ok ? a.rowd[2 * (row0 + i)] : 0.f;
-        srow[2 * E::BK + threadIdx.x] = ok ? a.rowd[2 * (row0 + i) + 1] : 0.f;
+    const RowLoader<T, DP, FAST> lq(reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh, a.qsn, a.M, a.d);
+    const RowLoader<T, DP, FAST> lg(reinterpret_cast<const T*>(a.go) + row0 * a.d, a.d, a.M, a.d);
+    rb.fetch(i0);
+    if (threadIdx.x < 64) {
+      const int i = i0 + threadIdx.x;
+      const bool ok = i < ihi;
+      const size_t at = row0 + min(i, a.M - 1);
+      r_lse = ok ? a.lse[at] : LSE_EMPTY;
+      r_d = ok ? a.rowd[2 * at] : 0.f;
+      r_f = ok ? a.rowd[2 * at + 1] : 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      lq.issue(sq + buf * TILE + n * E::TILE, i0 + n * E::BK);
+      lg.issue(sg + buf * TILE + n * E::TILE, i0 + n * E::BK);
+    }
+  };
+  auto put_rows = [&](int buf) {
+    if (threadIdx.x < 64) {
+      float* r = srow + buf * 192 + threadIdx.x;
+      r[0] = r_lse;
+      r[64] = r_d;
+      r[128] = r_f;
+    }
+  };
+  if (total > 0) {
+    issue(0, 0);
+    if (REL) stage_edges(a.rel, edge);
+    put_rows(0);
+  }
+
+  const bool key_ok = j < (SINK ? min(a.n_sink, a.N) : a.N) && (!mask || mask[j] != 0.f);
+  typename E::Frag kf, vf;
+  E::template load_frag<FAST>(
+      kf, key_ok ? reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + (size_t)j * a.ksn : nullptr, a.d, lane);
+  E::template load_frag<FAST>(
+      vf, key_ok ? reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + (size_t)j * a.vsn : nullptr, a.d, lane);
+  const float sc = a.scale * LOG2E;
+  f32x16 dk[E::NT] = {}, dv[E::NT] = {};
+  for (int it = 0; it < total; ++it) {
+    const int buf = it & 1;
+    lds_loads_done();
+    __syncthreads();  // this tile is there, and the other buffer's products are done
+    const uint64_t now = rb.get();
+    if (now != ~0ull) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        clear_rows<T, DP>(sq + buf * TILE + n * E::TILE, now >> (n * E::BK & 63));
+        clear_rows<T, DP>(sg + buf * TILE + n * E::TILE, now >> (n * E::BK & 63));
       }
-      lds_loads_done();
-      __syncthreads();
-      const uint64_t bits = rb.get();
-      if (bits != RowBits<E::BK>::ALL) {
-        clear_rows<T, DP>(sq, bits);
-        clear_rows<T, DP>(sg, bits);
-        __syncthreads();
+      // a masked query's row may have an lse of any value
+      if (threadIdx.x < 64 && !((now >> threadIdx.x) & 1u)) srow[buf * 192 + threadIdx.x] = LSE_EMPTY;
+    }
+    if (REL && it % nt == 0) build_rel_lut(a, hk * G + it / nt, edge, lut, nullptr);
+    if (now != ~0ull || (REL && it % nt == 0)) __syncthreads();
+    if (it + 1 < total) issue(it + 1, buf ^ 1);
+
+    const int sub = SINK ? wave : half, t0 = ilo + it % nt * 64 + 32 * sub + shift;
+    if (sub < 2 && !(SINK ? vis.all_near(t0, j0) : vis.none_near(t0, j0))) {
+      T *tq = sq + buf * TILE, *tg = sg + buf * TILE;
+      f32x16 p = E::row_product(tq, 32 * sub, kf, lane);
+      f32x16 ds = E::row_product(tg, 32 * sub, vf, lane);
+      const float* sr = srow + buf * 192 + 32 * sub + 4 * h32;
+      const int far = REL ? rel_far(a.rel, t0, j0) : 0;
+      if (REL && far < 0) {
+        const float* lp = lut + rel_lut_base(a.rel) + t0 + 4 * h32 - j;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = __builtin_fmaf(p[r], sc, lp[acc_row(r, 0)] - sr[acc_row(r, 0)]);
+      } else {
+        const float cst = REL ? lut[far] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = __builtin_fmaf(p[r], sc, cst - sr[acc_row(r, 0)]);
       }
-#pragma unroll
-      for (int sub = 0; sub < E::NSUB; ++sub) {
-        const int t0 = i0 + 32 * sub + shift;
-        if (SINK ? (sub != wave || vis.all_near(t0, j0)) : vis.none_near(t0, j0)) continue;
-        f32x16 p = E::row_product(sq, 32 * sub, kf, lane);
-        f32x16 ds = E::row_product(sg, 32 * sub, vf, lane);
-        if (REL) {
-          const int far = rel_far(a.rel, t0, j0);
-          if (far >= 0) {
-            const float cst = lut[far];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = __builtin_fmaf(p[r], sc, cst);
-          } else {
-            const float* lp = lut + rel_lut_base(a.rel) + t0 + 4 * h32 - j;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = __builtin_fmaf(p[r], sc, lp[acc_row(r, 0)]);
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) p[r] *= sc;
-        }
-        if (SINK || !vis.all_near(t0, j0)) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int t = t0 + acc_row(r, h32);
-            const bool near = vis.near(t, j);
-            p[r] = (SINK ? !near & vis.first(t, j) : near) ? p[r] : -INFINITY;
-          }
-        }
-        const float* sr = srow + 32 * sub + 4 * h32;
+      if (SINK || !vis.all_near(t0, j0)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int at = acc_row(r, 0);
-          p[r] = fast_exp2(p[r] - sr[at]);
-          ds[r] = p[r] * __builtin_fmaf(ds[r], sr[2 * E::BK + at], -sr[E::BK + at]);
+          const int t = t0 + acc_row(r, h32);
+          const bool near = vis.near(t, j);
+          p[r] = (SINK ? !near & vis.first(t, j) : near) ? p[r] : -INFINITY;
         }
-        typename E::Prob o;
-        E::to_operand(p, o);
-        E::column_product(sg, 32 * sub, o, dv, lane);
-        E::to_operand(ds, o);
-        E::column_product(sq, 32 * sub, o, dk, lane);
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int at = acc_row(r, 0);
+        p[r] = fast_exp2(p[r]);
+        ds[r] = p[r] * __builtin_fmaf(ds[r], sr[128 + at], -sr[64 + at]);
+      }
+      typename E::Prob o;
+      E::to_operand(p, o);
+      E::column_product(tg, 32 * sub, o, dv, lane);
+      E::to_operand(ds, o);
+      E::column_product(tq, 32 * sub, o, dk, lane);
     }
+    if (it + 1 < total) put_rows(buf ^ 1);
   }
+  // the waves that share keys add their sums in LDS, in wave order; dk and dv, one after the other: [keys][DP]
   const int ns = min(a.n_sink, a.N);
-  if (SINK) {
-    // the waves' sums meet in LDS, added in wave order
-    float* red = reinterpret_cast<float*>(smem);  // [32][2][DP] over the staged tiles
-    for (int w = 0; w < E::NSUB; ++w) {
-      __syncthreads();
-      if (wave != w) continue;
+  float* red = reinterpret_cast<float*>(smem);
+  const int kl = (SINK ? 0 : (wave & 1) * 32) + (lane & 31);  // this lane's key of the workgroup
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    f32x16(&acc)[E::NT] = which ? dv : dk;
+    __syncthreads();
+    if (SINK ? wave == 1 : half == 1) {
 #pragma unroll
       for (int n = 0; n < E::NT; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float* at = red + (lane & 31) * 2 * DP + 32 * n + acc_row(r, h32);
-          at[0] = w ? at[0] + dk[n][r] : dk[n][r];
-          at[DP] = w ? at[DP] + dv[n][r] : dv[n][r];
+        for (int r = 0; r < 16; r += 4) {
+          f32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = acc[n][r + e];
+          *reinterpret_cast<f32x4*>(red + kl * (DP + 4) + 32 * n + acc_row(r, h32)) = w;
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 32 * 2 * DP; e += WIN_NT) {
-      const int r = e / (2 * DP);
-      if (j0 + r < ns)
-        a.sink_part[(((size_t)bhk * (a.n_chunks + 1) + c) * ns + j0 + r) * 2 * DP + e % (2 * DP)] = red[e];
-    }
-    return;
-  }
-  if (j >= a.N) return;
-  if (a.n_chunks > 0 && j < ns) {  // joined with the chunks' sums by the finalize kernel
-    float* at = a.sink_part + (((size_t)bhk * (a.n_chunks + 1) + a.n_chunks) * ns + j) * 2 * DP;
+    if (SINK ? wave != 0 : half != 0) continue;
+    if (j >= (SINK ? ns : a.N)) continue;
+    float* part = nullptr;  // joined by the finalize kernel: the first tokens' rows
+    if (a.n_chunks > 0 && j < ns)
+      part = a.sink_part + (((size_t)bhk * (a.n_chunks + 1) + (SINK ? c : a.n_chunks)) * ns + j) * 2 * DP + which * DP;
+    T* out = reinterpret_cast<T*>(which ? a.dv : a.dk) + ((size_t)bhk * a.N + j) * a.d;
+    const float f = which ? 1.f : a.scale;
 #pragma unroll
     for (int n = 0; n < E::NT; ++n)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        at[32 * n + acc_row(r, h32)] = dk[n][r];
-        at[DP + 32 * n + acc_row(r, h32)] = dv[n][r];
+      for (int r = 0; r < 16; r += 4) {
+        const int col = 32 * n + acc_row(r, h32);
+        const f32x4 w = *reinterpret_cast<const f32x4*>(red + kl * (DP + 4) + col);
+        f32x4 s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = acc[n][r + e] + w[e];
+        if (part) {
+          *reinterpret_cast<f32x4*>(part + col) = s;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[e] = key_ok ? s[e] * f : 0.f;
+          store4<T, FAST>(out, col, a.d, s);
+        }
       }
-    return;
   }
-  const size_t krow = ((size_t)bhk * a.N + j) * a.d;
-#pragma unroll
-  for (int n = 0; n < E::NT; ++n)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int col = 32 * n + acc_row(r, h32);
-      if (col < a.d) {
-        reinterpret_cast<T*>(a.dk)[krow + col] = from_f32<T>(key_ok ? dk[n][r] * a.scale : 0.f);
-        reinterpret_cast<T*>(a.dv)[krow + col] = from_f32<T>(key_ok ? dv[n][r] : 0.f);
-      }
-    }
 }
 
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT) window_bwd_kv_kernel(WinArgs a, int n_sink_blocks) {
+__global__ void __launch_bounds__(WIN_NT, DP == 128 ? 1 : 2) window_bwd_kv_kernel(WinArgs a, int n_sink_blocks) {
   extern __shared__ __align__(16) unsigned char smem[];
   if ((int)blockIdx.x < n_sink_blocks)
     bwd_kv<T, DP, FAST, REL, true>(a, blockIdx.x, smem);
@@ -429,18 +459,20 @@ bool window_fast(const WinArgs& a, bool bf16_in, bool bwd);
 template <typename T, int DP, bool FAST, bool REL>
 static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
-  const size_t tiles = 2 * E::TILE * sizeof(T), lutn = REL ? rel_lut_size(a.rel) : 0;
+  const size_t lutn = REL ? rel_lut_size(a.rel) : 0, rel = REL ? (lutn + REL_EDGES) * 4 : 0;
   const bool tab = REL && a.dtable;
-  const size_t lq = tiles + lutn * 4 + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0);
-  // the first tokens' reduction takes 64 DP floats over the tiles
-  const size_t lkv = std::max(tiles + 3 * E::BK * 4 + lutn * 4, (size_t)64 * DP * 4);
+  const size_t lq1 = rel + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0), buf = 2 * E::TILE * sizeof(T);
+  const int n_buf = lq1 + 2 * buf <= 160 * 1024 ? 2 : 1;
+  const size_t lq = lq1 + n_buf * buf;
+  // (the joined sums, 64 (DP + 4) floats, lie over the tiles, 256 DP elements)
+  const size_t lkv = 4 * 64 * DP * sizeof(T) + 2 * 3 * 64 * 4 + rel;
   auto kq = window_bwd_q_kernel<T, DP, FAST, REL>;
   auto kkv = window_bwd_kv_kernel<T, DP, FAST, REL>;
   hipError_t e = set_lds_limit((const void*)kq, lq);
   if (e != hipSuccess) return e;
   if ((e = set_lds_limit((const void*)kkv, lkv)) != hipSuccess) return e;
-  const int nqt = (a.M + WIN_RES - 1) / WIN_RES, nkt = (a.N + WIN_RES - 1) / WIN_RES, ns = std::min(a.n_sink, a.N);
-  hipLaunchKernelGGL(kq, dim3((unsigned)(nqt * a.B * a.H)), dim3(WIN_NT), lq, s, a);
+  const int nqt = (a.M + WIN_RES - 1) / WIN_RES, nkt = (a.N + WIN_KEYS - 1) / WIN_KEYS, ns = std::min(a.n_sink, a.N);
+  hipLaunchKernelGGL(kq, dim3((unsigned)(nqt * a.B * a.H)), dim3(WIN_NT), lq, s, a, n_buf);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int nsb = a.n_chunks > 0 ? a.B * a.Hk * a.n_chunks * ((ns + 31) / 32) : 0;
   hipLaunchKernelGGL(kkv, dim3((unsigned)(nkt * a.B * a.Hk + nsb)), dim3(WIN_NT), lkv, s, a, nsb);

@@ -193,6 +193,7 @@ struct WinVis {
 // entries more than the table's range on both sides hold its end values, so that a 32 x 32
 // tile any pair of which is inside the range needs no clamp.
 constexpr int REL_PAD = 64;
+constexpr int REL_EDGES = 96;  // ints of the edges in LDS, behind a lookup table
 __host__ __device__ inline int rel_lut_size(const RelSpec& r) {
   return ((r.both ? 2 * r.dist() + 1 : r.dist() + 1) + 2 * REL_PAD + 3) & ~3;
 }
@@ -204,11 +205,24 @@ __device__ __forceinline__ int rel_bucket(const RelSpec& r, int rel) {
   for (int k = 0; k < r.n; ++k) b += r.edge[k] <= mag;
   return b + ((r.both && rel > 0) ? r.n + 1 : 0);
 }
-__device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, float* lut, uint8_t* bucket) {
+// The same from edges in LDS, by bisection.
+__device__ __forceinline__ int rel_bucket_lds(const int* edge, int n, int both, int rel) {
+  const int mag = both ? abs(rel) : max(-rel, 0);
+  int b = 0;
+#pragma unroll
+  for (int step = 64; step; step >>= 1)
+    if (b + step <= n && edge[b + step - 1] <= mag) b += step;
+  return b + ((both && rel > 0) ? n + 1 : 0);
+}
+// Edges to LDS; the caller synchronises before they are read.
+__device__ __forceinline__ void stage_edges(const RelSpec& r, int* edge) {
+  if ((int)threadIdx.x < r.n) edge[threadIdx.x] = r.edge[threadIdx.x];
+}
+__device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, const int* edge, float* lut, uint8_t* bucket) {
   const int n = rel_lut_size(a.rel), base = rel_lut_base(a.rel);
   const float* row = a.table + (size_t)h * a.rel.buckets();
   for (int x = threadIdx.x; x < n; x += blockDim.x) {
-    const int b = rel_bucket(a.rel, base - x);
+    const int b = rel_bucket_lds(edge, a.rel.n, a.rel.both, base - x);
     lut[x] = row[b] * LOG2E;
     if (bucket) bucket[x] = (uint8_t)b;
   }

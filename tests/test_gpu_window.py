@@ -74,6 +74,9 @@ def test_attention_long(causal, dtype):
     tile, one with the largest distance."""
     attention_case(1, 2, 1, 900, 900, 64, dtype, 400, 4, causal, True)
     attention_case(1, 2, 1, 600, 700, 32, dtype, 333, 128, causal, True, edges=(1, 5, 200, 2048) if causal else (3, 90))
+    # the largest table: its sums leave the key tiles one buffer
+    attention_case(1, 2, 1, 300, 310, 128, dtype, 290, 4, causal, True,
+                   edges=(*range(1, 95), 2048) if causal else (*range(2, 48), 2048))
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
