@@ -224,37 +224,40 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   }
 }
 
-// Key-resident pass: 64 keys of a (sample, key head) against the queries of their band, 64 staged queries at a time;
-// a wave has 32 of the keys (wave & 1) and 32 of the staged queries (wave >> 1), so that twice as many workgroups share
-// the keys as with 32 keys a wave each, and the two halves of a key's sum meet in LDS at the end.
-// SINK: 32 of the first tokens' keys against a chunk of the queries outside their band.
+// Key-resident pass: 64 keys of a (sample, key head) against the queries of their band, 64 staged queries at a time.
+// Wave (kg, half) forms p and ds of 32 keys (group kg) and 32 of the staged queries (`half`), and sums one result over
+// all of them: half 0 dv, half 1 dk.  So each hands the other half one operand through LDS (p or ds, in bf16 for bf16)
+// and keeps one accumulator, not two: 256 registers a lane and two workgroups a CU, where both sums in every wave took
+// 474 registers and left each matrix instruction's latency uncovered (196 us against PLACEHOLDER at 4096 tokens).
+// SINK: 64 of the first tokens' keys against a chunk of the queries outside their band.
 constexpr int WIN_KEYS = 64;
 
 template <typename T, int DP, bool FAST, bool REL, bool SINK>
-__device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* smem) {
+__device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsigned char* smem) {
   using E = WinEng<T, DP>;
   constexpr int NB = 64 / E::BK;  // LDS tiles of the engine's size in 64 rows
   constexpr int TILE = 64 * DP;
-  T* sq = reinterpret_cast<T*>(smem);  // [2] query tiles, [2] tiles of their output's gradient
-  T* sg = sq + 2 * TILE;
-  float* srow = reinterpret_cast<float*>(sg + 2 * TILE);  // [2][3][64]: lse, D, factor
+  T* sq = reinterpret_cast<T*>(smem);  // [n_buf] query tiles, [n_buf] tiles of their output's gradient
+  T* sg = sq + n_buf * TILE;
+  typename E::Prob* xch = reinterpret_cast<typename E::Prob*>(sg + n_buf * TILE);  // [kg][half][64]: operands handed over
+  float* srow = reinterpret_cast<float*>(xch + 4 * 64);                         // [2][3][64]: lse, D, factor
   float* lut = srow + 2 * 3 * 64;
   int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
-  const int G = a.H / a.Hk, shift = a.N - a.M, half = wave >> 1;
+  const int G = a.H / a.Hk, shift = a.N - a.M, kg = wave & 1, half = wave >> 1;
   const WinVis vis(a);
 
   int bhk, j0, c = 0;
   if (SINK) {
-    const int ngrp = (min(a.n_sink, a.N) + 31) / 32;
+    const int ngrp = (min(a.n_sink, a.N) + WIN_KEYS - 1) / WIN_KEYS;
     c = x % a.n_chunks;
     x /= a.n_chunks;
-    j0 = 32 * (x % ngrp);
+    j0 = WIN_KEYS * (x % ngrp) + 32 * kg;
     bhk = x / ngrp;
   } else {
     const int nkt = (a.N + WIN_KEYS - 1) / WIN_KEYS;
-    j0 = (x % nkt) * WIN_KEYS + (wave & 1) * 32;
+    j0 = (x % nkt) * WIN_KEYS + 32 * kg;
     bhk = x / nkt;
   }
   const int b = bhk / a.Hk, hk = bhk % a.Hk, j = j0 + (lane & 31);
@@ -266,7 +269,7 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     ilo = first + c * a.chunk;
     ihi = min(a.M, ilo + a.chunk);
   } else {
-    const int k0 = j0 - (wave & 1) * 32, k1 = min(a.N, k0 + WIN_KEYS) - 1;
+    const int k0 = j0 - 32 * kg, k1 = min(a.N, k0 + WIN_KEYS) - 1;
     ilo = max(0, k0 - vis.off - shift);
     ihi = min(a.M, k1 - vis.off + (int)vis.range - shift);
   }
@@ -301,9 +304,9 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
       r[128] = r_f;
     }
   };
-  if (total > 0) {
+  if (REL) stage_edges(a.rel, edge);
+  if (n_buf > 1 && total > 0) {
     issue(0, 0);
-    if (REL) stage_edges(a.rel, edge);
     put_rows(0);
   }
 
@@ -314,9 +317,17 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
   E::template load_frag<FAST>(
       vf, key_ok ? reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + (size_t)j * a.vsn : nullptr, a.d, lane);
   const float sc = a.scale * LOG2E;
-  f32x16 dk[E::NT] = {}, dv[E::NT] = {};
+  const int ns = min(a.n_sink, a.N);
+  f32x16 acc[E::NT] = {};  // half 0: dv, half 1: dk
+  // whether any of the wave's keys and the 32 queries from t0 on meet here
+  auto meet = [&](int t0) { return SINK ? (j0 < ns) & !vis.all_near(t0, j0) : !vis.none_near(t0, j0); };
   for (int it = 0; it < total; ++it) {
-    const int buf = it & 1;
+    const int buf = it & (n_buf - 1);
+    if (n_buf == 1) {
+      __syncthreads();
+      issue(it, 0);
+      put_rows(0);
+    }
     lds_loads_done();
     __syncthreads();  // this tile is there, and the other buffer's products are done
     const uint64_t now = rb.get();
@@ -331,14 +342,15 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
     }
     if (REL && it % nt == 0) build_rel_lut(a, hk * G + it / nt, edge, lut, nullptr);
     if (now != ~0ull || (REL && it % nt == 0)) __syncthreads();
-    if (it + 1 < total) issue(it + 1, buf ^ 1);
+    const bool next = n_buf > 1 && it + 1 < total;
+    if (next) issue(it + 1, buf ^ 1);
 
-    const int sub = SINK ? wave : half, t0 = ilo + it % nt * 64 + 32 * sub + shift;
-    if (sub < 2 && !(SINK ? vis.all_near(t0, j0) : vis.none_near(t0, j0))) {
-      T *tq = sq + buf * TILE, *tg = sg + buf * TILE;
-      f32x16 p = E::row_product(tq, 32 * sub, kf, lane);
-      f32x16 ds = E::row_product(tg, 32 * sub, vf, lane);
-      const float* sr = srow + buf * 192 + 32 * sub + 4 * h32;
+    const int tile0 = ilo + it % nt * 64 + shift, t0 = tile0 + 32 * half;
+    T *tq = sq + buf * TILE, *tg = sg + buf * TILE;
+    if (meet(t0)) {
+      f32x16 p = E::row_product(tq, 32 * half, kf, lane);
+      f32x16 ds = E::row_product(tg, 32 * half, vf, lane);
+      const float* sr = srow + buf * 192 + 32 * half + 4 * h32;
       const int far = REL ? rel_far(a.rel, t0, j0) : 0;
       if (REL && far < 0) {
         const float* lp = lut + rel_lut_base(a.rel) + t0 + 4 * h32 - j;
@@ -363,68 +375,47 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, unsigned char* s
         p[r] = fast_exp2(p[r]);
         ds[r] = p[r] * __builtin_fmaf(ds[r], sr[128 + at], -sr[64 + at]);
       }
-      typename E::Prob o;
-      E::to_operand(p, o);
-      E::column_product(tg, 32 * sub, o, dv, lane);
-      E::to_operand(ds, o);
-      E::column_product(tq, 32 * sub, o, dk, lane);
+      typename E::Prob o, other;
+      E::to_operand(half ? ds : p, o);
+      E::to_operand(half ? p : ds, other);
+      xch[(2 * kg + half) * 64 + lane] = other;
+      E::column_product(half ? tq : tg, 32 * half, o, acc, lane);
     }
-    if (it + 1 < total) put_rows(buf ^ 1);
-  }
-  // the waves that share keys add their sums in LDS, in wave order; dk and dv, one after the other: [keys][DP]
-  const int ns = min(a.n_sink, a.N);
-  float* red = reinterpret_cast<float*>(smem);
-  const int kl = (SINK ? 0 : (wave & 1) * 32) + (lane & 31);  // this lane's key of the workgroup
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    f32x16(&acc)[E::NT] = which ? dv : dk;
-    __syncthreads();
-    if (SINK ? wave == 1 : half == 1) {
-#pragma unroll
-      for (int n = 0; n < E::NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          f32x4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = acc[n][r + e];
-          *reinterpret_cast<f32x4*>(red + kl * (DP + 4) + 32 * n + acc_row(r, h32)) = w;
-        }
+    lds_barrier();
+    if (meet(tile0 + 32 * (half ^ 1))) {
+      const typename E::Prob o = xch[(2 * kg + (half ^ 1)) * 64 + lane];
+      E::column_product(half ? tq : tg, 32 * (half ^ 1), o, acc, lane);
     }
-    __syncthreads();
-    if (SINK ? wave != 0 : half != 0) continue;
-    if (j >= (SINK ? ns : a.N)) continue;
-    float* part = nullptr;  // joined by the finalize kernel: the first tokens' rows
-    if (a.n_chunks > 0 && j < ns)
-      part = a.sink_part + (((size_t)bhk * (a.n_chunks + 1) + (SINK ? c : a.n_chunks)) * ns + j) * 2 * DP + which * DP;
-    T* out = reinterpret_cast<T*>(which ? a.dv : a.dk) + ((size_t)bhk * a.N + j) * a.d;
-    const float f = which ? 1.f : a.scale;
-#pragma unroll
-    for (int n = 0; n < E::NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int col = 32 * n + acc_row(r, h32);
-        const f32x4 w = *reinterpret_cast<const f32x4*>(red + kl * (DP + 4) + col);
-        f32x4 s;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] = acc[n][r + e] + w[e];
-        if (part) {
-          *reinterpret_cast<f32x4*>(part + col) = s;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = key_ok ? s[e] * f : 0.f;
-          store4<T, FAST>(out, col, a.d, s);
-        }
-      }
+    if (next) put_rows(buf ^ 1);
   }
+  if (j >= (SINK ? ns : a.N)) return;
+  const int which = half ? 0 : 1;  // dk before dv in a partial row
+  float* part = nullptr;           // joined by the finalize kernel: the first tokens' rows
+  if (a.n_chunks > 0 && j < ns)
+    part = a.sink_part + (((size_t)bhk * (a.n_chunks + 1) + (SINK ? c : a.n_chunks)) * ns + j) * 2 * DP + which * DP;
+  T* out = reinterpret_cast<T*>(half ? a.dk : a.dv) + ((size_t)bhk * a.N + j) * a.d;
+  const float f = key_ok ? (half ? a.scale : 1.f) : 0.f;
+#pragma unroll
+  for (int n = 0; n < E::NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int col = 32 * n + acc_row(r, h32);
+      f32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = part ? acc[n][r + e] : key_ok ? acc[n][r + e] * f : 0.f;
+      if (part) *reinterpret_cast<f32x4*>(part + col) = w;
+      else store4<T, FAST>(out, col, a.d, w);
+    }
 }
 
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT, DP == 128 ? 1 : 2) window_bwd_kv_kernel(WinArgs a, int n_sink_blocks) {
+__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) window_bwd_kv_kernel(WinArgs a, int n_sink_blocks, int n_buf) {
   extern __shared__ __align__(16) unsigned char smem[];
   if ((int)blockIdx.x < n_sink_blocks)
-    bwd_kv<T, DP, FAST, REL, true>(a, blockIdx.x, smem);
+    bwd_kv<T, DP, FAST, REL, true>(a, blockIdx.x, n_buf, smem);
   else
-    bwd_kv<T, DP, FAST, REL, false>(a, xcd_order(blockIdx.x - n_sink_blocks, gridDim.x - n_sink_blocks), smem);
+    bwd_kv<T, DP, FAST, REL, false>(a, xcd_order(blockIdx.x - n_sink_blocks, gridDim.x - n_sink_blocks), n_buf,
+                                       smem);
 }
 
 // The first tokens' rows from their partial sums (band last), and the table's gradient from the query tiles'; a wave
@@ -464,8 +455,9 @@ static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   const size_t lq1 = rel + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0), buf = 2 * E::TILE * sizeof(T);
   const int n_buf = lq1 + 2 * buf <= 160 * 1024 ? 2 : 1;
   const size_t lq = lq1 + n_buf * buf;
-  // (the joined sums, 64 (DP + 4) floats, lie over the tiles, 256 DP elements)
-  const size_t lkv = 4 * 64 * DP * sizeof(T) + 2 * 3 * 64 * 4 + rel;
+  const size_t lkv1 = 4 * 64 * sizeof(typename E::Prob) + 2 * 3 * 64 * 4 + rel, kbuf = 2 * 64 * DP * sizeof(T);
+  const int n_kbuf = lkv1 + 2 * kbuf <= 160 * 1024 ? 2 : 1;
+  const size_t lkv = lkv1 + n_kbuf * kbuf;
   auto kq = window_bwd_q_kernel<T, DP, FAST, REL>;
   auto kkv = window_bwd_kv_kernel<T, DP, FAST, REL>;
   hipError_t e = set_lds_limit((const void*)kq, lq);
@@ -474,8 +466,8 @@ static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   const int nqt = (a.M + WIN_RES - 1) / WIN_RES, nkt = (a.N + WIN_KEYS - 1) / WIN_KEYS, ns = std::min(a.n_sink, a.N);
   hipLaunchKernelGGL(kq, dim3((unsigned)(nqt * a.B * a.H)), dim3(WIN_NT), lq, s, a, n_buf);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int nsb = a.n_chunks > 0 ? a.B * a.Hk * a.n_chunks * ((ns + 31) / 32) : 0;
-  hipLaunchKernelGGL(kkv, dim3((unsigned)(nkt * a.B * a.Hk + nsb)), dim3(WIN_NT), lkv, s, a, nsb);
+  const int nsb = a.n_chunks > 0 ? a.B * a.Hk * a.n_chunks * ((ns + WIN_KEYS - 1) / WIN_KEYS) : 0;
+  hipLaunchKernelGGL(kkv, dim3((unsigned)(nkt * a.B * a.Hk + nsb)), dim3(WIN_NT), lkv, s, a, nsb, n_kbuf);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int rows = a.n_chunks > 0 ? a.B * a.Hk * ns * (2 * DP / 64) : 0, tabs = tab ? a.H * a.rel.buckets() : 0;
   if (rows + tabs > 0) {

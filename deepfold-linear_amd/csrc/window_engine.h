@@ -23,6 +23,8 @@
 #include "common.h"
 #include "window_args.h"
 
+#include <type_traits>
+
 namespace dfl {
 
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
@@ -101,9 +103,9 @@ template <typename T, int DP> struct WinEng {
     return c;
   }
   // B operands of a column product
+  typedef typename std::conditional<sizeof(T) == 2, bf16x8, f32x16>::type ProbV;
   struct Prob {
-    bf16x8 h[sizeof(T) == 2 ? 2 : 1];
-    f32x16 f;
+    ProbV h[sizeof(T) == 2 ? 2 : 1];
   };
   // bf16: probabilities and score gradients are rounded to bf16 here, as their products' other operand is;
   // the sums stay in fp32
@@ -112,7 +114,7 @@ template <typename T, int DP> struct WinEng {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o.h[r / 8][r % 8] = (bf16)p[r];
     } else {
-      o.f = p;
+      o.h[0] = p;
     }
   }
   // acc[t] += (columns 32 t .. of rows r0 .. r0 + 31 of the tile)^T P
@@ -143,7 +145,7 @@ template <typename T, int DP> struct WinEng {
         for (int t = 0; t < NT; ++t) {
           const int col = 32 * t + (lane & 31);
           const float a = tile[row * DP + swz(row, col / VEC) * VEC + col % VEC];
-          acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p.f[r], acc[t], 0, 0, 0);
+          acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p.h[0][r], acc[t], 0, 0, 0);
         }
       }
     }
