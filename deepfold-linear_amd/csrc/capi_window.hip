@@ -99,14 +99,28 @@ struct Chunks {
   }
 };
 
+// Parts of a key tile's queries (window_attn_bwd.hip: 64 keys, 64 queries a step).  Below two workgroups a CU the
+// key pass waits for its own loads and barriers most of the time: at 16 / 4 heads of 4096 tokens, 256 workgroups,
+// window 1024, it takes PLACEHOLDER2 us in one part and PLACEHOLDER3 us in two.
+int kv_split(int B, int H, int Hk, int M, int N, int window, int causal) {
+  const long long tiles = ((long long)N + 63) / 64 * B * Hk;
+  const long long w = std::min(window, N), band = std::min<long long>(M, 63 + (causal ? w : 2 * w - 1));
+  const long long steps = (long long)(H / Hk) * ((band + 63) / 64);
+  int s = 1;
+  while (s < 8 && tiles * s < 512 && steps / (2 * s) >= 8) s *= 2;
+  return s;
+}
+
 struct WindowWs {
-  size_t rowd, sink, tab, total;
+  size_t rowd, sink, kv, tab, total;
   WindowWs(int B, int H, int Hk, int M, int N, int d, int window, int n_sink, int causal, int n_edges) {
     const Chunks c(M, N, window, n_sink, causal);
     const size_t DP = pad_dim(d), nqt = ((size_t)M + RES - 1) / RES, nb = causal ? n_edges + 1 : 2 * (n_edges + 1);
     rowd = 0;
     sink = r256((size_t)B * H * M * 8);
-    tab = sink + r256(c.n ? (size_t)B * Hk * (c.n + 1) * std::min(n_sink, N) * 2 * DP * 4 : 0);
+    kv = sink + r256(c.n ? (size_t)B * Hk * (c.n + 1) * std::min(n_sink, N) * 2 * DP * 4 : 0);
+    const int split = kv_split(B, H, Hk, M, N, window, causal);
+    tab = kv + r256(split > 1 ? (size_t)split * B * Hk * N * 2 * DP * 4 : 0);
     total = tab + r256(n_edges > 0 ? (size_t)B * H * nqt * nb * 4 : 0);
   }
 };
@@ -117,7 +131,7 @@ int check_attn(const dfl_window_attn_params* p, bool bwd) {
   if (int rc = check_window(p->window, p->n_sink)) return rc;
   if (p->M <= 0 || p->N <= 0 || p->M > p->N || p->N > MAX_N)
     return fail("M=%d, N=%d: need 0 < M <= N <= %lld", p->M, p->N, MAX_N);
-  if ((((long long)p->N + RES - 1) / RES + 1) * p->B * p->H >= (1ll << 31)) return fail("too many rows");
+  if ((((long long)p->N + 63) / 64 + 1) * p->B * p->H * 8 >= (1ll << 31)) return fail("too many rows");
   if (int rc = check_scale(p->scale)) return rc;
   if (!p->q || !p->k || !p->v || !p->o) return fail("required pointer is NULL");
   if (!p->rel_table != (p->n_edges == 0)) return fail("rel_table and rel_edges must be given together");
@@ -187,7 +201,7 @@ extern "C" {
 
 size_t dfl_window_attn_workspace_size(int B, int H, int Hk, int M, int N, int d, int window, int n_sink, int causal,
                                       int n_edges) {
-  if (B <= 0 || H <= 0 || Hk <= 0 || M <= 0 || N < M || d <= 0 || d > 128 || window < 1 || n_sink < 0 || n_edges < 0)
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || M <= 0 || N < M || d <= 0 || d > 128 || window < 1 || n_sink < 0 || n_edges < 0)
     return 0;
   return WindowWs(B, H, Hk, M, N, d, window, n_sink, causal, n_edges).total;
 }
@@ -215,6 +229,8 @@ int dfl_window_attn_bwd(const dfl_window_attn_params* p, void* workspace, size_t
     a.rowd = reinterpret_cast<float*>(ws + w.rowd);
     a.sink_part = reinterpret_cast<float*>(ws + w.sink);
     a.tab_part = reinterpret_cast<float*>(ws + w.tab);
+    a.kv_part = reinterpret_cast<float*>(ws + w.kv);
+    a.kv_split = kv_split(p->B, p->H, p->Hk, p->M, p->N, p->window, p->causal);
     a.n_chunks = c.n;
     a.chunk = c.size;
     const hipError_t e = dfl::launch_window_bwd(a, p->dtype == DFL_BF16, pad_dim(p->d), (hipStream_t)stream);

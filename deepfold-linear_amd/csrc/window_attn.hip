@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
     if ((now == 0) | vis.none(t0, j0, E::BK)) continue;
     f32x16 y[E::NSUB];
 #pragma unroll
-    for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::row_product(tk, 32 * sub, qf, lane);
+    for (int sub = 0; sub < E::NSUB; ++sub) y[sub] = E::template row_product<true>(tk, 32 * sub, qf, lane);
     // log2 of the weights: ya y + yc.  A tile all of whose pairs are visible and get one table value needs no test a
     // pair; else a table value a pair goes into y itself, and what is not visible becomes -inf.
     float ya[E::NSUB], yc[E::NSUB];
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       l += s;
       typename E::Prob p;
       E::to_operand(y[sub], p);
-      E::column_product(tv, 32 * sub, p, acc, lane);
+      E::template column_product<true>(tv, 32 * sub, p, acc, lane);
     }
   }
   l = xor32_pair(l, false);

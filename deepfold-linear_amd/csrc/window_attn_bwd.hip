@@ -248,7 +248,7 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   const int G = a.H / a.Hk, shift = a.N - a.M, kg = wave & 1, half = wave >> 1;
   const WinVis vis(a);
 
-  int bhk, j0, c = 0;
+  int bhk, j0, c = 0, sp = 0;
   if (SINK) {
     const int ngrp = (min(a.n_sink, a.N) + WIN_KEYS - 1) / WIN_KEYS;
     c = x % a.n_chunks;
@@ -257,6 +257,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
     bhk = x / ngrp;
   } else {
     const int nkt = (a.N + WIN_KEYS - 1) / WIN_KEYS;
+    sp = x % a.kv_split;
+    x /= a.kv_split;
     j0 = (x % nkt) * WIN_KEYS + 32 * kg;
     bhk = x / nkt;
   }
@@ -273,7 +275,10 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
     ilo = max(0, k0 - vis.off - shift);
     ihi = min(a.M, k1 - vis.off + (int)vis.range - shift);
   }
-  const int nt = ihi > ilo ? (ihi - ilo + 63) / 64 : 0, total = G * nt;
+  // (head, query tile) pairs, this workgroup's part of them [it0, it1)
+  const int nt = ihi > ilo ? (ihi - ilo + 63) / 64 : 0, all = G * nt;
+  const int it0 = SINK ? 0 : (int)((long long)all * sp / a.kv_split);
+  const int it1 = SINK ? all : (int)((long long)all * (sp + 1) / a.kv_split);
   RowBits<64> rb(mask ? mask + shift : nullptr, a.M);
   float r_lse, r_d, r_f;  // of the next tile's row threadIdx.x
   auto issue = [&](int it, int buf) {
@@ -305,8 +310,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
     }
   };
   if (REL) stage_edges(a.rel, edge);
-  if (n_buf > 1 && total > 0) {
-    issue(0, 0);
+  if (n_buf > 1 && it0 < it1) {
+    issue(it0, 0);
     put_rows(0);
   }
 
@@ -321,8 +326,9 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   f32x16 acc[E::NT] = {};  // half 0: dv, half 1: dk
   // whether any of the wave's keys and the 32 queries from t0 on meet here
   auto meet = [&](int t0) { return SINK ? (j0 < ns) & !vis.all_near(t0, j0) : !vis.none_near(t0, j0); };
-  for (int it = 0; it < total; ++it) {
-    const int buf = it & (n_buf - 1);
+  for (int it = it0; it < it1; ++it) {
+    const int buf = (it - it0) & (n_buf - 1);
+    const bool new_head = REL && (it == it0 || it % nt == 0);
     if (n_buf == 1) {
       __syncthreads();
       issue(it, 0);
@@ -340,9 +346,9 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
       // a masked query's row may have an lse of any value
       if (threadIdx.x < 64 && !((now >> threadIdx.x) & 1u)) srow[buf * 192 + threadIdx.x] = LSE_EMPTY;
     }
-    if (REL && it % nt == 0) build_rel_lut(a, hk * G + it / nt, edge, lut, nullptr);
-    if (now != ~0ull || (REL && it % nt == 0)) __syncthreads();
-    const bool next = n_buf > 1 && it + 1 < total;
+    if (new_head) build_rel_lut(a, hk * G + it / nt, edge, lut, nullptr);
+    if (now != ~0ull || new_head) __syncthreads();
+    const bool next = n_buf > 1 && it + 1 < it1;
     if (next) issue(it + 1, buf ^ 1);
 
     const int tile0 = ilo + it % nt * 64 + shift, t0 = tile0 + 32 * half;
@@ -390,8 +396,10 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   }
   if (j >= (SINK ? ns : a.N)) return;
   const int which = half ? 0 : 1;  // dk before dv in a partial row
-  float* part = nullptr;           // joined by the finalize kernel: the first tokens' rows
-  if (a.n_chunks > 0 && j < ns)
+  float* part = nullptr;           // joined by the finalize kernel: parts of the queries, the first tokens' rows
+  if (!SINK && a.kv_split > 1)
+    part = a.kv_part + (((size_t)sp * a.B * a.Hk + bhk) * a.N + j) * 2 * DP + which * DP;
+  else if (a.n_chunks > 0 && j < ns)
     part = a.sink_part + (((size_t)bhk * (a.n_chunks + 1) + (SINK ? c : a.n_chunks)) * ns + j) * 2 * DP + which * DP;
   T* out = reinterpret_cast<T*>(half ? a.dk : a.dv) + ((size_t)bhk * a.N + j) * a.d;
   const float f = key_ok ? (half ? a.scale : 1.f) : 0.f;
@@ -418,19 +426,24 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
                                        smem);
 }
 
-// The first tokens' rows from their partial sums (band last), and the table's gradient from the query tiles'; a wave
-// for 64 entries of a row or for one table entry, each sum in a fixed order.
+// Rows of dk and dv from their partial sums (parts of the band's queries in order, then the first tokens' chunks),
+// and the table's gradient from the query tiles'; a wave for 64 entries of a row or for one table entry, each sum in
+// a fixed order.
 template <typename T, int DP>
 __global__ void __launch_bounds__(WIN_NT) window_finalize_kernel(WinArgs a, int n_row_waves, int n_tab_waves) {
   const int lane = threadIdx.x & 63;
   int w = blockIdx.x * (WIN_NT / 64) + (threadIdx.x >> 6);
-  const int ns = min(a.n_sink, a.N);
+  const int ns = min(a.n_sink, a.N), rows = a.kv_split > 1 ? a.N : ns;
   if (w < n_row_waves) {
     const int per = 2 * DP / 64, part = w % per;
     w /= per;
-    const int j = w % ns, bhk = w / ns, e = part * 64 + lane, col = e % DP;
-    const float* p = a.sink_part + ((size_t)bhk * (a.n_chunks + 1) * ns + j) * 2 * DP + e;
-    const float s = ordered_sum(p, (size_t)ns * 2 * DP, a.n_chunks + 1, 0.f);
+    const int j = w % rows, bhk = w / rows, e = part * 64 + lane, col = e % DP;
+    float s = 0.f;
+    if (a.kv_split > 1)
+      s = ordered_sum(a.kv_part + ((size_t)bhk * a.N + j) * 2 * DP + e, (size_t)a.B * a.Hk * a.N * 2 * DP, a.kv_split, 0.f);
+    if (a.n_chunks > 0 && j < ns)  // (without a split the last chunk is the band's)
+      s = ordered_sum(a.sink_part + ((size_t)bhk * (a.n_chunks + 1) * ns + j) * 2 * DP + e, (size_t)ns * 2 * DP,
+                      a.n_chunks + (a.kv_split == 1), s);
     const bool ok = !a.mask || a.mask[(size_t)(bhk / a.Hk) * a.N + j] != 0.f;
     T* out = reinterpret_cast<T*>(e < DP ? a.dk : a.dv) + ((size_t)bhk * a.N + j) * a.d;
     if (col < a.d) out[col] = from_f32<T>(ok ? (e < DP ? s * a.scale : s) : 0.f);
@@ -467,9 +480,10 @@ static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(kq, dim3((unsigned)(nqt * a.B * a.H)), dim3(WIN_NT), lq, s, a, n_buf);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int nsb = a.n_chunks > 0 ? a.B * a.Hk * a.n_chunks * ((ns + WIN_KEYS - 1) / WIN_KEYS) : 0;
-  hipLaunchKernelGGL(kkv, dim3((unsigned)(nkt * a.B * a.Hk + nsb)), dim3(WIN_NT), lkv, s, a, nsb, n_kbuf);
+  hipLaunchKernelGGL(kkv, dim3((unsigned)(nkt * a.B * a.Hk * a.kv_split + nsb)), dim3(WIN_NT), lkv, s, a, nsb, n_kbuf);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int rows = a.n_chunks > 0 ? a.B * a.Hk * ns * (2 * DP / 64) : 0, tabs = tab ? a.H * a.rel.buckets() : 0;
+  const int rows = (a.kv_split > 1 ? a.N : a.n_chunks > 0 ? ns : 0) * a.B * a.Hk * (2 * DP / 64);
+  const int tabs = tab ? a.H * a.rel.buckets() : 0;
   if (rows + tabs > 0) {
     hipLaunchKernelGGL((window_finalize_kernel<T, DP>), dim3((unsigned)((rows + tabs + 3) / 4)), dim3(WIN_NT), 0, s, a,
                        rows, tabs);

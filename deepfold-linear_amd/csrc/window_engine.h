@@ -86,11 +86,27 @@ template <typename T, int DP> struct WinEng {
     }
     return c;
   }
+  // A lane's LDS addresses differ by one bit pattern a step (the swizzle is an exclusive or), so one register and
+  // one instruction a read do.  `opaque` keeps them out of the loop-invariant set: the compiler would hold dozens of
+  // them over the loop and spill, and a spilled register's reload waits for the tile loads in flight (key pass 180 ->
+  // 150 us).  HELD: left to it, where there is room (forward 392 -> 372 us at 8192 tokens).
+  __device__ static __forceinline__ unsigned opaque(unsigned x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+  __device__ static __forceinline__ unsigned lds_address(const T* p) {
+    return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) T*)p;
+  }
   // rows r0 .. r0 + 31 of the tile times the resident rows
+  template <bool HELD = false>
   __device__ static __forceinline__ f32x16 row_product(T* tile, int r0, const Frag& f, int lane) {
+    typedef const __attribute__((address_space(3))) u32x4* lptr;
     f32x16 c = {};
+    const int row = lane & 31;  // (r0 a multiple of 32: the same swizzle)
+    const unsigned base = lds_address(tile + r0 * DP);
+    const unsigned own = row * DP * (unsigned)sizeof(T) + 16u * swz(row, lane >> 5), at = HELD ? own : opaque(own);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) c = step(*chunk(tile, r0 + (lane & 31), 2 * s + (lane >> 5)), f.v[s], c);
+    for (int s = 0; s < STEPS; ++s) c = step(*(lptr)(uintptr_t)(base + (at ^ (32u * s))), f.v[s], c);
     // a few LDS reads ahead of the products (the scheduler would rather save their registers and wait for each)
     constexpr int AHEAD = STEPS < 4 ? STEPS : 4, PER = sizeof(T) == 2 ? 1 : 4;
     __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
@@ -118,20 +134,22 @@ template <typename T, int DP> struct WinEng {
     }
   }
   // acc[t] += (columns 32 t .. of rows r0 .. r0 + 31 of the tile)^T P
+  template <bool HELD = false>
   __device__ static __forceinline__ void column_product(T* tile, int r0, const Prob& p, f32x16 (&acc)[NT], int lane) {
     if constexpr (sizeof(T) == 2) {
       typedef __attribute__((address_space(3))) s16x4* lptr;
-      const int h = lane >> 5, q = (lane >> 4) & 1, i = (lane & 15) >> 2, e = lane & 3;
+      const int h = lane >> 5, q = (lane >> 4) & 1, i = (lane & 15) >> 2, e = lane & 3, ra = 4 * h + i;
+      constexpr unsigned RB = DP * 2;  // bytes of a row
+      const unsigned base = lds_address(tile + r0 * DP);
+      // 8 bytes of columns 16 q + 4 e .. of row 4 h + i; the row 8 further down has its chunks exchanged in pairs
+      const unsigned own = ra * RB + 16u * swz(ra, 2 * q + (e >> 1)) + 8u * (e & 1), at = HELD ? own : opaque(own);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          // chunk of columns 32 t + 16 q + 4 e ..: 8 bytes of it
-          const int c = 4 * t + 2 * q + (e >> 1), ra = r0 + 16 * s + 4 * h + i, rb = ra + 8;
-          T* pa = tile + ra * DP + swz(ra, c) * VEC + 4 * (e & 1);
-          T* pb = tile + rb * DP + swz(rb, c) * VEC + 4 * (e & 1);
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)pa);
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)pb);
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)(base + 16 * s * RB + (at ^ (64u * t))));
+          const s16x4 hi =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(uintptr_t)(base + (16 * s + 8) * RB + (at ^ (64u * t + 32u))));
           bf16x8 a;
           __builtin_memcpy(&a, &lo, 8);
           __builtin_memcpy(reinterpret_cast<char*>(&a) + 8, &hi, 8);
