@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   if (REL) {
     stage_edges(a.rel, edge);
     __syncthreads();
-    build_rel_lut(a, h, edge, lut, nullptr);
+    build_rel_lut(a, h, edge, lut);
   }
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;

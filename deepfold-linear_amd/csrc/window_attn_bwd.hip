@@ -42,10 +42,13 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   T* sv = sk + n_buf * E::TILE;
   float* lut = reinterpret_cast<float*>(sv + n_buf * E::TILE);
   int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
-  // sums by bucket, a column for each thread: every address has one writer
-  float* hist = reinterpret_cast<float*>(edge + (REL ? REL_EDGES : 0));
+  // The table's gradient: sums of ds by distance, one row of them a wave (every address has one writer), and where a
+  // wave turns the diagonals of its pairs into columns.
   const bool tab = REL && a.dtable;
-  uint8_t* lutb = reinterpret_cast<uint8_t*>(hist + (tab ? a.rel.buckets() * WIN_NT : 0));
+  const int lutn = REL ? rel_lut_size(a.rel) : 0;
+  float* hist = reinterpret_cast<float*>(edge + (REL ? REL_EDGES : 0));  // [4][lutn]
+  float* skew = hist + (tab ? 4 * lutn : 0);                              // [4][16][64]
+  float* far_sums = skew + (tab ? 4 * 16 * 64 : 0);                       // [4][2]
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform: tile tests are scalar
 
@@ -63,7 +66,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
   RowBits<E::BK> rb(mask, a.N);
   constexpr uint64_t KEYS = RowBits<E::BK>::ALL;
-  // Two buffers, the next tile on its way during this one's products; one where a large table's sums take their room.
+  // Two buffers, the next tile on its way during this one's products; one where a long table's sums take their room.
   auto issue = [&](int it, int buf) {
     const int j0 = kt.tile(it) * E::BK;
     lk.issue(sk + buf * E::TILE, j0);
@@ -74,10 +77,10 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   if (REL) {
     stage_edges(a.rel, edge);
     __syncthreads();
-    build_rel_lut(a, h, edge, lut, tab ? lutb : nullptr);
+    build_rel_lut(a, h, edge, lut);
   }
   if (tab)
-    for (int n = 0; n < a.rel.buckets(); ++n) hist[n * WIN_NT + threadIdx.x] = 0.f;
+    for (int n = threadIdx.x; n < 4 * lutn + 4 * 16 * 64; n += WIN_NT) hist[n] = 0.f;  // (skew behind it)
 
   const int i0 = qt * WIN_RES + wave * 32, t0 = i0 + shift, i = i0 + (lane & 31), t = i + shift;
   const bool row_ok = i < a.M && (!mask || mask[t] != 0.f);
@@ -186,11 +189,22 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             if (far > rel_lut_base(a.rel)) far_past += s;
             else far_next += s;
           } else {
-            const uint8_t* lb = lutb + rel_lut_base(a.rel) + t - js - 4 * h32;
+            // Key row m and query n lie at distance t0 - js + n - m.  16 rows at a time go to LDS with row m moved by
+            // m, so that a column holds one distance: lane x sums column x, distance t0 - js - 16 half - 15 + x.  The
+            // entries that no pair belongs to keep the zeros they start with.  (LDS float additions into sums by
+            // bucket, 16 a lane and pair, took the pass from 30 to 61 us at 2 x 16 heads of 1021 tokens.)
+            float* sw = skew + wave * 16 * 64;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              __hip_atomic_fetch_add(hist + lb[-acc_row(r, 0)] * WIN_NT + threadIdx.x, p[r], __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_WORKGROUP);
+            for (int half = 0; half < 2; ++half) {
+              float* to = sw + (4 * h32) * 64 + (lane & 31) - 4 * h32 + 15;
+#pragma unroll
+              for (int r = 0; r < 8; ++r) to[acc_row(r, 0) * 63] = p[8 * half + r];
+              float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int m = 0; m < 16; ++m) s[m & 3] += sw[m * 64 + lane];
+              float* at = hist + wave * lutn + rel_lut_base(a.rel) + t0 - js - 16 * half - 15 + lane;
+              if (lane < 47) *at += (s[0] + s[1]) + (s[2] + s[3]);
+            }
           }
         }
         typename E::Prob o;
@@ -212,14 +226,27 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   }
   if (tab) {
     const int nb = a.rel.buckets();
-    hist[a.rel.n * WIN_NT + threadIdx.x] += far_past;  // the last bucket of the queries' past ..
-    if (a.rel.both) hist[(nb - 1) * WIN_NT + threadIdx.x] += far_next;  // .. and of their future
+    far_past = wave_sum(far_past);
+    far_next = wave_sum(far_next);
+    if (lane == 0) far_sums[2 * wave] = far_past, far_sums[2 * wave + 1] = far_next;
     __syncthreads();
     float* part = a.tab_part + (((size_t)b * a.H + h) * nqt + qt) * nb;
+    const int base = rel_lut_base(a.rel), ne = a.rel.n;
     for (int n = wave; n < nb; n += WIN_NT / 64) {
-      const f32x4 s = *reinterpret_cast<const f32x4*>(hist + n * WIN_NT + 4 * lane);
-      const float tot = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
-      if (lane == 0) part[n] = tot;
+      // distances mag of bucket n, [lo, hi), at base + mag (past) or base - mag (future)
+      const int k = n <= ne ? n : n - ne - 1, lo = k ? edge[k - 1] : (n <= ne ? 0 : 1);
+      const int hi = k < ne ? edge[k] : (n <= ne ? lutn - base : base + 1);
+      float s = 0.f;
+      for (int mag = lo + lane; mag < hi; mag += 64) {
+        const float* at = hist + (n <= ne ? base + mag : base - mag);
+        s += (at[0] + at[lutn]) + (at[2 * lutn] + at[3 * lutn]);
+      }
+      s = wave_sum(s);
+      if (k == ne) {
+        const float* f4 = far_sums + (n <= ne ? 0 : 1);
+        s += (f4[0] + f4[2]) + (f4[4] + f4[6]);
+      }
+      if (lane == 0) part[n] = s;
     }
   }
 }
@@ -346,7 +373,7 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
       // a masked query's row may have an lse of any value
       if (threadIdx.x < 64 && !((now >> threadIdx.x) & 1u)) srow[buf * 192 + threadIdx.x] = LSE_EMPTY;
     }
-    if (new_head) build_rel_lut(a, hk * G + it / nt, edge, lut, nullptr);
+    if (new_head) build_rel_lut(a, hk * G + it / nt, edge, lut);
     if (now != ~0ull || new_head) __syncthreads();
     const bool next = n_buf > 1 && it + 1 < it1;
     if (next) issue(it + 1, buf ^ 1);
@@ -465,7 +492,7 @@ static hipError_t bwd_launch(const WinArgs& a, hipStream_t s) {
   using E = WinEng<T, DP>;
   const size_t lutn = REL ? rel_lut_size(a.rel) : 0, rel = REL ? (lutn + REL_EDGES) * 4 : 0;
   const bool tab = REL && a.dtable;
-  const size_t lq1 = rel + (tab ? a.rel.buckets() * WIN_NT * 4 + lutn : 0), buf = 2 * E::TILE * sizeof(T);
+  const size_t lq1 = rel + (tab ? (4 * lutn + 4 * 16 * 64 + 8) * 4 : 0), buf = 2 * E::TILE * sizeof(T);
   const int n_buf = lq1 + 2 * buf <= 160 * 1024 ? 2 : 1;
   const size_t lq = lq1 + n_buf * buf;
   const size_t lkv1 = 4 * 64 * sizeof(typename E::Prob) + 2 * 3 * 64 * 4 + rel, kbuf = 2 * 64 * DP * sizeof(T);

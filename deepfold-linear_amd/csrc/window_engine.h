@@ -238,13 +238,11 @@ __device__ __forceinline__ int rel_bucket_lds(const int* edge, int n, int both, 
 __device__ __forceinline__ void stage_edges(const RelSpec& r, int* edge) {
   if ((int)threadIdx.x < r.n) edge[threadIdx.x] = r.edge[threadIdx.x];
 }
-__device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, const int* edge, float* lut, uint8_t* bucket) {
+__device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, const int* edge, float* lut) {
   const int n = rel_lut_size(a.rel), base = rel_lut_base(a.rel);
   const float* row = a.table + (size_t)h * a.rel.buckets();
   for (int x = threadIdx.x; x < n; x += blockDim.x) {
-    const int b = rel_bucket_lds(edge, a.rel.n, a.rel.both, base - x);
-    lut[x] = row[b] * LOG2E;
-    if (bucket) bucket[x] = (uint8_t)b;
+    lut[x] = row[rel_bucket_lds(edge, a.rel.n, a.rel.both, base - x)] * LOG2E;
   }
 }
 // Where every distance t - j of 32 queries and n keys lies beyond the table's range: the index of its one value, else -1.
