@@ -159,8 +159,9 @@ dfl::WinArgs attn_args(const dfl_window_attn_params* p) {
   return a;
 }
 
-// Splits of a cache: enough workgroups to fill the chip about four times over, at least 64 slots each.
-constexpr int DECODE_WG = 1024, DECODE_MIN = 64;
+// Splits of a cache: about three workgroups a CU, what its registers let run at once (with 1024 a second, mostly empty
+// round follows), at least 64 slots each.
+constexpr int DECODE_WG = 768, DECODE_MIN = 64;
 struct Splits {
   int n, chunk;
   Splits(int B, int H, int Hk, int S) {

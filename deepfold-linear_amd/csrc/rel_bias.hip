@@ -56,6 +56,13 @@ template <bool POS> struct RelPlane {
 struct PlaneWalk {
   int i, j, di, dj, N;
   __device__ __forceinline__ PlaneWalk(size_t first, size_t step, int n) : N(n) {
+    if ((first | step) < (1ull << 32)) {  // 64-bit divisions take a microsecond
+      i = (int)((unsigned)first / (unsigned)n);
+      j = (int)((unsigned)first - (unsigned)i * n);
+      di = (int)((unsigned)step / (unsigned)n);
+      dj = (int)((unsigned)step - (unsigned)di * n);
+      return;
+    }
     i = (int)(first / n);
     j = (int)(first - (size_t)i * n);
     di = (int)(step / n);
@@ -191,8 +198,8 @@ __global__ void __launch_bounds__(256) rel_bias_sum_kernel(RelBiasArgs a) {
 hipError_t launch_rel_bias_fwd(const RelBiasArgs& a, bool bf16_out, hipStream_t s) {
   const int vec = bf16_out ? 8 : 4, lut = bucket_lut_size(a.rel);
   const size_t per = 256 * (size_t)vec, plane = (size_t)a.M * a.N;
-  // at most about 8 workgroups a CU in all: each builds its lookup table once
-  const unsigned nx = (unsigned)std::min<size_t>((plane + per - 1) / per, std::max(1, 2048 / a.B));
+  // at most about 4 workgroups a CU in all: each builds its lookup table once
+  const unsigned nx = (unsigned)std::min<size_t>((plane + per - 1) / per, std::max(1, 1024 / a.B));
   const size_t lds = lut + REL_EDGES * 4 + (size_t)std::min(a.H, 64) * a.rel.buckets() * 4;
   auto kern = a.q_pos ? (bf16_out ? rel_bias_fwd_kernel<bf16, true> : rel_bias_fwd_kernel<float, true>)
                       : (bf16_out ? rel_bias_fwd_kernel<bf16, false> : rel_bias_fwd_kernel<float, false>);
@@ -200,9 +207,9 @@ hipError_t launch_rel_bias_fwd(const RelBiasArgs& a, bool bf16_out, hipStream_t 
   return hipGetLastError();
 }
 
-// Parts of a plane: about 8 workgroups a CU in all, at least one round of vectors each.
+// Parts of a plane: about 4 workgroups a CU in all, at least one round of vectors each.
 int rel_bias_parts(int B, int H, int M, int N) {
-  const size_t n = (size_t)M * N, want = std::max<size_t>(1, 2048 / ((size_t)B * H));
+  const size_t n = (size_t)M * N, want = std::max<size_t>(1, 1024 / ((size_t)B * H));
   return (int)std::max<size_t>(1, std::min<size_t>(want, (n + 4095) / 4096));
 }
 

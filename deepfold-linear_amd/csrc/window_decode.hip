@@ -46,6 +46,8 @@ template <int L> __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
+constexpr int DEC_U = 4;
+
 // One (sample, key head, group of up to GB query heads, split of the slots) a workgroup.  L lanes hold a row, 16
 // bytes each; a wave takes 64 / L rows at a time, each lane group with a running reference, sum and output of its
 // own, joined in LDS at the end.
@@ -92,33 +94,63 @@ __global__ void __launch_bounds__(256) window_decode_kernel(DecodeArgs a) {
   const T* kn = reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh;
   const T* vn = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh;
   const int s1 = min(used, (sp + 1) * a.chunk);
-  for (int s = sp * a.chunk + rg; s < s1; s += NG) {
-    const bool mine = s == own;
-    const T* kr = mine ? kn : kc + (size_t)s * a.kcsn;
-    const T* vr = mine ? vn : vc + (size_t)s * a.vcsn;
-    const u32x4 kw = E::template load<FAST>(kr, c, a.d), vw = E::template load<FAST>(vr, c, a.d);
-    T ke[VEC], ve[VEC];
-    __builtin_memcpy(ke, &kw, 16);
-    __builtin_memcpy(ve, &vw, 16);
-    if (mine && hg == 0) {  // the token enters the cache; no workgroup reads its slot
+  // DEC_U rows of a lane group at a time: their loads in flight together, one move of the reference for all
+  for (int s0 = sp * a.chunk + rg; s0 < s1; s0 += NG * DEC_U) {
+    u32x4 kw[DEC_U], vw[DEC_U];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (c * VEC + i < a.d) kc[(size_t)s * a.kcsn + c * VEC + i] = ke[i], vc[(size_t)s * a.vcsn + c * VEC + i] = ve[i];
+    for (int u = 0; u < DEC_U; ++u) {
+      const int s = min(s0 + u * NG, s1 - 1);
+      const bool mine = s == own;
+      kw[u] = E::template load<FAST>(mine ? kn : kc + (size_t)s * a.kcsn, c, a.d);
+      vw[u] = E::template load<FAST>(mine ? vn : vc + (size_t)s * a.vcsn, c, a.d);
     }
-    int bk = 0;
-    if (REL) bk = s_lut[min(t - slot_position(s, t, a.n_sink, a.window), a.rel.dist())];
+    float y[DEC_U][GB];
+#pragma unroll
+    for (int u = 0; u < DEC_U; ++u) {
+      const int s = s0 + u * NG;
+      T ke[VEC];
+      __builtin_memcpy(ke, &kw[u], 16);
+      int bk = 0;
+      if (REL) bk = s_lut[min(t - slot_position(min(s, s1 - 1), t, a.n_sink, a.window), a.rel.dist())];
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x = __builtin_fmaf(q[g][i], to_f32(ke[i]), x);
+        x = row_sum<L>(x);
+        if (REL) x += s_tab[min(g, gn - 1) * a.rel.buckets() + bk];
+        y[u][g] = s < s1 ? x : -INFINITY;
+      }
+      if (s == own && s < s1 && hg == 0) {  // the token enters the cache; no workgroup reads its slot
+        T ve[VEC];
+        __builtin_memcpy(ve, &vw[u], 16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (c * VEC + i < a.d) kc[(size_t)s * a.kcsn + c * VEC + i] = ke[i], vc[(size_t)s * a.vcsn + c * VEC + i] = ve[i];
+      }
+    }
 #pragma unroll
     for (int g = 0; g < GB; ++g) {
-      float y = 0.f;
+      float mx = m[g];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) y = __builtin_fmaf(q[g][i], to_f32(ke[i]), y);
-      y = row_sum<L>(y);
-      if (REL) y += s_tab[min(g, gn - 1) * a.rel.buckets() + bk];
-      const float mx = fmaxf(m[g], y), al = fast_exp2(m[g] - mx), p = fast_exp2(y - mx);
+      for (int u = 0; u < DEC_U; ++u) mx = fmaxf(mx, y[u][g]);
+      const float al = fast_exp2(m[g] - mx);
       m[g] = mx;
-      l[g] = l[g] * al + p;
+      l[g] *= al;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) o[g][i] = __builtin_fmaf(p, to_f32(ve[i]), o[g][i] * al);
+      for (int i = 0; i < VEC; ++i) o[g][i] *= al;
+    }
+#pragma unroll
+    for (int u = 0; u < DEC_U; ++u) {
+      T ve[VEC];
+      __builtin_memcpy(ve, &vw[u], 16);
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        const float p = fast_exp2(y[u][g] - m[g]);
+        l[g] += p;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[g][i] = __builtin_fmaf(p, to_f32(ve[i]), o[g][i]);
+      }
     }
   }
 #pragma unroll
@@ -152,21 +184,40 @@ __global__ void __launch_bounds__(256) window_decode_kernel(DecodeArgs a) {
   }
 }
 
-// The splits' outputs joined, in split order: a workgroup a head.
-template <typename T, int DP> __global__ void __launch_bounds__(DP) window_decode_join_kernel(DecodeArgs a) {
+// The splits' outputs joined, in split order: a workgroup a head, a wave or more, the splits' references and sums in
+// LDS first so that the loop over the outputs has only independent loads.
+template <typename T, int DP> __global__ void __launch_bounds__(128) window_decode_join_kernel(DecodeArgs a) {
+  extern __shared__ float s_w[];  // [n_split] weights
   const size_t head = blockIdx.x;
-  const int col = threadIdx.x;
   const float* part = a.part + head * a.n_split * (DP + 2);
   float mx = NEG_BIG;
-  for (int s = 0; s < a.n_split; ++s) mx = fmaxf(mx, part[(size_t)s * (DP + 2)]);
-  float sl = 0.f, so = 0.f;
-  for (int s = 0; s < a.n_split; ++s) {
-    const float* p = part + (size_t)s * (DP + 2);
-    const float al = fast_exp2(p[0] - mx);
-    sl = __builtin_fmaf(p[1], al, sl);
-    so = __builtin_fmaf(p[2 + col], al, so);
+  for (int s = threadIdx.x; s < a.n_split; s += 128) mx = fmaxf(mx, s_w[s] = part[(size_t)s * (DP + 2)]);
+  __shared__ float s_red[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, WAVE));
+  if (lane == 0) s_red[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(s_red[0], s_red[1]);
+  float l = 0.f;
+  for (int s = threadIdx.x; s < a.n_split; s += 128) {
+    s_w[s] = fast_exp2(s_w[s] - mx);
+    l = __builtin_fmaf(s_w[s], part[(size_t)s * (DP + 2) + 1], l);
   }
-  if (col < a.d) reinterpret_cast<T*>(a.o)[head * a.d + col] = from_f32<T>(sl > 0.f ? so / sl : 0.f);
+  l = wave_sum(l);
+  if (lane == 0) s_red[2 + wave] = l;
+  __syncthreads();
+  l = s_red[2] + s_red[3];
+  const int col = threadIdx.x;
+  if (col >= a.d) return;
+  float o = 0.f;
+  for (int s0 = 0; s0 < a.n_split; s0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = s0 + k < a.n_split ? part[(size_t)(s0 + k) * (DP + 2) + 2 + col] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o = __builtin_fmaf(v[k], s0 + k < a.n_split ? s_w[s0 + k] : 0.f, o);
+  }
+  reinterpret_cast<T*>(a.o)[head * a.d + col] = from_f32<T>(l > 0.f ? o / l : 0.f);
 }
 
 template <typename T> static bool aligned(const void* p, std::initializer_list<long long> strides) {
@@ -199,7 +250,7 @@ template <typename T, int DP, int GB, bool FAST, bool REL> static hipError_t dec
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)(a.B * a.Hk * nhg * a.n_split)), dim3(256), lds, s, a);
   if ((e = hipGetLastError()) != hipSuccess || a.n_split == 1) return e;
-  hipLaunchKernelGGL((window_decode_join_kernel<T, DP>), dim3((unsigned)(a.B * a.H)), dim3(DP), 0, s, a);
+  hipLaunchKernelGGL((window_decode_join_kernel<T, DP>), dim3((unsigned)(a.B * a.H)), dim3(128), a.n_split * 4, s, a);
   return hipGetLastError();
 }
 template <typename T, int DP, int GB> static hipError_t decode_g(const DecodeArgs& a, bool fast, hipStream_t s) {
