@@ -38,9 +38,9 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   const WinVis vis(a);
 
   const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
-  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
-  lk.issue(sk, kt.tile(0) * E::BK);
-  lv.issue(sv, kt.tile(0) * E::BK);
+  const RowLoader<T, DP, FAST> lk(a.ksn, a.N, a.d), lv(a.vsn, a.N, a.d);
+  lk.issue(kb, sk, kt.tile(0) * E::BK);
+  lv.issue(vb, sv, kt.tile(0) * E::BK);
   RowBits<E::BK> rb(mask, a.N);
   rb.fetch(kt.tile(0) * E::BK);
   if (REL) {
@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
     }
     if (it + 1 < kt.total) {
       const int j1 = kt.tile(it + 1) * E::BK;
-      lk.issue(sk + (buf ^ 1) * E::TILE, j1);
-      lv.issue(sv + (buf ^ 1) * E::TILE, j1);
+      lk.issue(kb, sk + (buf ^ 1) * E::TILE, j1);
+      lv.issue(vb, sv + (buf ^ 1) * E::TILE, j1);
       rb.fetch(j1);
     }
     if ((now == 0) | vis.none(t0, j0, E::BK)) continue;

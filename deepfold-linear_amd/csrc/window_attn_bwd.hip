@@ -63,14 +63,14 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   const float* mask = a.mask ? a.mask + (size_t)b * a.N : nullptr;
   const WinVis vis(a);
   const KeyTiles kt(a, qt * WIN_RES + shift, min(a.M, (qt + 1) * WIN_RES) - 1 + shift, E::BK);
-  const RowLoader<T, DP, FAST> lk(kb, a.ksn, a.N, a.d), lv(vb, a.vsn, a.N, a.d);
+  const RowLoader<T, DP, FAST> lk(a.ksn, a.N, a.d), lv(a.vsn, a.N, a.d);
   RowBits<E::BK> rb(mask, a.N);
   constexpr uint64_t KEYS = RowBits<E::BK>::ALL;
   // Two buffers, the next tile on its way during this one's products; one where a long table's sums take their room.
   auto issue = [&](int it, int buf) {
     const int j0 = kt.tile(it) * E::BK;
-    lk.issue(sk + buf * E::TILE, j0);
-    lv.issue(sv + buf * E::TILE, j0);
+    lk.issue(kb, sk + buf * E::TILE, j0);
+    lv.issue(vb, sv + buf * E::TILE, j0);
     rb.fetch(j0);
   };
   if (n_buf > 1) issue(0, 0);
@@ -306,13 +306,14 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   const int nt = ihi > ilo ? (ihi - ilo + 63) / 64 : 0, all = G * nt;
   const int it0 = SINK ? 0 : (int)((long long)all * sp / a.kv_split);
   const int it1 = SINK ? all : (int)((long long)all * (sp + 1) / a.kv_split);
+  const RowLoader<T, DP, FAST> lq(a.qsn, a.M, a.d), lg(a.d, a.M, a.d);
   RowBits<64> rb(mask ? mask + shift : nullptr, a.M);
   float r_lse, r_d, r_f;  // of the next tile's row threadIdx.x
   auto issue = [&](int it, int buf) {
     const int h = hk * G + it / nt, i0 = ilo + it % nt * 64;
     const size_t row0 = ((size_t)b * a.H + h) * a.M;
-    const RowLoader<T, DP, FAST> lq(reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh, a.qsn, a.M, a.d);
-    const RowLoader<T, DP, FAST> lg(reinterpret_cast<const T*>(a.go) + row0 * a.d, a.d, a.M, a.d);
+    const T* qb = reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh;
+    const T* gb = reinterpret_cast<const T*>(a.go) + row0 * a.d;
     rb.fetch(i0);
     if (threadIdx.x < 64) {
       const int i = i0 + threadIdx.x;
@@ -324,8 +325,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
     }
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      lq.issue(sq + buf * TILE + n * E::TILE, i0 + n * E::BK);
-      lg.issue(sg + buf * TILE + n * E::TILE, i0 + n * E::BK);
+      lq.issue(qb, sq + buf * TILE + n * E::TILE, i0 + n * E::BK);
+      lg.issue(gb, sg + buf * TILE + n * E::TILE, i0 + n * E::BK);
     }
   };
   auto put_rows = [&](int buf) {

@@ -41,26 +41,24 @@ template <typename T, int DP, bool FAST> struct RowLoader {
   using E = WinEng<T, DP>;
   static constexpr int PER = E::BK * E::NCH / WIN_NT;  // chunks of a thread
   static constexpr int STEP = WIN_NT / E::NCH;         // rows between them
-  const T* base;
-  const T* mine;  // this thread's chunk of row 0 .. of the tile at row 0
-  long long stride;
+  long long stride, mine;  // mine: this thread's chunk of the rows from 0 on, in elements
   int N, d;
   __device__ __forceinline__ static int column(int row, int pos, int d) {
     const int c = E::swz(row, pos) * E::VEC;
     return c < d ? c : 0;
   }
-  __device__ __forceinline__ RowLoader(const T* b, long long s, int n, int dim) : base(b), stride(s), N(n), d(dim) {
+  __device__ __forceinline__ RowLoader(long long s, int n, int dim) : stride(s), N(n), d(dim) {
     const int r = threadIdx.x / E::NCH;
-    mine = base + r * stride + column(r, threadIdx.x % E::NCH, d);
+    mine = r * stride + column(r, threadIdx.x % E::NCH, d);
   }
-  __device__ __forceinline__ void issue(T* tile, int j0) const {
+  __device__ __forceinline__ void issue(const T* base, T* tile, int j0) const {
     const int r = threadIdx.x / E::NCH, pos = threadIdx.x % E::NCH;
     if constexpr (FAST) {
-      const unsigned to = __builtin_amdgcn_readfirstlane(
-          (unsigned)(uintptr_t)(__attribute__((address_space(3))) T*)(tile + (threadIdx.x & ~63u) * E::VEC));
+      const unsigned to = __builtin_amdgcn_readfirstlane(E::lds_address(tile + (threadIdx.x & ~63u) * E::VEC));
       if (STEP % 16 == 0 && j0 + E::BK <= N) {  // one column for all of the thread's rows
+        const T* from = base + j0 * stride + mine;
 #pragma unroll
-        for (int n = 0; n < PER; ++n) load_to_lds(mine + (j0 + n * STEP) * stride, to + n * WIN_NT * 16);
+        for (int n = 0; n < PER; ++n, from += STEP * stride) load_to_lds(from, to + n * WIN_NT * 16);
       } else {
 #pragma unroll
         for (int n = 0; n < PER; ++n) {
