@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
             // Key row m and query n lie at distance t0 - js + n - m.  16 rows at a time go to LDS with row m moved by
             // m, so that a column holds one distance: lane x sums column x, distance t0 - js - 16 half - 15 + x.  The
             // entries that no pair belongs to keep the zeros they start with.  (LDS float additions into sums by
-            // bucket, 16 a lane and pair, took the pass from 30 to 61 us at 2 x 16 heads of 1021 tokens.)
+            // bucket, 16 a lane and pair, made the pass 61 us instead of 31 at 2 x 16 heads of 1021 tokens.)
             float* sw = skew + wave * 16 * 64;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -255,7 +255,9 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
 // Wave (kg, half) forms p and ds of 32 keys (group kg) and 32 of the staged queries (`half`), and sums one result over
 // all of them: half 0 dv, half 1 dk.  So each hands the other half one operand through LDS (p or ds, in bf16 for bf16)
 // and keeps one accumulator, not two: 256 registers a lane and two workgroups a CU, where both sums in every wave took
-// 474 registers and left each matrix instruction's latency uncovered (196 us against PLACEHOLDER at 4096 tokens).
+// 474 registers and left each matrix instruction's latency uncovered (196 us against 171 at 16 / 4 heads of 4096 tokens,
+// d 128, window 1024, one workgroup a key tile; 146 with two, kv_split).  What bounds it now is the mix of a step: 32
+// matrix instructions, 250 others and two barriers a wave, at two waves a SIMD about half of the time in none.
 // SINK: 64 of the first tokens' keys against a chunk of the queries outside their band.
 constexpr int WIN_KEYS = 64;
 

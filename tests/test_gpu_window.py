@@ -106,6 +106,44 @@ def test_attention_masked(causal, dtype):
     assert torch.equal(o2, o) and all(torch.equal(a, b) for a, b in zip(g2, grads))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_masked_long(dtype):
+    """Key tiles whose queries are split over workgroups, with holes in the mask and first tokens among them."""
+    mask = (torch.rand(2, 650, generator=torch.Generator().manual_seed(9)) < 0.8).float()
+    mask[0, 400:] = 0
+    attention_case(2, 4, 1, 650, 650, 64, dtype, 300, 5, True, True, mask=mask)
+    attention_case(2, 4, 1, 600, 650, 128, dtype, 300, 5, False, False, mask=mask)
+
+
+def test_offsets_beyond_32_bits():
+    """Samples, and slots of a cache, more than 2^31 elements apart."""
+    from deepfold_amd import flash_window_attn, window_cache_fill, window_decode_attn
+
+    far, H, N, d, S = 2**31 + 64, 2, 40, 64, 24
+    big = torch.empty(far + 8 * N * d * 4, dtype=BF, device=DEV)
+    view = lambda at, *shape: big[at:].as_strided((2, *shape), (far, *torch.empty(shape, device="meta").stride()))
+    K, V = view(0, H, N, d), view(H * N * d, H, N, d)
+    q, k, v = (rnd(2, H, N, d, seed=s, dtype=BF).to(DEV) for s in (1, 2, 3))
+    K.copy_(k), V.copy_(v)
+    assert torch.equal(flash_window_attn(q, K, V, window=9, n_sink=2), flash_window_attn(q, k, v, window=9, n_sink=2))
+    got, want = [view(2 * H * N * d, H, S, d), view(3 * H * N * d, H, S, d)], [torch.zeros(2, H, S, d, dtype=BF, device=DEV) for _ in "kv"]
+    for c in got:
+        c.zero_()
+    lengths = torch.tensor([N, 7], device=DEV)
+    window_cache_fill(K, V, lengths, *got, n_sink=2)
+    window_cache_fill(k, v, lengths, *want, n_sink=2)
+    o = [window_decode_attn(q[:, :, 0], k[:, :, 1], v[:, :, 1], *c, lengths, n_sink=2) for c in (got, want)]
+    assert torch.equal(*o) and all(torch.equal(a, b) for a, b in zip(got, want))
+    # slots far apart
+    wide = big.as_strided((1, 1, 2, d), (0, 0, far, 1)), big[d:].as_strided((1, 1, 2, d), (0, 0, far, 1))
+    near = [torch.zeros(1, 1, 2, d, dtype=BF, device=DEV) for _ in "kv"]
+    for a, b in zip(wide, near):
+        a.copy_(b)
+    for c in (wide, near):
+        window_cache_fill(k[:1, :1], v[:1, :1], lengths[:1], *c)
+    assert all(torch.equal(a, b) and a.any() for a, b in zip(wide, near))
+
+
 def test_one_key_rows_have_no_score_gradient():
     """Where every row sees one key, the weights are one and dq, dk and the table's gradient exactly zero."""
     from deepfold_amd import flash_window_attn

@@ -244,7 +244,7 @@ def test_c_entries_refuse():
                       (dict(window=0), "window"), (dict(n_sink=129), "n_sink"), (dict(q=None), "NULL"), (dict(scale=0.0), "scale"), (dict(scale=math.inf), "scale"),
                       (dict(rel_table=fake), "together"),
                       (dict(rel_table=fake, rel_edges=ctypes.addressof(flat), n_edges=2), "ascend"),
-                      (dict(N=1 << 29, M=1), "M <= N")):
+                      (dict(N=1 << 29, M=1), "M <= N"), (dict(B=1 << 21), "too large")):
         p = _lib.WindowAttnParams(**{**good, **bad})
         assert lib.dfl_window_attn_fwd(ctypes.byref(p), None) < 0
         assert text in lib.dfl_last_error().decode(), bad
