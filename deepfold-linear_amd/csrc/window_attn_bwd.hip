@@ -20,7 +20,8 @@ namespace dfl {
 constexpr int WIN_EXACT_KEYS = 256;
 
 template <typename T, int DP>
-__device__ __forceinline__ float frag_dot(const typename WinEng<T, DP>::Frag& x, const typename WinEng<T, DP>::Frag& y) {
+__device__ __forceinline__ float frag_dot(const typename WinEng<T, DP>::Frag& x,
+                                          const typename WinEng<T, DP>::Frag& y) {
   using E = WinEng<T, DP>;
   float s = 0.f;
 #pragma unroll
@@ -35,7 +36,8 @@ __device__ __forceinline__ float frag_dot(const typename WinEng<T, DP>::Frag& x,
 }
 
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) window_bwd_q_kernel(WinArgs a, int n_buf) {
+__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+    window_bwd_q_kernel(WinArgs a, int n_buf) {
   using E = WinEng<T, DP>;
   extern __shared__ __align__(16) unsigned char smem[];
   T* sk = reinterpret_cast<T*>(smem);  // [n_buf] key tiles, [n_buf] value tiles
@@ -268,8 +270,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   constexpr int TILE = 64 * DP;
   T* sq = reinterpret_cast<T*>(smem);  // [n_buf] query tiles, [n_buf] tiles of their output's gradient
   T* sg = sq + n_buf * TILE;
-  typename E::Prob* xch = reinterpret_cast<typename E::Prob*>(sg + n_buf * TILE);  // [kg][half][64]: operands handed over
-  float* srow = reinterpret_cast<float*>(xch + 4 * 64);                         // [2][3][64]: lse, D, factor
+  typename E::Prob* xch = reinterpret_cast<typename E::Prob*>(sg + n_buf * TILE);  // [kg][half][64]: operands
+  float* srow = reinterpret_cast<float*>(xch + 4 * 64);                            // [2][3][64]: lse, D, factor
   float* lut = srow + 2 * 3 * 64;
   int* edge = reinterpret_cast<int*>(lut + (REL ? rel_lut_size(a.rel) : 0));
   const int lane = threadIdx.x & 63, h32 = lane >> 5;
@@ -447,7 +449,8 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
 }
 
 template <typename T, int DP, bool FAST, bool REL>
-__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) window_bwd_kv_kernel(WinArgs a, int n_sink_blocks, int n_buf) {
+__global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+    window_bwd_kv_kernel(WinArgs a, int n_sink_blocks, int n_buf) {
   extern __shared__ __align__(16) unsigned char smem[];
   if ((int)blockIdx.x < n_sink_blocks)
     bwd_kv<T, DP, FAST, REL, true>(a, blockIdx.x, n_buf, smem);
@@ -470,7 +473,8 @@ __global__ void __launch_bounds__(WIN_NT) window_finalize_kernel(WinArgs a, int 
     const int j = w % rows, bhk = w / rows, e = part * 64 + lane, col = e % DP;
     float s = 0.f;
     if (a.kv_split > 1)
-      s = ordered_sum(a.kv_part + ((size_t)bhk * a.N + j) * 2 * DP + e, (size_t)a.B * a.Hk * a.N * 2 * DP, a.kv_split, 0.f);
+      s = ordered_sum(a.kv_part + ((size_t)bhk * a.N + j) * 2 * DP + e, (size_t)a.B * a.Hk * a.N * 2 * DP,
+                      a.kv_split, 0.f);
     if (a.n_chunks > 0 && j < ns)  // (without a split the last chunk is the band's)
       s = ordered_sum(a.sink_part + ((size_t)bhk * (a.n_chunks + 1) * ns + j) * 2 * DP + e, (size_t)ns * 2 * DP,
                       a.n_chunks + (a.kv_split == 1), s);

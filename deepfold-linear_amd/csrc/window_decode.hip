@@ -130,7 +130,10 @@ __global__ void __launch_bounds__(256) window_decode_kernel(DecodeArgs a) {
         __builtin_memcpy(ve, &vw[u], 16);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-          if (c * VEC + i < a.d) kc[(size_t)s * a.kcsn + c * VEC + i] = ke[i], vc[(size_t)s * a.vcsn + c * VEC + i] = ve[i];
+          if (c * VEC + i < a.d) {
+            kc[(size_t)s * a.kcsn + c * VEC + i] = ke[i];
+            vc[(size_t)s * a.vcsn + c * VEC + i] = ve[i];
+          }
       }
     }
 #pragma unroll
