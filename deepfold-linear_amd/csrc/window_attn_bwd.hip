@@ -14,7 +14,7 @@
 
 namespace dfl {
 
-// Queries a tile of which sees at most this many keys take D_i as the sum of p dp in a pass of its own over them
+// Tiles of queries that see at most this many keys each take D_i as the sum of p dp in a pass of its own over them
 // (two products more), so that it holds no rounding of the stored o: where a row has few keys, o's rounding would
 // be as large in ds as ds itself.  With more keys o is small against v and do.o is as good.
 constexpr int WIN_EXACT_KEYS = 256;
@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   E::template load_frag<FAST>(gf, row_ok ? reinterpret_cast<const T*>(a.go) + row * a.d : nullptr, a.d, lane);
   const float sc = a.scale * LOG2E;
   const float lse = row_ok ? a.lse[row] : LSE_EMPTY;
-  const bool exact = kt.total * E::BK <= WIN_EXACT_KEYS;
+  const int near = min(a.window, a.N), last = a.causal ? min(a.M, (qt + 1) * WIN_RES) + shift : a.N;
+  const bool exact = min((a.causal ? near : 2 * near - 1) + min(a.n_sink, a.N), last) <= WIN_EXACT_KEYS;
   float D = 0.f, f = 1.f;
   if (!exact) {
     typename E::Frag of;
