@@ -12,6 +12,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdfl_amd.so")
@@ -381,6 +382,15 @@ def require_gpu(*tensors) -> torch.device:
     if dev is None:
         raise RuntimeError("deepfold_amd: no tensor inputs")
     return dev
+
+
+def through_autograd(*tensors) -> bool:
+    """Whether a call must go through its ``autograd.Function`` rather than straight to the launch: an input asks for a
+    gradient, a trace is being recorded (it holds a Function's call, but not what a launch writes), or forward-mode
+    differentiation is on (a Function refuses inputs with tangents, a launch would drop them)."""
+    if torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 class on_device:

@@ -176,8 +176,7 @@ def flash_window_attn(
     if B == 0 or H == 0 or M == 0:
         _lib.require_gpu(Q, K, V)
         raise ValueError("flash_window_attn: empty batch, heads or queries")
-    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad or
-                                    (rel_table is not None and rel_table.requires_grad)):
+    if _lib.through_autograd(Q, K, V, rel_table):
         O = WindowAttnFn.apply(Q, K, V, rel_table, mask, arr, window, n_sink, causal, scale)
     else:
         O = _forward(Q, K, V, rel_table, mask, arr, window, n_sink, causal, scale, False)[1]
@@ -211,15 +210,74 @@ def _check_caches(what, k_cache, v_cache, B, Hk, d, dtype, n_sink):
     return window
 
 
-def _lengths(what, lengths, B):
+def _check_lengths(what, lengths, B):
     if lengths.shape != (B,) or lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: lengths must be ({B},) int32 or int64")
+
+
+def _lengths(lengths):
     return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else lengths.to(torch.int32).contiguous()
 
 
 def _no_grad_inputs(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or train with flash_window_attn")
+
+
+def _fill(K, V, lengths, k_cache, v_cache, n_sink):
+    B, Hk, N, d = K.shape
+    dev, at = K.device, _lengths(lengths)
+    k, v = _unit_inner(K.detach()), _unit_inner(V.detach())
+    p = _lib.WindowCacheFillParams(
+        _lib.DFL_BF16 if K.dtype == torch.bfloat16 else _lib.DFL_F32, k.data_ptr(), v.data_ptr(), *k.stride()[:3],
+        *v.stride()[:3], at.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3],
+        *v_cache.stride()[:3], B, Hk, N, d, k_cache.shape[2] - n_sink, n_sink)
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        rc = _lib.timed_launch("window_cache_fill", dev, lambda: lib.dfl_window_cache_fill(
+            ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
+    _lib.check(rc, "dfl_window_cache_fill")
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+
+
+def _decode(q, k, v, k_cache, v_cache, lengths, rel_table, arr, n_sink, scale):
+    B, H, d = q.shape
+    Hk, window = k.shape[1], k_cache.shape[2] - n_sink
+    dev, at = q.device, _lengths(lengths)
+    tab = None if rel_table is None else rel_table.detach().to(torch.float32).contiguous()
+    q, k, v = _unit_inner(q.detach()), _unit_inner(k.detach()), _unit_inner(v.detach())
+    o = torch.empty(B, H, d, dtype=q.dtype, device=dev)
+    lib = _lib.load()
+    nbytes = lib.dfl_window_decode_workspace_size(B, H, Hk, d, window, n_sink)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    p = _lib.WindowDecodeParams(
+        _lib.DFL_BF16 if q.dtype == torch.bfloat16 else _lib.DFL_F32, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
+        *k_cache.stride()[:3], *v_cache.stride()[:3], at.data_ptr(), _lib.ptr(tab),
+        None if arr is None else ctypes.addressof(arr), 0 if arr is None else len(arr), B, H, Hk, d, window, n_sink,
+        scale, o.data_ptr())
+    with _lib.on_device(dev):
+        rc = _lib.timed_launch("window_decode_attn", dev, lambda: lib.dfl_window_decode(
+            ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
+    _lib.check(rc, "dfl_window_decode")
+    torch.autograd.graph.increment_version((k_cache, v_cache))
+    return o
+
+
+class _CacheFillFn(torch.autograd.Function):
+    """A fill as a node of a trace, without a gradient."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        _fill(*args)
+
+
+class _DecodeFn(torch.autograd.Function):
+    """A token's step as a node of a trace, without a gradient."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _decode(*args)
 
 
 def window_cache_fill(
@@ -241,23 +299,14 @@ def window_cache_fill(
     if K.dim() != 4 or K.shape != V.shape:
         raise ValueError(f"{what}: K and V must be (B,Hk,N,D) alike")
     _no_grad_inputs(what, K, V, k_cache, v_cache)
-    dev = _lib.require_gpu(K, V, lengths, k_cache, v_cache)
-    B, Hk, N, d = K.shape
+    _lib.require_gpu(K, V, lengths, k_cache, v_cache)
+    B, Hk, _, d = K.shape
     if V.dtype != K.dtype:
         raise TypeError(f"{what}: K is {K.dtype}, V is {V.dtype}")
-    window = _check_caches(what, k_cache, v_cache, B, Hk, d, K.dtype, int(n_sink))
-    at = _lengths(what, lengths, B)
-    k, v = _unit_inner(K.detach()), _unit_inner(V.detach())
-    p = _lib.WindowCacheFillParams(
-        _lib.DFL_BF16 if K.dtype == torch.bfloat16 else _lib.DFL_F32, k.data_ptr(), v.data_ptr(), *k.stride()[:3],
-        *v.stride()[:3], at.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3],
-        *v_cache.stride()[:3], B, Hk, N, d, window, int(n_sink))
-    lib = _lib.load()
-    with _lib.on_device(dev):
-        rc = _lib.timed_launch(what, dev, lambda: lib.dfl_window_cache_fill(
-            ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
-    _lib.check(rc, "dfl_window_cache_fill")
-    torch.autograd.graph.increment_version((k_cache, v_cache))
+    _check_caches(what, k_cache, v_cache, B, Hk, d, K.dtype, int(n_sink))
+    _check_lengths(what, lengths, B)
+    run = _CacheFillFn.apply if _lib.through_autograd(K, V, k_cache, v_cache) else _fill
+    run(K, V, lengths, k_cache, v_cache, int(n_sink))
 
 
 def window_decode_attn(
@@ -285,7 +334,7 @@ def window_decode_attn(
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"{what}: q must be (B,H,D), k and v (B,Hk,D)")
     _no_grad_inputs(what, q, k, v, k_cache, v_cache, rel_table)
-    dev = _lib.require_gpu(q, k, v, k_cache, v_cache, lengths, rel_table)
+    _lib.require_gpu(q, k, v, k_cache, v_cache, lengths, rel_table)
     B, H, d = q.shape
     Hk = k.shape[1]
     if k.shape[0] != B or k.shape[2] != d or Hk < 1 or H % Hk:
@@ -293,28 +342,10 @@ def window_decode_attn(
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"{what}: q is {q.dtype}, k {k.dtype}, v {v.dtype}")
     n_sink = int(n_sink)
-    window = _check_caches(what, k_cache, v_cache, B, Hk, d, q.dtype, n_sink)
-    at = _lengths(what, lengths, B)
+    _check_caches(what, k_cache, v_cache, B, Hk, d, q.dtype, n_sink)
+    _check_lengths(what, lengths, B)
     if (rel_table is None) != (rel_edges is None):
         raise ValueError(f"{what}: give rel_table and rel_edges together")
-    arr = tab = None
-    if rel_table is not None:
-        arr = edge_array(rel_table, rel_edges, H, False)
-        tab = rel_table.detach().to(torch.float32).contiguous()
-    q, k, v = _unit_inner(q.detach()), _unit_inner(k.detach()), _unit_inner(v.detach())
-    o = torch.empty(B, H, d, dtype=q.dtype, device=dev)
-    lib = _lib.load()
-    nbytes = lib.dfl_window_decode_workspace_size(B, H, Hk, d, window, n_sink)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    p = _lib.WindowDecodeParams(
-        _lib.DFL_BF16 if q.dtype == torch.bfloat16 else _lib.DFL_F32, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-        *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], k_cache.data_ptr(), v_cache.data_ptr(),
-        *k_cache.stride()[:3], *v_cache.stride()[:3], at.data_ptr(), _lib.ptr(tab),
-        None if arr is None else ctypes.addressof(arr), 0 if arr is None else len(arr), B, H, Hk, d, window, n_sink,
-        _scale(what, scale, d), o.data_ptr())
-    with _lib.on_device(dev):
-        rc = _lib.timed_launch(what, dev, lambda: lib.dfl_window_decode(
-            ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
-    _lib.check(rc, "dfl_window_decode")
-    torch.autograd.graph.increment_version((k_cache, v_cache))
-    return o
+    arr = None if rel_table is None else edge_array(rel_table, rel_edges, H, False)
+    run = _DecodeFn.apply if _lib.through_autograd(q, k, v, k_cache, v_cache, rel_table) else _decode
+    return run(q, k, v, k_cache, v_cache, lengths, rel_table, arr, n_sink, _scale(what, scale, d))
