@@ -50,9 +50,10 @@ constexpr int MAX_SINK = 128;
 int pad_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 size_t r256(size_t n) { return (n + 255) / 256 * 256; }
 
+bool edges_ok(int n, int both) { return n >= 0 && n <= (both ? (dfl::REL_MAX_EDGES + 1) / 2 - 1 : dfl::REL_MAX_EDGES); }
 int check_rel(const int* edges, int n, int both) {
   if (n < 0 || (n > 0 && !edges)) return fail("rel_edges is NULL");
-  if ((both ? 2 * (n + 1) : n + 1) > dfl::REL_MAX_EDGES + 1)
+  if (!edges_ok(n, both))
     return fail("%d edges give more than %d buckets", n, dfl::REL_MAX_EDGES + 1);
   for (int i = 0; i < n; ++i) {
     if (edges[i] < 1 || edges[i] > dfl::REL_MAX_DIST) return fail("edge %d outside [1, %d]", edges[i], dfl::REL_MAX_DIST);
@@ -68,11 +69,19 @@ dfl::RelSpec rel_spec(const int* edges, int n, int both) {
   for (int i = 0; i < n; ++i) r.edge[i] = edges[i];
   return r;
 }
+// A product of two ints fits 64 bits: tested first, so that none of the sizes formed from it can wrap around.
+constexpr long long MAX_BH = 1ll << 22;  // four waves for each of 128 first tokens of each are counted in 32 bits
+bool heads_ok(int B, int H, int Hk, int d) {
+  return B > 0 && H > 0 && Hk > 0 && H % Hk == 0 && d > 0 && d <= 128 && (long long)B * H < MAX_BH;
+}
+bool window_ok(int window, int n_sink) { return window >= 1 && n_sink >= 0 && n_sink <= MAX_SINK; }
+
 int check_heads(int dtype, int B, int H, int Hk, int d) {
   if (dtype != DFL_F32 && dtype != DFL_BF16) return fail("dtype must be DFL_F32 or DFL_BF16");
   if (B <= 0 || H <= 0 || Hk <= 0) return fail("B, H, Hk must be positive");
   if (H % Hk != 0) return fail("H=%d is no multiple of Hk=%d", H, Hk);
   if (d <= 0 || d > 128) return fail("head dim d=%d outside [1, 128]", d);
+  if (!heads_ok(B, H, Hk, d)) return fail("B * H = %lld is too large", (long long)B * H);
   return 0;
 }
 // The running reference is a maximum of scaled scores, taken before the scale.
@@ -134,7 +143,6 @@ int check_attn(const dfl_window_attn_params* p, bool bwd) {
     return fail("M=%d, N=%d: need 0 < M <= N <= %lld", p->M, p->N, MAX_N);
   if ((((long long)p->N + 63) / 64 + 1) * p->B * p->H * 8 >= (1ll << 31)) return fail("too many rows");
   if (int rc = check_scale(p->scale)) return rc;
-  if ((long long)p->B * p->H * 4 * MAX_SINK >= (1ll << 31)) return fail("B * H = %lld is too large", (long long)p->B * p->H);
   if (!p->q || !p->k || !p->v || !p->o) return fail("required pointer is NULL");
   if (!p->rel_table != (p->n_edges == 0)) return fail("rel_table and rel_edges must be given together");
   if (int rc = check_rel(p->rel_edges, p->n_edges, !p->causal)) return rc;
@@ -204,7 +212,7 @@ extern "C" {
 
 size_t dfl_window_attn_workspace_size(int B, int H, int Hk, int M, int N, int d, int window, int n_sink, int causal,
                                       int n_edges) {
-  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || M <= 0 || N < M || d <= 0 || d > 128 || window < 1 || n_sink < 0 || n_edges < 0)
+  if (!heads_ok(B, H, Hk, d) || M <= 0 || N < M || N > MAX_N || !window_ok(window, n_sink) || !edges_ok(n_edges, !causal))
     return 0;
   return WindowWs(B, H, Hk, M, N, d, window, n_sink, causal, n_edges).total;
 }
@@ -264,7 +272,7 @@ int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream) {
 }
 
 size_t dfl_window_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink) {
-  if (B <= 0 || H <= 0 || Hk <= 0 || d <= 0 || d > 128 || window < 1 || n_sink < 0) return 0;
+  if (!heads_ok(B, H, Hk, d) || !window_ok(window, n_sink) || window > MAX_N) return 0;
   const Splits s(B, H, Hk, window + n_sink);
   return s.n > 1 ? r256((size_t)B * H * s.n * (pad_dim(d) + 2) * 4) : 0;
 }
@@ -307,7 +315,8 @@ int dfl_window_decode(const dfl_window_decode_params* p, void* workspace, size_t
 }
 
 size_t dfl_rel_bias_workspace_size(int B, int H, int M, int N, int n_edges, int rel_both) {
-  if (B <= 0 || H <= 0 || M <= 0 || N <= 0 || n_edges < 0) return 0;
+  if (B <= 0 || H <= 0 || M <= 0 || N <= 0 || M > MAX_N || N > MAX_N || (long long)B * H > 65535 || !edges_ok(n_edges, rel_both))
+    return 0;
   return r256((size_t)B * H * dfl::rel_bias_parts(B, H, M, N) * (rel_both ? 2 : 1) * (n_edges + 1) * 4);
 }
 

@@ -1,8 +1,10 @@
 """CPU checks of the sequence operators' wrappers with the launches replaced by copies: what a trace
-records and what forward-mode differentiation sees."""
+records and what forward-mode differentiation sees.  And of the C entries' sizes."""
 
 import contextlib
 import ctypes
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -112,3 +114,48 @@ def test_forward_mode_is_refused(copies):
                                   rel_edges=(1, 2))
         o, dec = step(*x)
         assert torch.equal(o, x[0]) and torch.equal(dec, x[0][:, :, 0])
+
+
+SIZES = """
+import ctypes, sys
+lib = ctypes.CDLL(sys.argv[1])
+I = ctypes.c_int
+for name, n in (("dfl_window_decode_workspace_size", 6), ("dfl_window_attn_workspace_size", 10), ("dfl_rel_bias_workspace_size", 6)):
+    f = getattr(lib, name)
+    f.restype, f.argtypes = ctypes.c_size_t, [I] * n
+for call in sys.argv[2:]:
+    name, *args = call.split(",")
+    print(getattr(lib, "dfl_" + name)(*map(int, args)))
+"""
+
+
+def test_workspace_sizes_of_refused_arguments():
+    """A size asked for what the entry itself refuses is 0, whatever the numbers; in a process of its own, as a division
+    by zero would end it."""
+    top = 2**31 - 1
+    refused = [("window_decode", 1, 2, 4, 64, 128, 0), ("window_decode", 1, 3, 2, 64, 4096, 0),
+               ("window_decode", 1, 2, 2, 64, top, 1), ("window_decode", 1, 2, 2, 64, 4096, 129),
+               ("window_decode", 2**30, 2**30, 2**30, 64, 4096, 0), ("window_decode", 1 << 22, 1, 1, 64, 4096, 4),
+               ("window_attn", 1, 2, 4, 64, 64, 64, 16, 0, 1, 0), ("window_attn", 1, 2, 2, 1, top, 64, 16, 0, 1, 0),
+               ("window_attn", 2**30, 2**30, 2**30, 8, 8, 64, 16, 0, 1, 0), ("window_attn", 1, 2, 2, 8, 8, 64, 16, 129, 1, 0),
+               ("window_attn", 1, 2, 2, 8, 8, 64, 16, 0, 1, top), ("window_attn", 1, 2, 2, 8, 8, 64, 16, 0, 0, 48),
+               ("rel_bias", 1, 1, 8, 8, top, 1), ("rel_bias", 65536, 1, 8, 8, 3, 1), ("rel_bias", 1, 1, 8, 8, 96, 0)]
+    taken = [("window_decode", 1, 2, 2, 64, 4096, 128), ("window_attn", 1, 2, 2, 8, 8, 64, top, 128, 0, 47),
+             ("rel_bias", 1, 1, 8, 8, 95, 0)]
+    calls = [f"{name}_workspace_size," + ",".join(map(str, a)) for name, *a in refused + taken]
+    run = subprocess.run([sys.executable, "-c", SIZES, _lib.LIB_PATH, *calls], capture_output=True, text=True)
+    assert run.returncode == 0, (run.returncode, run.stderr[-500:])
+    got = list(map(int, run.stdout.split()))
+    assert got[:len(refused)] == [0] * len(refused)
+    assert all(n > 0 for n in got[len(refused):])
+
+
+def test_entries_refuse_head_counts_that_wrap_around():
+    """B * H of 2^60: the products formed from it would be 0 in 64 bits."""
+    lib, fake, n = _lib.load(), 4096, 1 << 30
+    p = _lib.WindowAttnParams(dtype=_lib.DFL_BF16, q=fake, k=fake, v=fake, B=n, H=n, Hk=n, M=8, N=8, d=64, window=4, causal=1,
+                              scale=1.0, o=fake)
+    assert lib.dfl_window_attn_fwd(ctypes.byref(p), None) < 0 and "too large" in lib.dfl_last_error().decode()
+    p = _lib.WindowDecodeParams(dtype=_lib.DFL_BF16, q=fake, k=fake, v=fake, k_cache=fake, v_cache=fake, lengths=fake, B=n, H=n,
+                                Hk=n, d=64, window=8, scale=1.0, o=fake)
+    assert lib.dfl_window_decode(ctypes.byref(p), None, 0, None) < 0 and "too large" in lib.dfl_last_error().decode()
