@@ -22,7 +22,7 @@ template <typename T, bool FAST> __global__ void __launch_bounds__(256) cache_fi
   constexpr int VEC = 16 / (int)sizeof(T);
   const int nch = (a.d + VEC - 1) / VEC, S = a.n_sink + a.window;
   const int bh = blockIdx.y, b = bh / a.Hk, hk = bh % a.Hk;
-  const int last = min(a.lengths[b], a.N) - 1;
+  const int last = max(min(a.lengths[b], a.N), 0) - 1;  // (a length of -2^31 has no predecessor)
   const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (slot, chunk)
   const int s = (int)(e / nch), c = (int)(e % nch);
   if (s >= S) return;

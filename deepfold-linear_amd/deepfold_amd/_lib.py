@@ -384,6 +384,15 @@ def require_gpu(*tensors) -> torch.device:
     return dev
 
 
+def to_int32(t: torch.Tensor) -> torch.Tensor:
+    """Integers in 32 bits; what lies outside becomes the nearest end of their range (a cast would wrap around)."""
+    if t.dtype == torch.int32:
+        return t
+    if t.dtype in (torch.int64, torch.uint32, torch.uint64):
+        t = t.to(torch.int64).clamp(-2**31, 2**31 - 1)
+    return t.to(torch.int32)
+
+
 def through_autograd(*tensors) -> bool:
     """Whether a call must go through its ``autograd.Function`` rather than straight to the launch: an input asks for a
     gradient, a trace is being recorded (it holds a Function's call, but not what a launch writes), or forward-mode

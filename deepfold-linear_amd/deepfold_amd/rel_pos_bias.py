@@ -84,7 +84,7 @@ def _positions(t, name, dims):
         raise TypeError(f"rel_pos_bias: {name} must hold integers, got {t.dtype}")
     if t.dim() != 2 or t.shape[1] != dims:
         raise ValueError(f"rel_pos_bias: {name} must be (B, {dims}) or ({dims},)")
-    return t.detach().to(torch.int32).contiguous()
+    return _lib.to_int32(t.detach()).contiguous()
 
 
 class _RelPosBias(torch.autograd.Function):
@@ -147,7 +147,8 @@ def rel_pos_bias(
 
     table (H, buckets); query i stands at position i + n_key - n_query and key j at j, or, with
     ``q_pos`` (B, n_query) / (n_query,) and ``k_pos`` (B, n_key) / (n_key,) integers, where those say (one of them
-    alone stands for both if n_query == n_key).  Returns (H, n_query, n_key), or (B, H, n_query, n_key) with
+    alone stands for both if n_query == n_key).  Positions are held in 32 bits: one beyond them stands at their end, so
+    shift a sample's positions into [-2^31, 2^31) first (only differences count).  Returns (H, n_query, n_key), or (B, H, n_query, n_key) with
     batched positions, contiguous, in ``dtype`` (bf16 or fp32; default: the table's if it is one of them)."""
     M = int(n_query)
     N = M if n_key is None else int(n_key)

@@ -216,7 +216,7 @@ def _check_lengths(what, lengths, B):
 
 
 def _lengths(lengths):
-    return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else lengths.to(torch.int32).contiguous()
+    return _lib.to_int32(lengths).contiguous()
 
 
 def _no_grad_inputs(what, *tensors):
@@ -291,8 +291,8 @@ def window_cache_fill(
 ) -> None:
     """Copies a prompt's keys and values into the rolling caches, in place.
 
-    K, V (B,Hk,N,D), any strides; lengths (B,) int: rows 0 .. lengths[b] - 1 are the prompt (above N counts as N,
-    below 1 leaves the sample's caches alone).  k_cache, v_cache (B,Hk,n_sink + window,D): position p < n_sink goes
+    K, V (B,Hk,N,D), any strides, in memory of their own; lengths (B,) int32 or int64: rows 0 .. lengths[b] - 1 are the
+    prompt (above N counts as N, below 1 leaves the sample's caches alone).  k_cache, v_cache (B,Hk,n_sink + window,D): position p < n_sink goes
     to slot p, any other to slot n_sink + (p - n_sink) % window, the last of those that share one; slots that no
     position of the prompt belongs to keep what they hold."""
     what = "window_cache_fill"
@@ -326,8 +326,8 @@ def window_decode_attn(
     attention for the query at position lengths[b].
 
     q (B,H,D); k, v (B,Hk,D) the token's own key and value, which enter k_cache, v_cache (B,Hk,n_sink + window,D) in
-    place at position lengths[b], the number of tokens that the sample's cache has taken so far; lengths (B,) int, on
-    the device, not changed by the call; a sample with lengths[b] < 0 has no token: its output is zero and its caches
+    place at position lengths[b], the number of tokens that the sample's cache has taken so far; lengths (B,) int32 or
+    int64, below 2^31 (above counts as 2^31 - 1), on the device, not changed by the call; a sample with lengths[b] < 0 has no token: its output is zero and its caches
     stay as they are.  All of q, k, v and the caches in bf16 or all in fp32.  The table has one direction
     (len(rel_edges) + 1 buckets).  No gradient.  Returns o (B,H,D)."""
     what = "window_decode_attn"

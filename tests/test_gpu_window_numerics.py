@@ -1,0 +1,32 @@
+"""The sequence operators on the GPU where their numbers are hard: lengths at the ends of their type, scores that grow
+along the sequence, sharp and diffuse rows, long sums.  Bounds as in oracle/window.py."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import window as ref
+from test_gpu_window import BF, DEV, EDGES, F32, holds, leaf, rnd
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_lengths_at_the_ends_of_their_type(dtype):
+    """Beyond N counts as N, below 1 leaves the caches alone, also where 32 bits end."""
+    from deepfold_amd import window_cache_fill
+
+    Hk, N, d, window, n_sink = 2, 30, 24, 9, 3
+    lengths = torch.tensor([2**32 + 5, 2**31, 2**31 - 1, -2**31, -2**31 - 1, -2**40, 2**62, 4])
+    B = len(lengths)
+    k, v = rnd(B, Hk, N, d, seed=1, dtype=dtype), rnd(B, Hk, N, d, seed=2, dtype=dtype)
+    kc, vc = rnd(B, Hk, n_sink + window, d, seed=3, dtype=dtype), rnd(B, Hk, n_sink + window, d, seed=4, dtype=dtype)
+    want = ref.fill(k, v, lengths, kc, vc, n_sink)
+    got = kc.to(DEV), vc.to(DEV)
+    window_cache_fill(k.to(DEV), v.to(DEV), lengths.to(DEV), *got, n_sink=n_sink)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+    short = lengths.clamp(-2**31, 2**31 - 1).to(torch.int32).to(DEV)
+    again = kc.to(DEV), vc.to(DEV)
+    window_cache_fill(k.to(DEV), v.to(DEV), short, *again, n_sink=n_sink)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])

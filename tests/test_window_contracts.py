@@ -14,6 +14,26 @@ import deepfold_amd as df
 from deepfold_amd import _lib
 
 
+END = 2**31
+
+
+def test_integers_beyond_32_bits_stay_at_the_end():
+    """Lengths and positions are held in 32 bits: what does not fit is the largest or lowest, not another number."""
+    from deepfold_amd import rel_pos_bias, window_attn
+
+    x = torch.tensor([0, -1, 5, END - 1, END, END + 5, 2 * END + 5, -END, -END - 1, 2**62, -2**62])
+    want = x.clamp(-END, END - 1).to(torch.int32)
+    assert torch.equal(window_attn._lengths(x), want)
+    assert torch.equal(window_attn._lengths(x[::2]), want[::2]) and window_attn._lengths(x[::2]).is_contiguous()
+    short = x[:4].to(torch.int32)
+    assert window_attn._lengths(short).data_ptr() == short.data_ptr()
+    module = sys.modules["deepfold_amd.rel_pos_bias"]
+    assert torch.equal(module._positions(x[None], "q_pos", len(x))[0], want)
+    assert rel_pos_bias is module.rel_pos_bias
+    for dtype in (torch.int16, torch.uint8, torch.int8):
+        assert module._positions(torch.tensor([[0, 7, 100]], dtype=dtype), "q_pos", 3).tolist() == [[0, 7, 100]]
+
+
 class Copies:
     """In place of the library: each launch copies its first input to what it writes (o = q, cache = k / v)."""
 
