@@ -183,6 +183,17 @@ def flash_window_attn(
     return O.squeeze(0) if unbatched else O
 
 
+def _meet(shape, stride, apart):
+    """Whether two tensors of one shape and stride, ``apart`` elements between their first, have an element in common.
+    Each stride reaches over the extents below it (``_check_caches``), so the difference of two elements is, widest stride
+    first, the quotient or the next in that dimension."""
+    rest = {apart}
+    for s, n in sorted(zip(stride, shape), reverse=True):
+        if n > 1:
+            rest = {r - c * s for r in rest for c in (r // s, r // s + 1) if -n < c < n}
+    return 0 in rest
+
+
 def _check_caches(what, k_cache, v_cache, B, Hk, d, dtype, n_sink):
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"{what}: k_cache and v_cache must be (B,Hk,n_sink + window,D) alike")
@@ -191,20 +202,25 @@ def _check_caches(what, k_cache, v_cache, B, Hk, d, dtype, n_sink):
     if k_cache.dtype != dtype or v_cache.dtype != dtype or dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"{what}: caches and inputs must all be bf16 or all fp32, got {k_cache.dtype}, "
                         f"{v_cache.dtype} and {dtype}")
-    if k_cache.data_ptr() == v_cache.data_ptr():
-        raise ValueError(f"{what}: k_cache and v_cache are the same memory")
+    extent = []  # elements from a cache's first to its last
     for c in (k_cache, v_cache):
         st = c.stride()
         if st[3] != 1 and d > 1:
             raise ValueError(f"{what}: the caches' last dimension must be contiguous")
         # every slot a memory of its own: strides that can hold the extents below them
         if c.is_contiguous():
+            extent.append(c.numel())
             continue
         at = d
         for s, n in sorted((s, n) for s, n in zip(st[:3], c.shape[:3]) if n > 1):
             if s < at:
                 raise ValueError(f"{what}: the cache's slots overlap (strides {st})")
             at = s * (n - 1) + at
+        extent.append(at)
+    apart, odd = divmod(v_cache.data_ptr() - k_cache.data_ptr(), k_cache.element_size())
+    if -extent[1] < apart < extent[0] and (
+            odd or k_cache.stride() != v_cache.stride() or _meet(k_cache.shape, k_cache.stride(), apart)):
+        raise ValueError(f"{what}: k_cache and v_cache share memory, or interleave with different strides")
     window = k_cache.shape[2] - n_sink
     _check_window(what, window, n_sink)
     return window

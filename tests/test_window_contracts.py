@@ -34,6 +34,40 @@ def test_integers_beyond_32_bits_stay_at_the_end():
         assert module._positions(torch.tensor([[0, 7, 100]], dtype=dtype), "q_pos", 3).tolist() == [[0, 7, 100]]
 
 
+def test_caches_that_share_memory_are_refused():
+    """k_cache and v_cache must not have an element in common; interleaved ones (a view of keys and values) are taken.
+    The answer is held against the sets of addresses."""
+    import random
+
+    from deepfold_amd import window_attn
+
+    rng, seen = random.Random(3), [0, 0]
+    for _ in range(600):
+        n, hk, slots, d = rng.choice([1, 2, 3]), rng.choice([1, 2]), rng.choice([1, 2, 5]), rng.choice([1, 2, 4])
+        order, stride, at = rng.sample(range(3), 3), [0, 0, 0], d
+        for dim in order:  # nested strides in any order, with gaps now and then
+            stride[dim] = at + rng.choice([0, 0, d, 3])
+            at = stride[dim] * ((n, hk, slots)[dim] - 1) + at
+        buf = torch.zeros(4 * at + 64)
+        shape, first = (n, hk, slots, d), at + 8
+        a, b = (buf.as_strided(shape, (*stride, 1), first), buf.as_strided(shape, (*stride, 1), first + rng.randint(-at, at)))
+        where = [set((x.storage_offset() + sum(i * s for i, s in zip(ix, x.stride()))) for ix in
+                     torch.cartesian_prod(*map(torch.arange, shape)).tolist()) for x in (a, b)]
+        shared = bool(where[0] & where[1])
+        seen[shared] += 1
+        if shared:
+            with pytest.raises(ValueError, match="share memory"):
+                window_attn._check_caches("t", a, b, n, hk, d, torch.float32, 0)
+        else:
+            assert window_attn._check_caches("t", a, b, n, hk, d, torch.float32, 0) == slots
+    assert min(seen) > 50
+    kc = torch.zeros(2, 2, 6, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        window_attn._check_caches("t", kc[:, :, :5], kc[:, :, 1:], 2, 2, 8, torch.float32, 1)
+    # the same storage, one behind the other
+    assert window_attn._check_caches("t", kc[:1], kc[1:], 1, 2, 8, torch.float32, 1) == 5
+
+
 class Copies:
     """In place of the library: each launch copies its first input to what it writes (o = q, cache = k / v)."""
 
