@@ -4,20 +4,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "window_geometry.h"
+
 namespace dfl {
-
-constexpr int REL_MAX_EDGES = 95;   // at most 96 buckets a table
-constexpr int REL_MAX_DIST = 2048;  // largest edge
-
-// Bucket of a relative position rel = key - query: mag = |rel| with `both`, else
-// max(-rel, 0); bucket = #{k : edge[k] <= mag}, plus n + 1 with `both` and rel > 0.
-struct RelSpec {
-  int n;     // edges, ascending
-  int both;  // both directions: 2 (n + 1) buckets, else n + 1
-  int edge[REL_MAX_EDGES];
-  __host__ __device__ int buckets() const { return both ? 2 * (n + 1) : n + 1; }
-  __host__ __device__ int dist() const { return n ? edge[n - 1] : 0; }  // from here on one bucket a direction
-};
 
 struct WinArgs {
   const void* q;  // (B,H,M,d), element strides qsb/qsh/qsn, unit inner stride

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
 #pragma unroll
       for (int sub = 0; sub < E::NSUB; ++sub) {
         const int js = j0 + 32 * sub;
-        if (REL && far < 0) {
+        if (REL && far < 0 && !vis.none(t0, js)) {
           const int one = rel_far(a.rel, t0, js);
           if (one >= 0) {
             yc[sub] = lut[one];

@@ -358,7 +358,7 @@ __device__ __forceinline__ void bwd_kv(const WinArgs& a, int x, int n_buf, unsig
   const int ns = min(a.n_sink, a.N);
   f32x16 acc[E::NT] = {};  // half 0: dv, half 1: dk
   // whether any of the wave's keys and the 32 queries from t0 on meet here
-  auto meet = [&](int t0) { return SINK ? (j0 < ns) & !vis.all_near(t0, j0) : !vis.none_near(t0, j0); };
+  auto meet = [&](int t0) { return SINK ? (j0 < ns) & vis.some_first(t0, j0) : !vis.none_near(t0, j0); };
   for (int it = it0; it < it1; ++it) {
     const int buf = (it - it0) & (n_buf - 1);
     const bool new_head = REL && (it == it0 || it % nt == 0);

@@ -180,44 +180,9 @@ __device__ __forceinline__ int xcd_order(int w, int n) {
   return x * per + min(x, rem) + (w >> 3);
 }
 
-// Visibility of key j to the query at position t, without the mask.
-struct WinVis {
-  int off, n_sink, causal;
-  unsigned range;
-  __device__ __forceinline__ explicit WinVis(const WinArgs& a) {
-    const int w = min(a.window, a.N);
-    off = a.causal ? 0 : w - 1;
-    range = (unsigned)(a.causal ? w : 2 * w - 1);
-    n_sink = a.n_sink;
-    causal = a.causal;
-  }
-  __device__ __forceinline__ bool near(int t, int j) const { return (unsigned)(t - j + off) < range; }
-  __device__ __forceinline__ bool first(int t, int j) const { return (j < n_sink) & ((causal == 0) | (j <= t)); }
-  // (combined with & and |: a chain of branches around single elements of an accumulator loses some of the writes
-  // to them in this compiler)
-  __device__ __forceinline__ bool sees(int t, int j) const { return near(t, j) | first(t, j); }
-  // all / none of the pairs of 32 queries from t0 and n keys from j0 on
-  __device__ __forceinline__ bool all_near(int t0, int j0, int n = 32) const {
-    return near(t0, j0 + n - 1) & near(t0 + 31, j0);
-  }
-  __device__ __forceinline__ bool none_near(int t0, int j0, int n = 32) const {
-    return (t0 + 31 - j0 + off < 0) | (t0 - (j0 + n - 1) + off >= (int)range);
-  }
-  __device__ __forceinline__ bool none(int t0, int j0, int n = 32) const {
-    return none_near(t0, j0, n) & !((j0 < n_sink) & ((causal == 0) | (j0 <= t0 + 31)));
-  }
-};
-
 // ---------------------------------------------------------------------------
-// Bias lookup in LDS: lut[x] for the distance x = t - j + base(), in units of log2.  REL_PAD
-// entries more than the table's range on both sides hold its end values, so that a 32 x 32
-// tile any pair of which is inside the range needs no clamp.
-constexpr int REL_PAD = 64;
+// Bias lookup in LDS: lut[x] for the distance x = t - j + base, in units of log2 (window_geometry.h).
 constexpr int REL_EDGES = 96;  // ints of the edges in LDS, behind a lookup table
-__host__ __device__ inline int rel_lut_size(const RelSpec& r) {
-  return ((r.both ? 2 * r.dist() + 1 : r.dist() + 1) + 2 * REL_PAD + 3) & ~3;
-}
-__device__ __forceinline__ int rel_lut_base(const RelSpec& r) { return (r.both ? r.dist() : 0) + REL_PAD; }
 // bucket of rel = j - t
 __device__ __forceinline__ int rel_bucket(const RelSpec& r, int rel) {
   const int mag = r.both ? abs(rel) : max(-rel, 0);
@@ -244,13 +209,6 @@ __device__ __forceinline__ void build_rel_lut(const WinArgs& a, int h, const int
   for (int x = threadIdx.x; x < n; x += blockDim.x) {
     lut[x] = row[rel_bucket_lds(edge, a.rel.n, a.rel.both, base - x)] * LOG2E;
   }
-}
-// Where every distance t - j of 32 queries and n keys lies beyond the table's range: the index of its one value, else -1.
-__device__ __forceinline__ int rel_far(const RelSpec& r, int t0, int j0, int n = 32) {
-  const int dist = r.dist();
-  if (t0 - (j0 + n - 1) >= dist) return rel_lut_base(r) + dist;
-  if (r.both && j0 - (t0 + 31) > dist) return rel_lut_base(r) - dist - 1;
-  return -1;
 }
 
 }  // namespace dfl

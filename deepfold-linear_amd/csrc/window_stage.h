@@ -1,24 +1,8 @@
-// Which key tiles a workgroup of the window attention visits, and their staging into LDS.
+// Staging of the window attention's tiles into LDS.
 #pragma once
 #include "window_engine.h"
 
 namespace dfl {
-
-// Key tiles of queries t0 .. t1: the first tokens' tiles in front of the band, then the band (and, in both
-// directions, the first tokens' tiles behind it).
-struct KeyTiles {
-  int pre, b0, total;
-  __device__ __forceinline__ KeyTiles(const WinArgs& a, int t0, int t1, int BK) {
-    const int w = min(a.window, a.N);
-    const int lo = max(0, t0 - w + 1), hi = a.causal ? t1 : min(a.N - 1, t1 + w - 1);
-    const int nst = (min(a.n_sink, a.N) + BK - 1) / BK;
-    b0 = lo / BK;
-    const int b1 = hi / BK + 1;
-    pre = min(nst, b0);
-    total = pre + (a.causal ? b1 : max(b1, nst)) - b0;
-  }
-  __device__ __forceinline__ int tile(int it) const { return it < pre ? it : b0 + it - pre; }
-};
 
 // One 16-byte load a lane from `from` to `to` + 16 lane in LDS (`to` uniform, in bytes), not waited for: lds_loads_done().
 // Written out because the compiler, where it knows of such a load, waits for all of them before the next transposing LDS
