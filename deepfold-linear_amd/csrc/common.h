@@ -317,6 +317,14 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Orders the LDS accesses of one wave across its lanes: what any lane wrote before is there for every lane after, and
+// what any lane read before is read.  The hardware keeps a wave's LDS accesses in order; this holds the compiler to it.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // True when this workgroup runs on the XCD that the round-robin dispatch order
 // assigns to it (workgroup id mod 8), read from the hardware XCC id register.
 __device__ __forceinline__ bool xcc_placed() {

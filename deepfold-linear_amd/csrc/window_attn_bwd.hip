@@ -200,8 +200,10 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               float* to = sw + (4 * h32) * 64 + (lane & 31) - 4 * h32 + 15;
+              wave_lds_fence();  // the last half's columns are read, its sums written
 #pragma unroll
               for (int r = 0; r < 8; ++r) to[acc_row(r, 0) * 63] = p[8 * half + r];
+              wave_lds_fence();  // a column is other lanes' entries
               float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int m = 0; m < 16; ++m) s[m & 3] += sw[m * 64 + lane];

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import window as ref
-from test_gpu_window import BF, DEV, EDGES, F32, holds, leaf, rnd
+from test_gpu_window import BF, DEV, EDGES, F32, attention_case, holds, leaf, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +30,16 @@ def test_lengths_at_the_ends_of_their_type(dtype):
     again = kc.to(DEV), vc.to(DEV)
     window_cache_fill(k.to(DEV), v.to(DEV), short, *again, n_sink=n_sink)
     assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+def test_table_gradient_over_many_tiles(causal, dtype):
+    """A wave adds up the diagonals of many tiles in a row, each through the same columns of LDS: the table's gradient at
+    every distance (a bucket for each of the first ones), and the same bits from call to call."""
+    edges = (*range(1, 90), 400) if causal else (*range(1, 46), 700)
+    case = dict(rel=True, edges=edges, seed=21)
+    first = attention_case(1, 2, 2, 640, 640, 64, dtype, 640, 0, causal, **case)[1]
+    for _ in range(3):
+        again = attention_case(1, 2, 2, 640, 640, 64, dtype, 640, 0, causal, **case)[1]
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
