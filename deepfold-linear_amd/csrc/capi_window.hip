@@ -189,6 +189,7 @@ int check_bias(const dfl_rel_bias_params* p) {
   if (p->B <= 0 || p->H <= 0 || p->M <= 0 || p->N <= 0 || p->M > MAX_N || p->N > MAX_N)
     return fail("B, H, M, N must be positive and M, N at most %lld", MAX_N);
   if ((long long)p->B * p->H > 65535) return fail("B * H = %lld > 65535", (long long)p->B * p->H);
+  if ((long long)p->B * dfl::rel_bias_parts(p->B, p->H, p->M, p->N) >= (1ll << 31)) return fail("M * N is too large");
   if (!p->q_pos != !p->k_pos) return fail("q_pos and k_pos must be given together");
   if (p->n_edges < 1) return fail("rel_edges is empty");
   return check_rel(p->rel_edges, p->n_edges, p->rel_both);

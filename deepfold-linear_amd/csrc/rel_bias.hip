@@ -126,8 +126,11 @@ __global__ void __launch_bounds__(256) rel_bias_fwd_kernel(RelBiasArgs a, int lu
 // A workgroup sums its part of one plane by bucket: every thread has a column of its own in LDS, so no address has
 // two writers and the order of each sum is fixed.  Neighbours of one bucket, most of them away from the diagonal, are
 // added up before the column is touched; BWD_U vectors of a thread are loaded at once (one at a time, loads in flight
-// bound the pass to a quarter of the memory rate).
+// bound the pass to a quarter of the memory rate).  A thread adds up at most BWD_CHAIN elements in fp32, whatever the
+// plane's size (an error of at most BWD_CHAIN half steps of a column's sum of magnitudes); the parts are joined in 64
+// bits.
 constexpr int BWD_U = 4;
+constexpr int BWD_CHAIN = 1024;
 template <typename T, bool POS>
 __global__ void __launch_bounds__(256) rel_bias_bwd_kernel(RelBiasArgs a, int lut_bytes) {
   constexpr int V = Vec<T>::N;
@@ -192,11 +195,11 @@ __global__ void __launch_bounds__(256) rel_bias_sum_kernel(RelBiasArgs a) {
   const int nb = a.rel.buckets(), w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w >= a.H * nb) return;
   const int h = w / nb, n = w % nb;
-  float s = 0.f;
+  double s = 0.;
   for (int e = lane; e < a.B * a.n_part; e += 64)
     s += a.part[(((size_t)(e / a.n_part) * a.H + h) * a.n_part + e % a.n_part) * nb + n];
-  s = wave_sum(s);
-  if (lane == 0) a.dtable[w] = s;
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, WAVE);
+  if (lane == 0) a.dtable[w] = (float)s;
 }
 
 hipError_t launch_rel_bias_fwd(const RelBiasArgs& a, bool bf16_out, hipStream_t s) {
@@ -211,10 +214,12 @@ hipError_t launch_rel_bias_fwd(const RelBiasArgs& a, bool bf16_out, hipStream_t 
   return hipGetLastError();
 }
 
-// Parts of a plane: about 4 workgroups a CU in all, at least one round of vectors each.
+// Parts of a plane: about 4 workgroups a CU in all, at least one round of vectors each, at most BWD_CHAIN elements a
+// thread (the last vector of a thread's share may be one more; 2^20 parts are planes beyond any memory).
 int rel_bias_parts(int B, int H, int M, int N) {
   const size_t n = (size_t)M * N, want = std::max<size_t>(1, 1024 / ((size_t)B * H));
-  return (int)std::max<size_t>(1, std::min<size_t>(want, (n + 4095) / 4096));
+  const size_t chains = n > 256 * BWD_CHAIN ? n / (256 * (BWD_CHAIN - 8)) + 1 : 1;
+  return (int)std::min<size_t>(1 << 20, std::max(chains, std::min<size_t>(want, (n + 4095) / 4096)));
 }
 
 hipError_t launch_rel_bias_bwd(const RelBiasArgs& a, bool bf16_in, hipStream_t s) {

@@ -43,3 +43,19 @@ def test_table_gradient_over_many_tiles(causal, dtype):
     for _ in range(3):
         again = attention_case(1, 2, 2, 640, 640, 64, dtype, 640, 0, causal, **case)[1]
         assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_bias_gradient_of_many_heads_and_a_large_plane():
+    """Where the heads alone fill the card a plane is still cut up: at most 1024 additions a thread in fp32, 256 columns
+    added up in a tree of 10, the parts in 64 bits.  Equal addends round the same way each time."""
+    from deepfold_amd import rel_pos_bias
+
+    H, M, N = 1024, 512, 2048
+    table = torch.zeros(H, 2, device=DEV, requires_grad=True)
+    out = rel_pos_bias(table, (700,), M, N, bidirectional=False)
+    value = (torch.arange(H, dtype=F32) + 1.3) / 3
+    g = torch.autograd.grad(out, table, value.to(DEV)[:, None, None].expand(H, M, N))[0]
+    rel = torch.arange(N)[None, :] - torch.arange(M)[:, None] - (N - M)
+    far = int((rel <= -700).sum())
+    want = value.double()[:, None] * torch.tensor([M * N - far, far]).double()
+    holds("dtable", g, want, (1024 + 10 + 1) * ref.U32 * want)

@@ -213,3 +213,15 @@ def test_entries_refuse_head_counts_that_wrap_around():
     p = _lib.WindowDecodeParams(dtype=_lib.DFL_BF16, q=fake, k=fake, v=fake, k_cache=fake, v_cache=fake, lengths=fake, B=n, H=n,
                                 Hk=n, d=64, window=8, scale=1.0, o=fake)
     assert lib.dfl_window_decode(ctypes.byref(p), None, 0, None) < 0 and "too large" in lib.dfl_last_error().decode()
+
+
+def test_bias_gradient_chains_are_bounded():
+    """The workspace holds one sum a bucket for each part of a plane: a thread of a part adds up at most 1024 elements in
+    fp32, however large the plane and however many heads there are."""
+    lib = _lib.load()
+    for heads in (1, 3, 64, 1000, 1024, 4096, 65535):
+        for m, n in ((1, 7), (97, 97), (512, 512), (777, 777), (1, 2**20), (4096, 4096), (16384, 16384), (2**17 + 1, 2**13 + 3)):
+            size = lib.dfl_rel_bias_workspace_size(1, heads, m, n, 47, 1)
+            parts = size // (heads * 96 * 4)
+            assert m * n / (256 * parts) <= 1024, (heads, m, n, parts)
+            assert parts <= max(1, 1024 // heads, m * n // 2**18 + m * n // 2**23 + 2), (heads, m, n, parts)
