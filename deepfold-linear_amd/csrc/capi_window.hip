@@ -165,6 +165,7 @@ dfl::WinArgs attn_args(const dfl_window_attn_params* p) {
   a.window = p->window; a.n_sink = p->n_sink; a.causal = p->causal != 0;
   a.scale = p->scale;
   a.o = p->o;
+  a.o_rest = p->o_rest;
   a.lse = p->lse;
   return a;
 }

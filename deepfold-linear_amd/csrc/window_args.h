@@ -22,6 +22,7 @@ struct WinArgs {
   int window, n_sink, causal;
   float scale;
   void* o;     // (B,H,M,d) contiguous
+  void* o_rest;  // (B,H,M,d) or null; bf16: sum p~ v / sum p~ - o with the rounded weights p~, where !win_few_keys
   float* lse;  // (B,H,M) base-2 log of the row sums; LSE_EMPTY on rows that see nothing
   // backward
   const void* go;  // (B,H,M,d) contiguous

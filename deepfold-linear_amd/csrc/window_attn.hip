@@ -63,7 +63,13 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
   E::template load_frag<FAST>(
       qf, row_ok ? reinterpret_cast<const T*>(a.q) + b * a.qsb + h * a.qsh + (size_t)i * a.qsn : nullptr, a.d, lane);
   const float sc = a.scale * LOG2E;
-  float m = NEG_BIG, l = 0.f;
+  // What the backward takes D = do.o from: the weights of the sums are rounded to bf16, and o once more.  Divided by
+  // the sum of the rounded weights, and kept in two parts, o gives a D that is off by the weights' roundings times
+  // dp - D alone (the errors of sum p~ dp and D sum p~ cancel), where o's own would be as large as ds in rows that
+  // few keys take most of or whose values have much in common.  (Training only: 64 us with it, 58 without, at 16 / 4
+  // heads of 4096 tokens, d 128, window 1024.)
+  const bool rest = sizeof(T) == 2 && a.o_rest && !win_few_keys(a, (qt + 1) * WIN_RES);
+  float m = NEG_BIG, l = 0.f, lr = 0.f;
   f32x16 acc[E::NT] = {};
 
   constexpr uint64_t KEYS = RowBits<E::BK>::ALL;  // all keys of a tile inside and unmasked
@@ -133,6 +139,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       const float to = fmaxf(mx, m), al = fast_exp2(m - to);
       m = to;
       l *= al;
+      lr *= al;
 #pragma unroll
       for (int n = 0; n < E::NT; ++n) acc[n] *= al;
     }
@@ -148,12 +155,17 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
       l += s;
       typename E::Prob p;
       E::to_operand(y[sub], p);
+      if constexpr (sizeof(T) == 2) {
+        if (rest) lr += E::operand_sum(p, 0.f);
+      }
       E::template column_product<true>(tv, 32 * sub, p, acc, lane);
     }
   }
   l = xor32_pair(l, false);
   const bool some = row_ok && l > 0.f;
   const float inv = some ? 1.f / l : 0.f;
+  lr = xor32_pair(lr, false);
+  const float inv_r = some ? 1.f / lr : 0.f;
   if (i < a.M) {
     const size_t row = ((size_t)b * a.H + h) * a.M + i;
     if (a.lse && h32 == 0) a.lse[row] = some ? m + fast_log2(l) : LSE_EMPTY;
@@ -167,6 +179,19 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
         for (int e = 0; e < 4; ++e) w[e] = some ? acc[n][r + e] * inv : 0.f;
         store4<T, FAST>(o, 32 * n + acc_row(r, h32), a.d, w);
       }
+    if (rest) {
+      T* left = reinterpret_cast<T*>(a.o_rest) + row * a.d;
+#pragma unroll
+      for (int n = 0; n < E::NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          f32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = some ? acc[n][r + e] * inv_r - to_f32(from_f32<T>(acc[n][r + e] * inv)) : 0.f;
+          store4<T, FAST>(left, 32 * n + acc_row(r, h32), a.d, w);
+        }
+    }
   }
 }
 
@@ -174,7 +199,7 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) w
 template <typename T> static bool win_fast(const WinArgs& a, bool bwd) {
   auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
   auto st = [](long long s) { return ((s * (long long)sizeof(T)) & 15) == 0; };
-  bool ok = (a.d * sizeof(T)) % 16 == 0 && al(a.q) && al(a.k) && al(a.v) && al(a.o);
+  bool ok = (a.d * sizeof(T)) % 16 == 0 && al(a.q) && al(a.k) && al(a.v) && al(a.o) && al(a.o_rest);
   ok = ok && st(a.qsb) && st(a.qsh) && st(a.qsn) && st(a.ksb) && st(a.ksh) && st(a.ksn) && st(a.vsb) && st(a.vsh) &&
        st(a.vsn);
   if (bwd) ok = ok && al(a.go) && al(a.dq) && al(a.dk) && al(a.dv);

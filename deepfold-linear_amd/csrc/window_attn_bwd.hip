@@ -14,11 +14,10 @@
 
 namespace dfl {
 
-// Tiles of queries that see at most this many keys each take D_i as the sum of p dp in a pass of its own over them
-// (two products more), so that it holds no rounding of the stored o: where a row has few keys, o's rounding would
-// be as large in ds as ds itself.  With more keys o is small against v and do.o is as good.
-constexpr int WIN_EXACT_KEYS = 256;
-
+// D_i.  Tiles of queries that see at most WIN_EXACT_KEYS keys each take it as the sum of p dp in a pass of its own over
+// them (two products more), so that it holds no rounding of the stored o: where a row has few keys, o's rounding would
+// be as large in ds as ds itself.  With more keys fp32 takes do.o and bf16 do.(o + o_rest), see the forward: 74 us
+// against 115 with the pass at 16 / 4 heads of 4096 tokens, d 128, window 1024.  Without o_rest bf16 has the pass.
 template <typename T, int DP>
 __device__ __forceinline__ float frag_dot(const typename WinEng<T, DP>::Frag& x,
                                           const typename WinEng<T, DP>::Frag& y) {
@@ -93,13 +92,16 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
   E::template load_frag<FAST>(gf, row_ok ? reinterpret_cast<const T*>(a.go) + row * a.d : nullptr, a.d, lane);
   const float sc = a.scale * LOG2E;
   const float lse = row_ok ? a.lse[row] : LSE_EMPTY;
-  const int near = min(a.window, a.N), last = a.causal ? min(a.M, (qt + 1) * WIN_RES) + shift : a.N;
-  const bool exact = min((a.causal ? near : 2 * near - 1) + min(a.n_sink, a.N), last) <= WIN_EXACT_KEYS;
+  const bool exact = win_few_keys(a, (qt + 1) * WIN_RES) || (sizeof(T) == 2 && !a.o_rest);
   float D = 0.f, f = 1.f;
   if (!exact) {
     typename E::Frag of;
     E::template load_frag<FAST>(of, row_ok ? reinterpret_cast<const T*>(a.o) + row * a.d : nullptr, a.d, lane);
     D = frag_dot<T, DP>(of, gf);
+    if constexpr (sizeof(T) == 2) {
+      E::template load_frag<FAST>(of, row_ok ? reinterpret_cast<const T*>(a.o_rest) + row * a.d : nullptr, a.d, lane);
+      D += frag_dot<T, DP>(of, gf);
+    }
   }
 
   // body(p, dp, js) for every 32 x 32 pair that the wave sees something of; `buf`: where the first tile is or goes

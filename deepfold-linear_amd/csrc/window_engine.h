@@ -133,6 +133,16 @@ template <typename T, int DP> struct WinEng {
       o.h[0] = p;
     }
   }
+  // s + the sum of a bf16 operand's values, as they were rounded
+  __device__ static __forceinline__ float operand_sum(const Prob& p, float s) {
+    typedef __attribute__((__vector_size__(2 * sizeof(bf16)))) bf16 pair;
+    const pair ones = {(bf16)1.f, (bf16)1.f};
+    pair x[8];
+    __builtin_memcpy(x, &p, sizeof(x));
+#pragma unroll
+    for (int n = 0; n < 8; ++n) s = __builtin_amdgcn_fdot2_f32_bf16(x[n], ones, s, false);
+    return s;
+  }
   // acc[t] += (columns 32 t .. of rows r0 .. r0 + 31 of the tile)^T P
   template <bool HELD = false>
   __device__ static __forceinline__ void column_product(T* tile, int r0, const Prob& p, f32x16 (&acc)[NT], int lane) {

@@ -74,6 +74,14 @@ struct KeyTiles {
   __host__ __device__ int tile(int it) const { return it < pre ? it : b0 + it - pre; }
 };
 
+// Tiles of queries that see at most this many keys each (those before row `end`): their D_i is the sum of p dp in a
+// pass of its own (window_attn_bwd.hip); of the others, in bf16, the forward keeps what the rounding of o leaves.
+constexpr int WIN_EXACT_KEYS = 256;
+template <class Args> __host__ __device__ inline bool win_few_keys(const Args& a, int end) {
+  const int near = win_min(a.window, a.N), last = a.causal ? win_min(a.M, end) + a.N - a.M : a.N;
+  return win_min((a.causal ? near : 2 * near - 1) + win_min(a.n_sink, a.N), last) <= WIN_EXACT_KEYS;
+}
+
 // The bias by distance: entry rel_lut_base + t - j of rel_lut_size.  REL_PAD entries more than the table's range on
 // both sides hold its end values, so that 32 queries and 32 keys need no clamp where a pair of them is inside the
 // range (rel_far() < 0) and, in one direction, one key is not ahead of all the queries (!none, !none_near,

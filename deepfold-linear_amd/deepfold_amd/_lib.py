@@ -230,7 +230,7 @@ class WindowAttnParams(ctypes.Structure):
         ("B", I32), ("H", I32), ("Hk", I32), ("M", I32), ("N", I32), ("d", I32),
         ("window", I32), ("n_sink", I32), ("causal", I32), ("scale", F32),
         ("o", P), ("lse", P),
-        ("grad_o", P), ("dq", P), ("dk", P), ("dv", P), ("drel_table", P),
+        ("grad_o", P), ("dq", P), ("dk", P), ("dv", P), ("drel_table", P), ("o_rest", P),
     ]
 
 

@@ -71,13 +71,15 @@ def _forward(q, k, v, table, mask, arr, window, n_sink, causal, scale, train):
     B, H, M, d = qc.shape
     o = torch.empty(B, H, M, d, dtype=dt, device=dev)
     lse = torch.empty(B, H, M, dtype=torch.float32, device=dev) if train else None
+    rest = torch.empty_like(o) if train and dt == torch.bfloat16 else None
     p = _fwd_params(dt, qc, kc, vc, mk, tab, arr, window, n_sink, causal, scale, o, lse)
+    p.o_rest = _lib.ptr(rest)
     lib = _lib.load()
     with _lib.on_device(dev):
         rc = _lib.timed_launch("window_attn_fwd", dev, lambda: lib.dfl_window_attn_fwd(
             ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
     _lib.check(rc, "dfl_window_attn_fwd")
-    return (qc, kc, vc, tab, mk, o, lse), (o if dt == q.dtype else o.to(q.dtype))
+    return (qc, kc, vc, tab, mk, o, rest, lse), (o if dt == q.dtype else o.to(q.dtype))
 
 
 class WindowAttnFn(torch.autograd.Function):
@@ -96,7 +98,7 @@ class WindowAttnFn(torch.autograd.Function):
         none = (None,) * 6
         if grad_o is None:
             return (None,) * 4 + none
-        qc, kc, vc, tab, mk, o, lse = ctx.saved_tensors
+        qc, kc, vc, tab, mk, o, rest, lse = ctx.saved_tensors
         arr, window, n_sink, causal, scale, qdt, kdt, vdt, tdt = ctx.meta
         need = ctx.needs_input_grad
         dev, dt = qc.device, qc.dtype
@@ -110,6 +112,7 @@ class WindowAttnFn(torch.autograd.Function):
         p = _fwd_params(dt, qc, kc, vc, mk, tab, arr, window, n_sink, causal, scale, o, lse)
         p.grad_o, p.dq, p.dk, p.dv, p.drel_table = (go.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                                     _lib.ptr(dtab))
+        p.o_rest = _lib.ptr(rest)
         lib = _lib.load()
         # a workspace of the call's own: calls on other streams and captured graphs cannot share it
         ws = torch.empty(lib.dfl_window_attn_workspace_size(B, H, Hk, M, N, d, window, n_sink, int(causal), p.n_edges),

@@ -20,7 +20,11 @@
  * t - window < j <= t (causal = 0: |t - j| < window) or j < n_sink (causal: and j <= t),
  * and mask[b,j] != 0; rows with mask[b,t] = 0, or that see nothing, are zero.  The table's
  * direction is that of the attention: rel_both = !causal.  A table entry of -inf
- * (or below about -1e30) takes its keys out.  scale is positive (1e-30 to 1e30). */
+ * (or below about -1e30) takes its keys out.  scale is positive (1e-30 to 1e30).
+ *
+ * Training: the forward writes lse (B,H,M) and, in bf16, o_rest (B,H,M,d), what the rounding of o leaves; both go to the
+ * backward with o.  o_rest may be NULL: the backward then takes a pass more.  It is not read, nor written, where
+ * dtype is fp32 or the rows see at most 256 keys. */
 typedef struct dfl_window_attn_params {
   int dtype;
   const void* q;
@@ -43,6 +47,7 @@ typedef struct dfl_window_attn_params {
   void* dk;
   void* dv;
   float* drel_table;
+  void* o_rest;
 } dfl_window_attn_params;
 
 /* Rolling cache of S = n_sink + window slots (B,Hk,S,d): position p < n_sink lies in slot p,

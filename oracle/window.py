@@ -13,6 +13,11 @@ rounded, u = 0), w the results' half step and e the bound of the fp32 arithmetic
 * o: (u + e) sum p |v| + w |o|; dv: (u + e) sum p |do| + w |dv|;
 * D = do.o: from the stored o, sum |do| err(o), or as the sum of p dp (kernels do so where a row tile
   sees few keys): e' sum p |do|.|v| with e' = 2 e + (n + d) 2^-24; the larger of the two is used;
+  With ``remainder`` the tighter bound of a D that does not know the stored o's rounding: what the forward kept
+  is sum p~ v / sum p~ of the rounded probabilities p~ = p (1 + eps_j), |eps_j| <= u, in two roundings of the
+  operand type (the first o's own; the second, of what is left of it, at most 2 u |o| before and so 2 u u |o| off).  As
+  sum p~ dp / sum p~ - D = sum p eps (dp - D) / (1 + sum p eps), that D is off by u / (1 - u) sum p |dp - D| +
+  2 u u sum |do| |o| + e' sum p |do|.|v|;
 * ds = p (dp - D): e' p (|do|.|v| + sum p |do|.|v|) + p err(D);
 * dq, dk: sums of (u |ds| + err(ds)) against |k|, |q|, plus (n + 8) 2^-24 of sum |ds| |k|, plus w of the result;
 * dtable: sums of err(ds) and (n + 8) 2^-24 |ds| by bucket, plus its own rounding.
@@ -73,7 +78,7 @@ def _by_group(x, Hk):
 
 
 def attention(q, k, v, *, window, n_sink=0, causal=True, mask=None, scale=None, table=None, edges=None, grad=None,
-              operand=torch.float32, result=torch.float32, table_dtype=torch.float32):
+              operand=torch.float32, result=torch.float32, table_dtype=torch.float32, remainder=False):
     """Values and bounds: {"o", "dq", "dk", "dv", "dtable"} -> (float64 value, elementwise bound)."""
     q, k, v = q.double(), k.double(), v.double()
     B, H, M, d = q.shape
@@ -118,6 +123,8 @@ def attention(q, k, v, *, window, n_sink=0, causal=True, mask=None, scale=None, 
     D, Da = (p * dp).sum(-1, keepdim=True), (p * dpa).sum(-1, keepdim=True)
     ds = p * (dp - D)
     dD = torch.maximum((g.abs() * out["o"][1]).sum(-1, keepdim=True), e2 * Da)
+    if remainder:
+        dD = u / (1 - u) * ds.abs().sum(-1, keepdim=True) + 2 * u * u * (g.abs() * o.abs()).sum(-1, keepdim=True) + e2 * Da
     eds = e2 * p * (dpa + Da) + p * dD
     a = ds.abs()
     soft = u * a + eds + (n + 8) * U32 * a

@@ -59,3 +59,65 @@ def test_bias_gradient_of_many_heads_and_a_large_plane():
     far = int((rel <= -700).sum())
     want = value.double()[:, None] * torch.tensor([M * N - far, far]).double()
     holds("dtable", g, want, (1024 + 10 + 1) * ref.U32 * want)
+
+
+def hard_rows(kind, causal, dtype, d, N=700, H=2, Hk=1):
+    """Rows whose outputs are large against their score gradients, among more than 256 keys each."""
+    q, k, v = rnd(1, H, N, d, seed=1), rnd(1, Hk, N, d, seed=2), rnd(1, Hk, N, d, seed=3)
+    mask = table = None
+    if kind == "sharp":  # one key or a few take most of a row
+        q = q * 6
+    elif kind == "sharper":
+        q = q * 14
+    elif kind == "offset":  # values with a large common part: the softmax gradient cancels it
+        v = v + 9
+    elif kind == "masked":  # padding on the left and holes: few keys are left of a wide window
+        mask = (torch.rand(1, N, generator=torch.Generator().manual_seed(5)) < 0.02).float()
+        mask[0, -3:] = 1
+    elif kind == "table":  # entries of -inf leave the three nearest keys (of either side)
+        table = rnd(H, 4 * (1 if causal else 2), seed=6)
+        table[:, 3::4] = -math.inf
+    return [t.to(dtype) for t in (q, k, v)], mask, table
+
+
+@pytest.mark.parametrize("d", [8, 16, 40, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kind", ["sharp", "sharper", "offset", "masked", "table", "plain"])
+def test_score_gradients_know_no_rounding_of_the_output(kind, causal, d):
+    """bf16 rows that see more than 256 places: D is as good as the rounded probabilities, not as the rounded output."""
+    (q, k, v), mask, table = hard_rows(kind, causal, BF, d)
+    go = rnd(*q.shape, seed=4, dtype=BF)
+    kw = dict(window=600, n_sink=3, causal=causal)
+    want = ref.attention(q, k, v, mask=mask, table=table, edges=(1, 2, 3), grad=go, operand=BF, result=BF, remainder=True, **kw)
+    from deepfold_amd import flash_window_attn
+
+    x = [leaf(t) for t in (q, k, v, table)]
+    o = flash_window_attn(*x[:3], None if mask is None else mask.to(DEV), rel_table=x[3],
+                          rel_edges=None if table is None else (1, 2, 3), **kw)
+    grads = torch.autograd.grad(o, [t for t in x if t is not None], go.to(DEV))
+    for name, got in zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)):
+        holds(f"{kind} {name}", got, *want[name])
+
+
+@pytest.mark.parametrize("kind", ["sharp", "offset", "table"])
+def test_backward_without_the_remainder(kind, monkeypatch):
+    """A caller of the C entries that kept only o: the backward forms D from the products themselves."""
+    from deepfold_amd import flash_window_attn, window_attn
+
+    (q, k, v), mask, table = hard_rows(kind, True, BF, 16)
+    go = rnd(*q.shape, seed=4, dtype=BF)
+    kw = dict(window=600, n_sink=3)
+    want = ref.attention(q, k, v, mask=mask, table=table, edges=(1, 2, 3), grad=go, operand=BF, result=BF, remainder=True, **kw)
+    forward = window_attn._forward
+
+    def dropped(*args):
+        (*head, rest, lse), out = forward(*args)
+        assert rest is not None
+        return (*head, None, lse), out
+
+    monkeypatch.setattr(window_attn, "_forward", dropped)
+    x = [leaf(t) for t in (q, k, v, table)]
+    o = flash_window_attn(*x[:3], rel_table=x[3], rel_edges=None if table is None else (1, 2, 3), **kw)
+    grads = torch.autograd.grad(o, [t for t in x if t is not None], go.to(DEV))
+    for name, got in zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)):
+        holds(f"{kind} {name}", got, *want[name])
