@@ -30,7 +30,7 @@ struct WinArgs {
   void* dk;        // (B,Hk,N,d) contiguous
   void* dv;
   float* dtable;    // (H, buckets) or null
-  float* rowd;      // [B*H][M][2]: D_i and the row's factor (0 where one key takes the whole row, else 1)
+  float* rowd;      // [B*H][M][2]: D_i and the row's factor (0 where the row has one key, else 1)
   float* sink_part; // [B*Hk][n_chunks + 1][n_sink][2][DP] partial dK / dV of the first tokens (n_chunks > 0)
   float* kv_part;   // [kv_split][B*Hk][N][2][DP] partial dK / dV (kv_split > 1)
   float* tab_part;  // [B*H*q blocks][buckets]

@@ -157,22 +157,23 @@ __global__ void __launch_bounds__(WIN_NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
 
   int buf = 0;
   if (exact) {
-    float sum = 0.f, sdp = 0.f, top = 0.f;
+    float sum = 0.f, sdp = 0.f, top = 0.f, next = 0.f;  // next: the second largest weight
     sweep(
         [&](const f32x16& p, const f32x16& dp, int, int, T*, int) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             sum += p[r];
             sdp = __builtin_fmaf(p[r], dp[r], sdp);
+            next = __builtin_amdgcn_fmed3f(p[r], top, next);
             top = fmaxf(top, p[r]);
           }
         },
         buf, true);
     sum = xor32_pair(sum, false);
     sdp = xor32_pair(sdp, false);
-    top = xor32_pair(top, true);
-    // a row that one key takes whole has no score gradient; its rounding errors are none either
-    f = (sum > 0.f && top == sum) ? 0.f : 1.f;
+    next = fmaxf(xor32_pair(next, true), -xor32_pair(-top, true));  // the lane pair's smaller top is a candidate
+    // a row with one key has no score gradient; its rounding errors are none either
+    f = (sum > 0.f && next == 0.f) ? 0.f : 1.f;
     D = (sum > 0.f && f != 0.f) ? sdp / sum : 0.f;
   }
   if (i < a.M && h32 == 0) {

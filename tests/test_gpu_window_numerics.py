@@ -121,3 +121,25 @@ def test_backward_without_the_remainder(kind, monkeypatch):
     grads = torch.autograd.grad(o, [t for t in x if t is not None], go.to(DEV))
     for name, got in zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)):
         holds(f"{kind} {name}", got, *want[name])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("N", [5, 100, 400])
+def test_small_weights_beside_a_dominant_key(N, dtype):
+    """One key outweighs the others by far more than fp32 holds beside 1 (e^-20 .. e^-30 each): the others' own gradients
+    are small, not zero, in rows of few keys as in rows of many."""
+    H, d = 2, 8
+    q, k, v = rnd(1, H, N, d, seed=1), rnd(1, H, N, d, seed=2), rnd(1, H, N, d, seed=3)
+    q[..., 0] = 8 + q[..., 0].abs()  # against key 0, the first token: scores of 22 and more
+    k[:, :, 1:, 0] = 0
+    k[:, :, 0, 0] = 8
+    q, k, v, go = (t.to(dtype) for t in (q, k, v, rnd(1, H, N, d, seed=4)))
+    want = ref.attention(q, k, v, window=N, n_sink=1, grad=go, operand=dtype, result=dtype, remainder=True)
+    from deepfold_amd import flash_window_attn
+
+    x = [leaf(t) for t in (q, k, v)]
+    o = flash_window_attn(*x, window=N, n_sink=1)
+    grads = torch.autograd.grad(o, x, go.to(DEV))
+    for name, got in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        holds(name, got, *want[name])
+    assert grads[1][:, :, 1:].any()
