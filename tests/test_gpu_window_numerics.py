@@ -143,3 +143,83 @@ def test_small_weights_beside_a_dominant_key(N, dtype):
     for name, got in zip(("o", "dq", "dk", "dv"), (o, *grads)):
         holds(name, got, *want[name])
     assert grads[1][:, :, 1:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("scale", [0.01, 0.6, 3.0])
+def test_scales(scale, causal, dtype):
+    """A scale of the caller's own, in short and long rows, forward and both passes of the backward."""
+    attention_case(2, 4, 2, 130, 150, 24, dtype, 40, 3, causal, True, scale=scale)
+    attention_case(1, 2, 1, 520, 520, 64, dtype, 400, 4, causal, True, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("growth", [3.0, 14.0, -14.0, 60.0])
+def test_scores_that_grow_along_the_sequence(growth, causal, dtype):
+    """Each 64 keys raise (or lower) the scores by ``growth`` in log2: the running reference moves up in steps of any size
+    (8 and more rescale a row), or stays at the first keys."""
+    from deepfold_amd import flash_window_attn
+
+    B, H, Hk, N, d, scale = 1, 4, 2, 450, 16, 0.4
+    q, k, v, go = (rnd(B, h, N, d, seed=s) for s, h in ((1, H), (2, Hk), (3, Hk), (4, H)))
+    # column 0: q 1, k the wanted score / (scale log2 e)
+    q[..., 0] = 1
+    k[..., 0] = torch.arange(N) / 64 * growth / (scale * math.log2(math.e))
+    q, k, v, go = (t.to(dtype) for t in (q, k, v, go))
+    table = rnd(H, (len(EDGES) + 1) * (1 if causal else 2), seed=5)
+    # A weight below 2^-126, fp32's smallest normal number, may be zero in the kernel (at a growth of 60 they go down to
+    # 2^-420): each of the H / Hk N of a key's rows is then off by 2^-126 times at most |q|, |k| or |do| and |dp - D| <=
+    # 2 max |do|.|v|, each taken as its largest, plus as much for the result itself.
+    big = max(float(t.abs().max()) for t in (q, k, go)) * (1 + 2 * float(go.double().abs().sum(-1).max() * v.abs().max()))
+    tiny = 2.0 ** -126 * (H // Hk * N * N + 1) * big
+    for window, n_sink in ((450, 0), (200, 2)):
+        kw = dict(window=window, n_sink=n_sink, causal=causal, scale=scale)
+        want = ref.attention(q, k, v, table=table, edges=EDGES, grad=go, operand=dtype, result=dtype,
+                             remainder=dtype == BF, **kw)
+        x = [leaf(t) for t in (q, k, v, table)]
+        o = flash_window_attn(*x[:3], rel_table=x[3], rel_edges=EDGES, **kw)
+        grads = torch.autograd.grad(o, x, go.to(DEV))
+        for name, got in zip(("o", "dq", "dk", "dv", "dtable"), (o, *grads)):
+            holds(f"{name} window {window}", got, want[name][0], want[name][1] + tiny)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale,growth", [(0.02, 0.0), (2.0, 0.0), (0.5, 20.0), (0.5, -20.0)])
+def test_decode_scales_and_growth(scale, growth, dtype):
+    from deepfold_amd import window_decode_attn
+
+    B, H, Hk, d, window, n_sink = 3, 8, 2, 48, 700, 2
+    S = window + n_sink
+    q, k, v = rnd(B, H, d, seed=1), rnd(B, Hk, d, seed=2), rnd(B, Hk, d, seed=3)
+    kc, vc = rnd(B, Hk, S, d, seed=4), rnd(B, Hk, S, d, seed=5)
+    q[..., 0] = 1
+    if growth:
+        kc[..., 0] = torch.arange(S) / 64 * growth / (scale * math.log2(math.e))
+    lengths = torch.tensor([S - 1, 350, 5 * S])
+    table = rnd(H, len(EDGES) + 1, seed=6)
+    q, k, v, kc, vc = (t.to(dtype) for t in (q, k, v, kc, vc))
+    want, bound, _, _ = ref.decode(q, k, v, kc, vc, lengths, n_sink, scale=scale, table=table, edges=EDGES, operand=dtype,
+                                   result=dtype)
+    o = window_decode_attn(*(t.to(DEV) for t in (q, k, v, kc, vc, lengths)), n_sink=n_sink, scale=scale,
+                           rel_table=table.to(DEV), rel_edges=EDGES)
+    holds("o", o, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_gradients_beside_an_outweighing_table_entry(dtype):
+    """Entries of -1e9, which keep no digits of the scores beside them: heads with other keys are right, all is finite."""
+    from deepfold_amd import flash_window_attn
+
+    H, N, d, edges = 2, 140, 32, (1, 2, 4)
+    x = [rnd(1, H, N, d, seed=s, dtype=dtype) for s in (1, 2, 3)]
+    go, table = rnd(1, H, N, d, seed=4, dtype=dtype), rnd(H, 4, seed=5)
+    gone = table.clone()
+    table[:, 2:], gone[:, 2:] = -1e9, -math.inf  # a key two or more away: the same weights of zero
+    y = [leaf(t) for t in (*x, table)]
+    o = flash_window_attn(*y[:3], window=50, rel_table=y[3], rel_edges=edges)
+    got = (o, *torch.autograd.grad(o, y, go.to(DEV)))
+    want = ref.attention(*x, window=50, table=gone, edges=edges, grad=go, operand=dtype, result=dtype)
+    for name, t in zip(("o", "dq", "dk", "dv", "dtable"), got):
+        holds(name, t, *want[name])
