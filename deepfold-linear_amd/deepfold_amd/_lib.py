@@ -393,13 +393,11 @@ def to_int32(t: torch.Tensor) -> torch.Tensor:
     return t.to(torch.int32)
 
 
-def through_autograd(*tensors) -> bool:
-    """Whether a call must go through its ``autograd.Function`` rather than straight to the launch: an input asks for a
-    gradient, a trace is being recorded (it holds a Function's call, but not what a launch writes), or forward-mode
+def recording() -> bool:
+    """Whether a call that needs no gradient must go through its ``autograd.Function`` all the same rather than straight
+    to the launch: a trace is being recorded (it holds a Function's call, but not what a launch writes), or forward-mode
     differentiation is on (a Function refuses inputs with tangents, a launch would drop them)."""
-    if torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0:
-        return True
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
 
 
 class on_device:

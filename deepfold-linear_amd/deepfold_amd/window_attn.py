@@ -179,7 +179,8 @@ def flash_window_attn(
     if B == 0 or H == 0 or M == 0:
         _lib.require_gpu(Q, K, V)
         raise ValueError("flash_window_attn: empty batch, heads or queries")
-    if _lib.through_autograd(Q, K, V, rel_table):
+    if _lib.recording() or torch.is_grad_enabled() and (
+            Q.requires_grad or K.requires_grad or V.requires_grad or (rel_table is not None and rel_table.requires_grad)):
         O = WindowAttnFn.apply(Q, K, V, rel_table, mask, arr, window, n_sink, causal, scale)
     else:
         O = _forward(Q, K, V, rel_table, mask, arr, window, n_sink, causal, scale, False)[1]
@@ -324,7 +325,7 @@ def window_cache_fill(
         raise TypeError(f"{what}: K is {K.dtype}, V is {V.dtype}")
     _check_caches(what, k_cache, v_cache, B, Hk, d, K.dtype, int(n_sink))
     _check_lengths(what, lengths, B)
-    run = _CacheFillFn.apply if _lib.through_autograd(K, V, k_cache, v_cache) else _fill
+    run = _CacheFillFn.apply if _lib.recording() else _fill
     run(K, V, lengths, k_cache, v_cache, int(n_sink))
 
 
@@ -366,5 +367,5 @@ def window_decode_attn(
     if (rel_table is None) != (rel_edges is None):
         raise ValueError(f"{what}: give rel_table and rel_edges together")
     arr = None if rel_table is None else edge_array(rel_table, rel_edges, H, False)
-    run = _DecodeFn.apply if _lib.through_autograd(q, k, v, k_cache, v_cache, rel_table) else _decode
+    run = _DecodeFn.apply if _lib.recording() else _decode
     return run(q, k, v, k_cache, v_cache, lengths, rel_table, arr, n_sink, _scale(what, scale, d))
