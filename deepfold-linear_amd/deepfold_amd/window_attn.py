@@ -35,6 +35,7 @@ from .rel_pos_bias import edge_array
 
 MAX_HEAD_DIM = 128
 MAX_SINK = 128
+EXACT_KEYS = 256  # rows of at most this many keys need no remainder of o (csrc/window_geometry.h)
 
 
 def _check_window(what, window, n_sink):
@@ -71,7 +72,9 @@ def _forward(q, k, v, table, mask, arr, window, n_sink, causal, scale, train):
     B, H, M, d = qc.shape
     o = torch.empty(B, H, M, d, dtype=dt, device=dev)
     lse = torch.empty(B, H, M, dtype=torch.float32, device=dev) if train else None
-    rest = torch.empty_like(o) if train and dt == torch.bfloat16 else None
+    # (without it the backward forms D from the products, as it does for rows of so few keys in any case)
+    keys = min((window if causal else 2 * window - 1) + n_sink, kc.shape[2])
+    rest = torch.empty_like(o) if train and dt == torch.bfloat16 and keys > EXACT_KEYS else None
     p = _fwd_params(dt, qc, kc, vc, mk, tab, arr, window, n_sink, causal, scale, o, lse)
     p.o_rest = _lib.ptr(rest)
     lib = _lib.load()

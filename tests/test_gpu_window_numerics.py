@@ -223,3 +223,45 @@ def test_gradients_beside_an_outweighing_table_entry(dtype):
     want = ref.attention(*x, window=50, table=gone, edges=edges, grad=go, operand=dtype, result=dtype)
     for name, t in zip(("o", "dq", "dk", "dv", "dtable"), got):
         holds(name, t, *want[name])
+
+
+def test_graph_replays_of_wide_windows():
+    """A training step whose rows see more than 256 keys, captured and replayed on new inputs with eager work between."""
+    from deepfold_amd import flash_window_attn
+
+    x = [rnd(1, h, 600, 64, seed=s, dtype=BF).to(DEV) for s, h in ((1, 4), (2, 2), (3, 2))]
+    go = rnd(1, 4, 600, 64, seed=4, dtype=BF).to(DEV)
+
+    def train():
+        y = [t.detach().requires_grad_(True) for t in x]
+        o = flash_window_attn(*y, window=400, n_sink=4)
+        return [o, *torch.autograd.grad(o, y, go)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        train()
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = train()
+    for step in range(3):
+        for t in (*x, go):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(70 + step)).to(BF))
+        g.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, train()))
+
+
+@pytest.mark.parametrize("window,n_sink,causal,kept", [(252, 4, True, False), (253, 4, True, True), (126, 5, False, False),
+                                                       (127, 4, False, True), (2000, 0, True, True)])
+def test_the_remainder_is_kept_where_it_is_used(window, n_sink, causal, kept):
+    from deepfold_amd import window_attn
+
+    x = [rnd(1, 2, 400, 64, seed=s, dtype=BF).to(DEV) for s in (1, 2, 3)]
+    for train in (True, False):
+        saved, _ = window_attn._forward(*x, None, None, None, window, n_sink, causal, 0.1, train)
+        assert (saved[6] is not None) == (kept and train)
+    saved, _ = window_attn._forward(*(t.float() for t in x), None, None, None, window, n_sink, causal, 0.1, True)
+    assert saved[6] is None
