@@ -111,7 +111,11 @@ struct Chunks {
 // Parts of a key tile's queries (window_attn_bwd.hip: 64 keys, 64 queries a step).  Below two workgroups a CU the
 // key pass waits for its own loads and barriers most of the time: at 16 / 4 heads of 4096 tokens, 256 workgroups,
 // window 1024, it takes 171 us in one part and, with 10 us more for joining them, 146 us in two; four gave the same as
-// two.  A part has at least 8 steps, so that the joining stays small beside it.
+// two.  A part has at least 8 steps, so that the joining stays small beside it.  Whole training steps (us) in one part,
+// by this rule, and with twice the workgroups and half the steps: 16 / 4 heads of 4096 tokens, d 128 as above 294, 270,
+// 275; 8 of 2048, d 64, window 512 68, 68, 77; 2 x 8 / 2 of 1500, d 64, 200 both ways 115, 83, 87; fp32 8 / 2 of 2000,
+// d 64, window 700 467, 266, 272; 32 / 8 of 1024, d 128 216, 134, 139; 4 / 1 of 600, d 64, all both ways 118, 66, 60;
+// fp32 4 of 1000, d 32, 300 both ways 146, 146, 131; fp32 8 of 4096, d 128, window 1024 844, 840, 885.
 int kv_split(int B, int H, int Hk, int M, int N, int window, int causal) {
   const long long tiles = ((long long)N + 63) / 64 * B * Hk;
   const long long w = std::min(window, N), band = std::min<long long>(M, 63 + (causal ? w : 2 * w - 1));
@@ -170,8 +174,11 @@ dfl::WinArgs attn_args(const dfl_window_attn_params* p) {
   return a;
 }
 
-// Splits of a cache: about three workgroups a CU, what its registers let run at once (with 1024 a second, mostly empty
-// round follows), at least 64 slots each.
+// Splits of a cache: about three workgroups a CU, what the registers of the bf16 form with four heads a group let run at
+// once (with 1024 a second, mostly empty round follows), at least 64 slots each.  Calls (us) with 512, 768 and 1024:
+// bf16 32 x 32 / 8 heads, 4100 slots, d 128 125, 117, 132; fp32 8 x 32 / 8, the same 52, 54, 55; bf16 16 x 16, 2052
+// slots, d 64 31, 31, 31; fp32 8 x 16, 504 slots, d 32, table 17, 16, 17; bf16 1 x 16 / 4, 1028 slots, d 64 20, 15, 20;
+// 1 x 32 / 8, 16388 slots, d 128 30, 30, 35.
 constexpr int DECODE_WG = 768, DECODE_MIN = 64;
 struct Splits {
   int n, chunk;

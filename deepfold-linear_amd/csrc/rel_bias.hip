@@ -6,7 +6,7 @@
 //
 // Bounds: the plane's bytes, once.  Forward 16 us for 34 MB (16 heads of 1024 x 1024 in bf16: half of it launch and the
 // tables in LDS) and 58 us for 155 MB (4 x 16 of 777 x 777 in fp32, where a row's 16-byte stores start at any element);
-// backward 17 and 92 us: a thread's read-add-write of its column for each run of one bucket, a chain of LDS latencies.
+// backward 17 and 94 us: a thread's read-add-write of its column for each run of one bucket, a chain of LDS latencies.
 #include "window_engine.h"
 
 #include <algorithm>

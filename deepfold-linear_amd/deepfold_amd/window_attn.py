@@ -148,7 +148,8 @@ def flash_window_attn(
     Q (B,H,M,D) or (H,M,D); K, V (B,Hk,N,D) or (Hk,N,D) with H a multiple of Hk (query head h reads key head
     h // (H // Hk)), M <= N, D <= 128, any strides.  mask (B,N) or (N,), 0 = masked: a masked key reaches nothing,
     whatever its values, and rows of masked queries are zero, as is a row that sees no key.  (A key that only the
-    window hides is ordinary data: a NaN or infinity in its V may reach queries nearby.)  ``scale`` defaults to
+    window or the table hides is ordinary data: a NaN or infinity in its V may reach queries nearby, and one in the
+    gradient of a query's row the keys nearby.)  ``scale`` defaults to
     D ** -0.5 and is positive.  ``rel_table`` with ``rel_edges``: scores get table[h, bucket(j - t)], see ``rel_pos_bias``, whose
     ``bidirectional`` is ``not causal`` here; an entry of -inf (or below -1e30) takes its keys out.
 
