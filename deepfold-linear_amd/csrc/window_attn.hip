@@ -9,7 +9,8 @@
 // buffer during this one's products.
 //
 // Bounds (MI355X, bf16, d 128, window 2048, 32 / 8 heads of 8192 tokens with a table, 240 GFLOP): 322 us among other
-// passes, 745 TFLOP/s (379 us under a kernel trace), against 190 us at the rate of a large library product and 115 us at what the matrix instructions alone reach.
+// passes, 745 TFLOP/s (379 us under a kernel trace), against 190 us at the rate of a large library product and 115 us at
+// what the matrix instructions alone reach.
 // A wave's step of 64 keys is 32 matrix instructions (1024 cycles of its SIMD) and about 220 others (1100 cycles with
 // the 32 exponentials at a quarter rate); two waves a SIMD overlap the two in part, the rest is their barrier and LDS
 // latency.  32 queries a wave and not 64: twice the queries would halve the LDS reads, which take 22 % of the time, but

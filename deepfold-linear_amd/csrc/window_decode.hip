@@ -3,10 +3,10 @@
 // Position p < n_sink lies in slot p, any other in slot n_sink + (p - n_sink) % window: what the slots hold once
 // token t is in is exactly what t sees, so a token reads each slot in use once and nothing else.
 //
-// Bounds: the cache's bytes, once for four query heads of a key head (a group of heads more reads them once more: 8
-// sequences of 4100 slots, 32 / 4 heads, d 128, bf16, 67 MB: 38 us).  32 sequences of 4100 slots, 32 / 8 heads, d 128, bf16, 537 MB: 107 us, 5.0 TB/s of the
-// 6.2-6.4 that a copy or read reaches (join 5 us more); 270 MB of prompts into 32 caches: 43 us, 6.2 TB/s.  One sequence of
-// 1028 slots, 16 / 4 heads, d 64: 7 + 3.5 us, both of them latency.
+// Bounds: the cache's bytes, once for four query heads of a key head (each group of heads more reads them once more: 8
+// sequences of 4100 slots, 32 / 4 heads, d 128, bf16, 67 MB: 38 us).  32 sequences of 4100 slots, 32 / 8 heads, d 128,
+// bf16, 537 MB: 106 us, 5.0 TB/s of the 6.2-6.4 that a copy or read reaches (join 5 us more); 270 MB of prompts into 32
+// caches: 43 us, 6.2 TB/s.  One sequence of 1028 slots, 16 / 4 heads, d 64: 7 + 3.6 us, both of them latency.
 #include "window_engine.h"
 
 #include <algorithm>

@@ -148,8 +148,9 @@ def rel_pos_bias(
     table (H, buckets); query i stands at position i + n_key - n_query and key j at j, or, with
     ``q_pos`` (B, n_query) / (n_query,) and ``k_pos`` (B, n_key) / (n_key,) integers, where those say (one of them
     alone stands for both if n_query == n_key).  Positions are held in 32 bits: one beyond them stands at their end, so
-    shift a sample's positions into [-2^31, 2^31) first (only differences count).  Returns (H, n_query, n_key), or (B, H, n_query, n_key) with
-    batched positions, contiguous, in ``dtype`` (bf16 or fp32; default: the table's if it is one of them)."""
+    shift a sample's positions into [-2^31, 2^31) first (only differences count).  Returns (H, n_query, n_key), or
+    (B, H, n_query, n_key) with batched positions, contiguous, in ``dtype`` (bf16 or fp32;
+    default: the table's if it is one of them)."""
     M = int(n_query)
     N = M if n_key is None else int(n_key)
     if M < 1 or N < 1:

@@ -150,8 +150,8 @@ def flash_window_attn(
     whatever its values, and rows of masked queries are zero, as is a row that sees no key.  (A key that only the
     window or the table hides is ordinary data: a NaN or infinity in its V may reach queries nearby, and one in the
     gradient of a query's row the keys nearby.)  ``scale`` defaults to
-    D ** -0.5 and is positive.  ``rel_table`` with ``rel_edges``: scores get table[h, bucket(j - t)], see ``rel_pos_bias``, whose
-    ``bidirectional`` is ``not causal`` here; an entry of -inf (or below -1e30) takes its keys out.
+    D ** -0.5 and is positive.  ``rel_table`` with ``rel_edges``: scores get table[h, bucket(j - t)], see
+    ``rel_pos_bias``, whose ``bidirectional`` is ``not causal`` here; an entry of -inf (or below -1e30) takes its keys out.
 
     Returns O with the shape and dtype of Q; gradients to Q, K, V and rel_table."""
     if not Q.dim() == K.dim() == V.dim() or Q.dim() not in (3, 4):
@@ -316,9 +316,10 @@ def window_cache_fill(
     """Copies a prompt's keys and values into the rolling caches, in place.
 
     K, V (B,Hk,N,D), any strides, in memory of their own; lengths (B,) int32 or int64: rows 0 .. lengths[b] - 1 are the
-    prompt (above N counts as N, below 1 leaves the sample's caches alone).  k_cache, v_cache (B,Hk,n_sink + window,D): position p < n_sink goes
-    to slot p, any other to slot n_sink + (p - n_sink) % window, the last of those that share one; slots that no
-    position of the prompt belongs to keep what they hold."""
+    prompt (above N counts as N, below 1 leaves the sample's caches alone).  k_cache, v_cache
+    (B,Hk,n_sink + window,D): position p < n_sink goes to slot p, any other to slot n_sink + (p - n_sink) % window, the
+    last of those that share one; slots that no position of the prompt belongs to keep what they hold.  The two caches
+    may interleave in one buffer, but have no element in common."""
     what = "window_cache_fill"
     if K.dim() != 4 or K.shape != V.shape:
         raise ValueError(f"{what}: K and V must be (B,Hk,N,D) alike")
@@ -351,8 +352,8 @@ def window_decode_attn(
 
     q (B,H,D); k, v (B,Hk,D) the token's own key and value, which enter k_cache, v_cache (B,Hk,n_sink + window,D) in
     place at position lengths[b], the number of tokens that the sample's cache has taken so far; lengths (B,) int32 or
-    int64, below 2^31 (above counts as 2^31 - 1), on the device, not changed by the call; a sample with lengths[b] < 0 has no token: its output is zero and its caches
-    stay as they are.  All of q, k, v and the caches in bf16 or all in fp32.  The table has one direction
+    int64, below 2^31 (above counts as 2^31 - 1), on the device, not changed by the call; a sample with
+    lengths[b] < 0 has no token: its output is zero and its caches stay as they are.  All of q, k, v and the caches in bf16 or all in fp32.  The table has one direction
     (len(rel_edges) + 1 buckets).  No gradient.  Returns o (B,H,D)."""
     what = "window_decode_attn"
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape:
