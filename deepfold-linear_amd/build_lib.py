@@ -19,7 +19,7 @@ SOURCES = ["capi.hip", "sinkhorn_fwd.hip", "sinkhorn_fwd_stream.hip", "sinkhorn_
            "sinkhorn_fwd_blk.hip", "sinkhorn_bwd.hip",
            "sinkhorn_bwd_stream.hip", "sinkhorn_bwd_reg.hip", "attention.hip", "dense.hip", "balanced_bwd.hip",
            "unrolled_bwd.hip", "trunk_steps.hip", "capi_window.hip", "window_attn.hip", "window_attn_bwd.hip",
-           "window_decode.hip", "rel_bias.hip"]
+           "window_decode.hip", "rel_bias.hip", "capi_lowbit.hip", "lowbit_cache.hip", "lowbit_decode.hip", "int8_linear.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # issue-rate / exchange probes (bench.py --workload peaks only): a library of its own
 PROBE_SOURCE = "peaks.hip"

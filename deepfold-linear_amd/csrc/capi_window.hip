@@ -258,7 +258,7 @@ int dfl_window_attn_bwd(const dfl_window_attn_params* p, void* workspace, size_t
   });
 }
 
-int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream) {
+int dfl_window_cache_append(const dfl_window_cache_fill_params* p, const int* starts, void* stream) {
   return guarded([&] {
     if (!p) return fail("params is NULL");
     if (int rc = check_heads(p->dtype, p->B, p->Hk, p->Hk, p->d)) return rc;
@@ -271,6 +271,7 @@ int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream) {
     a.ksb = p->k_stride_b; a.ksh = p->k_stride_h; a.ksn = p->k_stride_n;
     a.vsb = p->v_stride_b; a.vsh = p->v_stride_h; a.vsn = p->v_stride_n;
     a.lengths = p->lengths;
+    a.starts = starts;
     a.kc = p->k_cache; a.vc = p->v_cache;
     a.kcsb = p->kc_stride_b; a.kcsh = p->kc_stride_h; a.kcsn = p->kc_stride_n;
     a.vcsb = p->vc_stride_b; a.vcsh = p->vc_stride_h; a.vcsn = p->vc_stride_n;
@@ -278,6 +279,10 @@ int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream) {
     const hipError_t e = dfl::launch_cache_fill(a, p->dtype == DFL_BF16, (hipStream_t)stream);
     return e == hipSuccess ? 0 : dfl::capi_hip_fail(e, "cache fill launch");
   });
+}
+
+int dfl_window_cache_fill(const dfl_window_cache_fill_params* p, void* stream) {
+  return dfl_window_cache_append(p, nullptr, stream);
 }
 
 size_t dfl_window_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink) {

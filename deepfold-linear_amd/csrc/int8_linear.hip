@@ -1,0 +1,287 @@
+// Products of tokens and weights in 8-bit integers: codes and a scale for each token, formed here, codes and a scale for
+// each row of the weights, and the exact 32-bit integer sums times both scales.
+#include "lowbit_args.h"
+#include "lowbit_codes.h"
+
+#include <initializer_list>
+
+namespace dfl {
+
+typedef __attribute__((__vector_size__(4 * sizeof(int)))) int i32x4;
+typedef __attribute__((__vector_size__(16 * sizeof(int)))) int i32x16;
+
+constexpr float I8_MIN_SCALE = 0x1p-100f;
+
+// The integer nearest to x / s, ties to even: rint(x * (1 / s)) is it or a neighbour, and the remainder x - q s, which
+// one fused multiply-add gives exactly, says which (fp32 quotients would round onto a tie now and then).
+__device__ __forceinline__ float i8_code(float x, float s, float inv) {
+  float q = __builtin_rintf(x * inv);
+  const float r = __builtin_fmaf(-q, s, x), half = 0.5f * s;
+  const bool odd = ((int)q & 1) != 0;
+  if (r > half || (r == half && odd)) q += 1.f;
+  if (r < -half || (r == -half && odd)) q -= 1.f;
+  return q;
+}
+
+// A row a workgroup of 64 W threads, its elements in registers where they fit.
+constexpr int I8_KEEP = 4;  // 8 elements each
+template <typename T, bool FAST, int W> __global__ void __launch_bounds__(64 * W) row_codes_kernel(RowCodesArgs a) {
+  __shared__ unsigned s_top[W];
+  const size_t row = blockIdx.x;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.xs;
+  int8_t* out = a.codes + row * a.cs;
+  float e[I8_KEEP][8];
+  unsigned top = 0;
+  auto look = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  };
+#pragma unroll
+  for (int k = 0; k < I8_KEEP; ++k) {
+    load8<T, FAST>(x, threadIdx.x + k * 64 * W, a.K, e[k]);
+    look(e[k]);
+  }
+  for (int c = threadIdx.x + I8_KEEP * 64 * W; c * 8 < a.K; c += 64 * W) {
+    float v[8];
+    load8<T, FAST>(x, c, a.K, v);
+    look(v);
+  }
+  top = wave_max_u32(top);
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) s_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = max(top, s_top[w]);
+  }
+  const bool fine = top < 0x7f800000u;
+  const float s = fine ? fmaxf(__uint_as_float(top) / 127.f, I8_MIN_SCALE) : __builtin_nanf("");
+  const float inv = 1.f / s;
+  if (threadIdx.x == 0) a.scale[row] = s;
+  auto put = [&](int c, const float (&v)[8]) {
+    unsigned w[2] = {0u, 0u};
+    if (fine) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i / 4] |= ((unsigned)(int)i8_code(v[i], s, inv) & 255u) << (8 * (i % 4));
+    }
+    *reinterpret_cast<uint2*>(out + c * 8) = make_uint2(w[0], w[1]);
+  };
+#pragma unroll
+  for (int k = 0; k < I8_KEEP; ++k) {
+    const int c = threadIdx.x + k * 64 * W;
+    if ((long long)c * 8 < a.cs) put(c, e[k]);
+  }
+  for (int c = threadIdx.x + I8_KEEP * 64 * W; (long long)c * 8 < a.cs; c += 64 * W) {
+    float v[8];
+    load8<T, FAST>(x, c, a.K, v);
+    put(c, v);
+  }
+}
+
+// The sum of a token and a row of weights as a result.
+template <typename T> struct I8Out {
+  const float* ws;
+  const T* bias;
+  T* y;
+  int N;
+  __device__ __forceinline__ explicit I8Out(const Int8LinearArgs& a)
+      : ws(a.w_scale), bias(reinterpret_cast<const T*>(a.bias)), y(reinterpret_cast<T*>(a.y)), N(a.N) {}
+  __device__ __forceinline__ T value(int sum, float as, float wsn, float bn) const {
+    return from_f32<T>(__builtin_fmaf((float)sum * wsn, as, bn));
+  }
+};
+
+// Few tokens: the weights go by once.  A workgroup has 16 rows of weights and MT tiles of 16 tokens; its waves share K,
+// in steps of 64 bytes, straight from memory into the operands: lane l holds row l % 16 and a quarter l / 16 of the step.
+template <typename T, int MT> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
+  constexpr int WAVES = 8, U = 4;
+  __shared__ int s_sum[WAVES][MT][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+  const int8_t* w = a.w + (long long)min(n0 + r, a.N - 1) * a.ws;
+  const int8_t* x[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) x[i] = a.a + (long long)min(m0 + 16 * i + r, a.M - 1) * a.as;
+  const int steps = (a.K + 63) / 64, tail = ((a.K + 15) & ~15) - 16;  // last 16 bytes of a row of weights
+  i32x4 sum[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) sum[i] = i32x4{0, 0, 0, 0};
+  for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
+    i32x4 wv[U], xv[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = min(s0 + u * WAVES, steps - 1) * 64 + 16 * h;
+      wv[u] = *reinterpret_cast<const i32x4*>(w + min(k, tail));  // (past the row's end: tokens are zero there)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xv[u][i] = *reinterpret_cast<const i32x4*>(x[i] + k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * WAVES < steps) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], xv[u][i], sum[i], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s_sum[wave][i][r][4 * h + j] = sum[i][j];  // [token][row of weights]
+  __syncthreads();
+  const I8Out<T> out(a);
+  for (int e = threadIdx.x; e < MT * 256; e += 512) {
+    const int m = e >> 4, c = e & 15;
+    if (m0 + m >= a.M || n0 + c >= a.N) continue;
+    int t = 0;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) t += s_sum[v][m >> 4][m & 15][c];
+    const float b = out.bias ? to_f32(out.bias[n0 + c]) : 0.f;
+    out.y[(size_t)(m0 + m) * a.N + n0 + c] = out.value(t, a.a_scale[m0 + m], out.ws[n0 + c], b);
+  }
+}
+
+// One 16-byte load a lane from `from` to `to` + 16 lane in LDS (`to` uniform, in bytes); waited for by i8_wait.
+__device__ __forceinline__ void i8_load_to_lds(const void* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
+}
+// All but the latest N of the wave's loads done.
+template <int N> __device__ __forceinline__ void i8_wait() {
+  static_assert(N < 64, "vmcnt has six bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+
+// Tiles of TM tokens and TN rows of weights, WM x WN waves of 32 x 32 blocks.  K goes by in steps of 64 bytes through
+// four LDS buffers, loaded three steps ahead without passing through registers; a 64-byte row's 16-byte chunk c lies at
+// position c ^ (row / 4 % 4), so that 16 lanes reading the same chunk of 16 rows meet every bank once.
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs a) {
+  constexpr int NT = 64 * WM * WN, BUF = 4, BK = 64, MI = TM / WM / 32, NI = TN / WN / 32;
+  constexpr int CHUNKS = (TM + TN) * 4, PER = CHUNKS / NT, STEP = NT / 4;  // rows between a thread's chunks
+  static_assert(CHUNKS % NT == 0 && STEP % 16 == 0 && TM % STEP == 0, "whole loads of one swizzle");
+  extern __shared__ __align__(16) int8_t s_tile[];  // [BUF][TM + TN][64]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // neighbouring tiles on one XCD; within it columns of 8 tiles of tokens, so that few rows of weights are in use at once
+  const int mt = (a.M + TM - 1) / TM, nt = (a.N + TN - 1) / TN;
+  int at = blockIdx.x;
+  {
+    const int total = mt * nt, per = total >> 3, rem = total & 7, xcd = at & 7;
+    at = xcd * per + min(xcd, rem) + (at >> 3);
+  }
+  const int band = at / (8 * nt), rows = min(8, mt - band * 8), in = at - band * 8 * nt;
+  const int m0 = (band * 8 + in % rows) * TM, n0 = in / rows * TN;
+
+  const int r0 = threadIdx.x >> 2, chunk = (threadIdx.x & 3) ^ ((r0 >> 2) & 3);
+  const int8_t* from[PER];
+  int last[PER];  // the furthest chunk that a row may be read at
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int r = r0 + p * STEP;
+    if (p * STEP < TM) {
+      from[p] = a.a + (long long)min(m0 + r, a.M - 1) * a.as;
+      last[p] = (int)a.as - 16;
+    } else {
+      from[p] = a.w + (long long)min(n0 + r - TM, a.N - 1) * a.ws;
+      last[p] = ((a.K + 15) & ~15) - 16;  // (past the row's end: tokens are zero there)
+    }
+  }
+  const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t*)s_tile;
+  const unsigned to = __builtin_amdgcn_readfirstlane(base + (threadIdx.x & ~63u) * 16);
+  const int steps = (a.K + BK - 1) / BK;
+  auto issue = [&](int step) {
+    const int k = min(step, steps - 1) * BK + chunk * 16;
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      i8_load_to_lds(from[p] + min(k, last[p]), to + (step % BUF) * (TM + TN) * BK + p * NT * 16);
+  };
+
+  i32x16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = i32x16{};
+  const int wm = wave / WN, wn = wave % WN, row = lane & 31, hi = lane >> 5;
+#pragma unroll
+  for (int s = 0; s < BUF - 1; ++s) issue(s);
+  for (int s = 0; s < steps; ++s) {
+    i8_wait<(BUF - 2) * PER>();
+    lds_barrier();  // this step's tile is there for every wave; every wave is done with the one before it
+    issue(s + BUF - 1);
+    const int8_t* tile = s_tile + (s % BUF) * (TM + TN) * BK;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      i32x4 x[MI], w[NI];
+      const int pos = ((2 * kk + hi) ^ ((row >> 2) & 3)) * 16;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<const i32x4*>(tile + (wm * MI * 32 + i * 32 + row) * BK + pos);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) w[j] = *reinterpret_cast<const i32x4*>(tile + (TM + wn * NI * 32 + j * 32 + row) * BK + pos);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], w[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  i8_wait<0>();  // no load is left in flight when the workgroup's LDS goes to another
+  const I8Out<T> out(a);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int n = n0 + wn * NI * 32 + j * 32 + row;
+    const bool in_n = n < a.N;
+    const float wsn = in_n ? out.ws[n] : 0.f, b = in_n && out.bias ? to_f32(out.bias[n]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int m = m0 + wm * MI * 32 + i * 32 + 8 * (e / 4) + 4 * hi + e % 4;
+        if (in_n && m < a.M) out.y[(size_t)m * a.N + n] = out.value(acc[i][j][e], a.a_scale[m], wsn, b);
+      }
+  }
+}
+
+template <typename T> static bool aligned16(const void* p, std::initializer_list<long long> strides) {
+  bool ok = ((uintptr_t)p & 15u) == 0;
+  for (long long s : strides) ok = ok && ((s * (long long)sizeof(T)) & 15) == 0;
+  return ok;
+}
+template <typename T, int W> static hipError_t codes_w(const RowCodesArgs& a, hipStream_t s) {
+  const bool fast = a.K % 8 == 0 && aligned16<T>(a.x, {a.xs});
+  if (fast) hipLaunchKernelGGL((row_codes_kernel<T, true, W>), dim3((unsigned)a.M), dim3(64 * W), 0, s, a);
+  else hipLaunchKernelGGL((row_codes_kernel<T, false, W>), dim3((unsigned)a.M), dim3(64 * W), 0, s, a);
+  return hipGetLastError();
+}
+hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s) {
+  const bool wide = a.K > 64 * 8 * I8_KEEP;
+  if (bf16_in) return wide ? codes_w<bf16, 4>(a, s) : codes_w<bf16, 1>(a, s);
+  return wide ? codes_w<float, 4>(a, s) : codes_w<float, 1>(a, s);
+}
+
+template <typename T, int TM, int TN, int WM, int WN> static hipError_t tile_t(const Int8LinearArgs& a, hipStream_t s) {
+  auto kern = int8_tile_kernel<T, TM, TN, WM, WN>;
+  const size_t lds = 4 * (TM + TN) * 64;
+  const hipError_t e = set_lds_limit((const void*)kern, lds);
+  if (e != hipSuccess) return e;
+  const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + TN - 1) / TN);
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * WM * WN), lds, s, a);
+  return hipGetLastError();
+}
+template <typename T, int MT> static hipError_t few_t(const Int8LinearArgs& a, hipStream_t s) {
+  const dim3 grid((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT));
+  hipLaunchKernelGGL((int8_few_kernel<T, MT>), grid, dim3(512), 0, s, a);
+  return hipGetLastError();
+}
+template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int form, hipStream_t s) {
+  switch (form) {
+    case 1: return few_t<T, 1>(a, s);
+    case 2: return few_t<T, 2>(a, s);
+    case 3: return few_t<T, 4>(a, s);
+    case 4: return tile_t<T, 64, 64, 2, 2>(a, s);
+    case 5: return tile_t<T, 128, 128, 2, 2>(a, s);
+    default: return tile_t<T, 256, 256, 2, 4>(a, s);
+  }
+}
+hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s) {
+  return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
+}
+
+}  // namespace dfl

@@ -1,0 +1,74 @@
+// Argument blocks of the operators of a layer served in few bits (rolling caches in 8 or 4 bits, products in 8-bit
+// integers), shared by the kernels and the C-ABI layer.  Semantics: include/dfl_lowbit.h.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "window_geometry.h"
+
+namespace dfl {
+
+struct LowbitCache {
+  uint8_t* codes;     // (B,Hk,S,row bytes), byte strides, multiples of 16
+  uint8_t* exps;      // (B,Hk,groups,S'), byte strides, multiples of 4
+  long long sb, sh, sn;
+  long long esb, esh, esg;
+};
+
+struct LowbitFillArgs {
+  const void* k;  // (B,Hk,N,d), element strides
+  const void* v;
+  long long ksb, ksh, ksn, vsb, vsh, vsn;
+  const int* lengths;  // (B) rows of each sample
+  const int* starts;   // (B) position of row 0, or null: 0
+  LowbitCache kc, vc;
+  int B, Hk, N, d, window, n_sink;
+};
+
+struct CacheReadArgs {
+  LowbitCache kc, vc;  // plain caches: codes are elements, strides in elements
+  const int* lengths;  // (B) positions that have entered
+  void* k;             // (B,Hk,S,d) contiguous
+  void* v;
+  float* mask;  // (B,S)
+  int B, Hk, d, window, n_sink;
+};
+
+struct LowbitDecodeArgs {
+  const void* q;  // (B,H,d), element strides
+  const void* k;  // (B,Hk,d)
+  const void* v;
+  long long qsb, qsh, ksb, ksh, vsb, vsh;
+  LowbitCache kc, vc;
+  const int* lengths;  // (B) position of the token; < 0: none
+  const float* table;
+  RelSpec rel;
+  int B, H, Hk, d, window, n_sink;
+  float scale;
+  void* o;      // (B,H,d) contiguous
+  float* part;  // [B*H][n_split][2 + DP]: reference, sum, output of a split (n_split > 1)
+  int n_split, chunk;  // slots of a split, a multiple of 32
+};
+
+struct RowCodesArgs {
+  const void* x;  // (M,K), element stride
+  long long xs;
+  int8_t* codes;  // (M, cs), zeros from K on; 16-byte aligned, cs a multiple of 16
+  long long cs;
+  float* scale;  // (M)
+  long long M;
+  int K;
+};
+
+struct Int8LinearArgs {
+  const int8_t* a;  // (M, as) codes of the tokens, zeros from K on; as a multiple of 64
+  const float* a_scale;
+  const int8_t* w;  // (N, ws) codes of the weights
+  const float* w_scale;
+  const void* bias;  // (N) or null
+  void* y;           // (M,N)
+  long long as, ws;
+  int M, K, N;
+};
+
+}  // namespace dfl

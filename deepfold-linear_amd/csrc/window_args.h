@@ -47,6 +47,7 @@ struct CacheFillArgs {
   const void* v;
   long long ksb, ksh, ksn, vsb, vsh, vsn;
   const int* lengths;  // (B) rows of each sample
+  const int* starts;   // (B) position of row 0, or null: 0
   void* kc;            // (B,Hk,n_sink + window,d), element strides
   void* vc;
   long long kcsb, kcsh, kcsn, vcsb, vcsh, vcsn;

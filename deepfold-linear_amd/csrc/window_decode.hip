@@ -23,14 +23,17 @@ template <typename T, bool FAST> __global__ void __launch_bounds__(256) cache_fi
   constexpr int VEC = 16 / (int)sizeof(T);
   const int nch = (a.d + VEC - 1) / VEC, S = a.n_sink + a.window;
   const int bh = blockIdx.y, b = bh / a.Hk, hk = bh % a.Hk;
-  const int last = max(min(a.lengths[b], a.N), 0) - 1;  // (a length of -2^31 has no predecessor)
+  const int n = min(a.lengths[b], a.N), start = a.starts ? a.starts[b] : 0;
+  if (n <= 0 || start < 0) return;
+  const unsigned last = (unsigned)start + (unsigned)n - 1;  // at most 2^31 + 2^28
   const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (slot, chunk)
   const int s = (int)(e / nch), c = (int)(e % nch);
-  if (s >= S) return;
-  const int p = slot_position(s, last, a.n_sink, a.window);
-  if (p < 0) return;
-  const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + (size_t)p * a.ksn + c * VEC;
-  const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + (size_t)p * a.vsn + c * VEC;
+  if (s >= S || (unsigned)s > last) return;
+  const unsigned p = s < a.n_sink ? s : s + (last - s) / a.window * a.window;  // latest position that the slot holds
+  if (p < (unsigned)start) return;
+  const size_t row = p - (unsigned)start;
+  const T* k = reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + row * a.ksn + c * VEC;
+  const T* v = reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + row * a.vsn + c * VEC;
   T* ko = reinterpret_cast<T*>(a.kc) + b * a.kcsb + hk * a.kcsh + (size_t)s * a.kcsn + c * VEC;
   T* vo = reinterpret_cast<T*>(a.vc) + b * a.vcsb + hk * a.vcsh + (size_t)s * a.vcsn + c * VEC;
   if (FAST) {

@@ -279,6 +279,75 @@ class RelBiasParams(ctypes.Structure):
     ]
 
 
+class LowbitCache(ctypes.Structure):
+    """Mirror of ``dfl_lowbit_cache``."""
+
+    _fields_ = [
+        ("codes", P), ("exponents", P),
+        ("stride_b", I64), ("stride_h", I64), ("stride_n", I64),
+        ("exp_stride_b", I64), ("exp_stride_h", I64), ("exp_stride_g", I64),
+    ]
+
+
+class LowbitCacheFillParams(ctypes.Structure):
+    """Mirror of ``dfl_lowbit_cache_fill_params``."""
+
+    _fields_ = [
+        ("dtype", I32), ("bits", I32),
+        ("k", P), ("v", P),
+        ("k_stride_b", I64), ("k_stride_h", I64), ("k_stride_n", I64),
+        ("v_stride_b", I64), ("v_stride_h", I64), ("v_stride_n", I64),
+        ("lengths", P), ("starts", P),
+        ("k_cache", LowbitCache), ("v_cache", LowbitCache),
+        ("B", I32), ("Hk", I32), ("N", I32), ("d", I32), ("window", I32), ("n_sink", I32),
+    ]
+
+
+class WindowCacheReadParams(ctypes.Structure):
+    """Mirror of ``dfl_window_cache_read_params``."""
+
+    _fields_ = [
+        ("dtype", I32), ("bits", I32),
+        ("k_cache", LowbitCache), ("v_cache", LowbitCache),
+        ("lengths", P), ("k", P), ("v", P), ("mask", P),
+        ("B", I32), ("Hk", I32), ("d", I32), ("window", I32), ("n_sink", I32),
+    ]
+
+
+class LowbitDecodeParams(ctypes.Structure):
+    """Mirror of ``dfl_lowbit_decode_params``."""
+
+    _fields_ = [
+        ("dtype", I32), ("bits", I32),
+        ("q", P), ("k", P), ("v", P),
+        ("q_stride_b", I64), ("q_stride_h", I64),
+        ("k_stride_b", I64), ("k_stride_h", I64),
+        ("v_stride_b", I64), ("v_stride_h", I64),
+        ("k_cache", LowbitCache), ("v_cache", LowbitCache),
+        ("lengths", P), ("rel_table", P), ("rel_edges", P), ("n_edges", I32),
+        ("B", I32), ("H", I32), ("Hk", I32), ("d", I32), ("window", I32), ("n_sink", I32), ("scale", F32),
+        ("o", P),
+    ]
+
+
+class QuantizeRowsParams(ctypes.Structure):
+    """Mirror of ``dfl_quantize_rows_params``."""
+
+    _fields_ = [
+        ("dtype", I32), ("x", P), ("x_stride", I64), ("M", I64), ("K", I32),
+        ("codes", P), ("code_stride", I64), ("scale", P),
+    ]
+
+
+class Int8LinearParams(ctypes.Structure):
+    """Mirror of ``dfl_int8_linear_params``."""
+
+    _fields_ = [
+        ("dtype", I32), ("x", P), ("x_stride", I64), ("w", P), ("w_stride", I64), ("w_scale", P), ("bias", P), ("y", P),
+        ("M", I32), ("K", I32), ("N", I32),
+    ]
+
+
 DFL_ATTN_BIAS_NONE = 0
 DFL_ATTN_BIAS_BINS = 1
 DFL_ATTN_BIAS_DENSE = 2
@@ -333,6 +402,14 @@ SIGNATURES = [
     ("dfl_rel_bias_workspace_size", ctypes.c_size_t, [I32] * 6),
     ("dfl_rel_bias_fwd", I32, [ctypes.POINTER(RelBiasParams), P]),
     ("dfl_rel_bias_bwd", I32, [ctypes.POINTER(RelBiasParams), P, ctypes.c_size_t, P]),
+    ("dfl_window_cache_append", I32, [ctypes.POINTER(WindowCacheFillParams), P, P]),
+    ("dfl_window_cache_read", I32, [ctypes.POINTER(WindowCacheReadParams), P]),
+    ("dfl_lowbit_cache_fill", I32, [ctypes.POINTER(LowbitCacheFillParams), P]),
+    ("dfl_lowbit_decode_workspace_size", ctypes.c_size_t, [I32] * 6),
+    ("dfl_lowbit_decode", I32, [ctypes.POINTER(LowbitDecodeParams), P, ctypes.c_size_t, P]),
+    ("dfl_quantize_rows", I32, [ctypes.POINTER(QuantizeRowsParams), P]),
+    ("dfl_int8_linear_workspace_size", ctypes.c_size_t, [I32] * 3),
+    ("dfl_int8_linear", I32, [ctypes.POINTER(Int8LinearParams), P, ctypes.c_size_t, P]),
 ]
 
 

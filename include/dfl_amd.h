@@ -35,6 +35,7 @@
 
 #include <stddef.h>
 
+#include "dfl_lowbit.h"
 #include "dfl_window.h"
 
 #ifdef __cplusplus
@@ -688,6 +689,21 @@ int dfl_window_decode(const dfl_window_decode_params* p, void* workspace, size_t
 size_t dfl_rel_bias_workspace_size(int B, int H, int M, int N, int n_edges, int rel_both);
 int dfl_rel_bias_fwd(const dfl_rel_bias_params* p, void* stream);
 int dfl_rel_bias_bwd(const dfl_rel_bias_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * A layer served in few bits: rolling caches in 8 or 4 bits, written, read back and attended to by one token,
+ * and products in 8-bit integers.  Parameter blocks and semantics in dfl_lowbit.h.  (The reference has no
+ * counterpart.)  Head dims up to 128; all may be captured into a graph, as those above.
+ */
+/* dfl_window_cache_fill for rows that stand at positions starts[b] + i; starts[b] < 0 leaves the sample's caches alone. */
+int dfl_window_cache_append(const dfl_window_cache_fill_params* p, const int* starts, void* stream);
+int dfl_window_cache_read(const dfl_window_cache_read_params* p, void* stream);
+int dfl_lowbit_cache_fill(const dfl_lowbit_cache_fill_params* p, void* stream);
+size_t dfl_lowbit_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink);
+int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t workspace_bytes, void* stream);
+int dfl_quantize_rows(const dfl_quantize_rows_params* p, void* stream);
+size_t dfl_int8_linear_workspace_size(int M, int K, int N);
+int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
