@@ -16,7 +16,7 @@ int capi_hip_fail(hipError_t e, const char* what);
 hipError_t launch_lowbit_fill(const LowbitFillArgs& a, bool bf16_in, int bits, hipStream_t s);
 hipError_t launch_cache_read(const CacheReadArgs& a, bool bf16_out, int bits, hipStream_t s);
 hipError_t launch_lowbit_decode(const LowbitDecodeArgs& a, bool bf16_in, int bits, int DP, hipStream_t s);
-int lowbit_decode_heads(bool bf16_in, int G);
+LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S);
 hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s);
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s);
 }  // namespace dfl
@@ -74,22 +74,19 @@ int check_codes(const dfl_lowbit_cache& c, int bits) {
     return fail("a cache's exponents and their strides must be multiples of 4 bytes");
   return 0;
 }
+// The decode's offsets: 32 rows of codes, and a head's exponents, within 2^31 bytes; rows behind each other.
+int check_near(const dfl_lowbit_cache& c, int bits, int d, int S) {
+  const int groups = (d + 31) / 32;
+  if (S > 1 && (c.stride_n < groups * 4 * bits || c.stride_n >= (1 << 26)))
+    return fail("a cache's row stride must hold a row and be below 2^26 bytes");
+  if (groups > 1 && (c.exp_stride_g < S || c.exp_stride_g > MAX_N + MAX_SINK + 64))
+    return fail("a cache's group stride must hold the slots and be at most %lld bytes", MAX_N + MAX_SINK + 64);
+  return 0;
+}
 dfl::LowbitCache cache(const dfl_lowbit_cache& c) {
   return {static_cast<uint8_t*>(c.codes), static_cast<uint8_t*>(c.exponents), c.stride_b, c.stride_h, c.stride_n,
           c.exp_stride_b, c.exp_stride_h, c.exp_stride_g};
 }
-
-// Splits of a cache, in blocks of the 32 slots that a wave takes at a time.
-constexpr int DECODE_WG = 768, DECODE_MIN = 128;
-struct Splits {
-  int n, chunk;
-  Splits(int B, int Hk, int S) {
-    const long long want = std::max<long long>(1, DECODE_WG / ((long long)B * Hk)), most = (S + DECODE_MIN - 1) / DECODE_MIN;
-    n = (int)std::min(want, most);
-    chunk = ((S + n - 1) / n + 31) / 32 * 32;
-    n = (S + chunk - 1) / chunk;
-  }
-};
 
 // Which kernel a product takes.
 int linear_form(int M, int K, int N) {
@@ -160,8 +157,9 @@ int dfl_window_cache_read(const dfl_window_cache_read_params* p, void* stream) {
 
 size_t dfl_lowbit_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink) {
   if (!heads_ok(B, H, Hk, d) || !window_ok(window, n_sink)) return 0;
-  const Splits s(B, Hk, window + n_sink);
-  return s.n > 1 ? r256((size_t)B * H * s.n * (pad_dim(d) + 2) * 4) : 0;
+  const int n = std::max(dfl::lowbit_decode_plan(true, B, H, Hk, d, window + n_sink).n_split,
+                         dfl::lowbit_decode_plan(false, B, H, Hk, d, window + n_sink).n_split);
+  return n > 1 ? r256((size_t)B * H * n * (pad_dim(d) + 2) * 4) : 0;
 }
 
 int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -170,6 +168,9 @@ int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t
     if (int rc = check_shape(p->dtype, p->B, p->H, p->Hk, p->d, p->window, p->n_sink)) return rc;
     if (int rc = check_codes(p->k_cache, p->bits)) return rc;
     if (int rc = check_codes(p->v_cache, p->bits)) return rc;
+    const int S = p->window + p->n_sink;
+    if (int rc = check_near(p->k_cache, p->bits, p->d, S)) return rc;
+    if (int rc = check_near(p->v_cache, p->bits, p->d, S)) return rc;
     if (!(p->scale >= 1e-30f && p->scale <= 1e30f)) return fail("scale=%g outside [1e-30, 1e30]", (double)p->scale);
     if (!p->q || !p->k || !p->v || !p->lengths || !p->o) return fail("required pointer is NULL");
     if (!p->rel_table != (p->n_edges == 0)) return fail("rel_table and rel_edges must be given together");
@@ -186,6 +187,7 @@ int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t
     a.qsb = p->q_stride_b; a.qsh = p->q_stride_h; a.ksb = p->k_stride_b; a.ksh = p->k_stride_h;
     a.vsb = p->v_stride_b; a.vsh = p->v_stride_h;
     a.kc = cache(p->k_cache); a.vc = cache(p->v_cache);
+    if (S == 1) a.kc.sn = a.vc.sn = (p->d + 31) / 32 * 4 * p->bits;  // (of one row, any stride)
     a.lengths = p->lengths;
     a.table = p->rel_table;
     a.rel.n = p->n_edges;
@@ -194,11 +196,12 @@ int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t
     a.scale = p->scale;
     a.o = p->o;
     a.part = static_cast<float*>(workspace);
-    const Splits s(p->B, p->Hk, p->window + p->n_sink);
-    a.n_split = s.n;
-    a.chunk = s.chunk;
-    const int G = p->H / p->Hk, heads = dfl::lowbit_decode_heads(p->dtype == DFL_BF16, G);
-    if ((long long)p->B * p->Hk * ((G + heads - 1) / heads) * s.n >= (1ll << 31)) return fail("too many rows");
+    const dfl::LowbitPlan plan = dfl::lowbit_decode_plan(p->dtype == DFL_BF16, p->B, p->H, p->Hk, p->d, S);
+    a.waves = plan.waves;
+    a.n_split = plan.n_split;
+    a.chunk = plan.chunk;
+    const int G = p->H / p->Hk;
+    if ((long long)p->B * p->Hk * ((G + plan.heads - 1) / plan.heads) * plan.n_split >= (1ll << 31)) return fail("too many rows");
     const hipError_t e = dfl::launch_lowbit_decode(a, p->dtype == DFL_BF16, p->bits, pad_dim(p->d), (hipStream_t)stream);
     return e == hipSuccess ? 0 : dfl::capi_hip_fail(e, "few-bit decode launch");
   });

@@ -47,7 +47,13 @@ struct LowbitDecodeArgs {
   float scale;
   void* o;      // (B,H,d) contiguous
   float* part;  // [B*H][n_split][2 + DP]: reference, sum, output of a split (n_split > 1)
+  int waves;           // of a workgroup
   int n_split, chunk;  // slots of a split, a multiple of 32
+};
+
+// How a decode is cut up: query heads and waves of a workgroup, splits of the cache and slots of one.
+struct LowbitPlan {
+  int heads, waves, n_split, chunk;
 };
 
 struct RowCodesArgs {

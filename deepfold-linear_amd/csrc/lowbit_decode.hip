@@ -3,18 +3,27 @@
 // Codes become bf16 operands of 16x16x32 matrix instructions in registers, exactly (a code has at most 7 bits, its scale
 // is a power of two), straight from the loads: no LDS between.  In vector instructions alone the products of four heads
 // would take longer than the codes take to arrive.  A wave takes 32 slots at a time:
-//   scores (slots x heads): A = 16 rows of keys, lane l the row l % 16 and a quarter l / 16 of its elements, as they
-//     lie in memory; B = the queries with the same elements.  Accumulator: lane = head l % 16, slots 4 (l / 16) + r.
-//   outputs (heads x columns): A = the weights, head l % 16, slots 4 (l / 16) + r of both halves: they stay in their lane;
-//     B = 16 columns of the values of these slots: lane l loads the elements l % 16 * DP / 16 .. of each of its slots.
+//   scores (slots x heads): A = 16 rows of keys, lane l one row and a quarter l / 16 of its elements, as they lie in
+//     memory; B = the queries with the same elements.  Rows are taken such that lane l of the accumulator has head l % 16
+//     and the slots 4 r + l / 16, r = 0 .. 3, of a half block.
+//   outputs (heads x columns): A = the weights, head l % 16, slots 4 r + l / 16 of both halves: they stay in their lane;
+//     B = 16 columns of the values of these slots: lane l loads the elements l % 16 * DP / 16 .. of each of its slots, so
+//     that a load of the wave has four neighbouring rows.
 // The 16 rows of the weights hold GP heads in TERMS parts: bf16 results take two bf16 numbers for a weight (16 bits of
 // it), fp32 results three (24 bits), so no weight is rounded to 8 bits and the matrix rows would be idle otherwise.  fp32
 // queries are three bf16 numbers, products of their own.  Sums, references and outputs are fp32.
+//
+// Bounds: the cache's bytes, and about 230 vector instructions a block of 4 bits.  32 sequences of 4100 slots, 32 / 8 heads,
+// d 128, 4 bits, 143 MB: 31 us, 4.6 TB/s of the 6.2 that a copy reaches (bf16 caches, 537 MB: 106 us).  One sequence of 131072
+// slots, the same heads, 8 bits, 276 MB: 48.5 us, 5.7 TB/s, and 4.6 us for joining the splits.  One sequence of 1028 slots,
+// 16 / 4 heads, d 64, 4 bits: 10.8 us, latency.  Registers: the keys' are free for the next block once the scores are
+// formed, the values' once the outputs are, so that one set lets three waves a SIMD run (two sets, two waves: 33.7 us); loads go
+// through buffer resources (with 64-bit addresses a lane and clamped rows 36 us).
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 #include "window_engine.h"
 
-#include <initializer_list>
+#include <algorithm>
 
 namespace dfl {
 
@@ -23,8 +32,13 @@ template <typename T> struct LbHeads {
   static constexpr int GP = 16 / TERMS;                 // heads of a tile
   static constexpr int QT = sizeof(T) == 2 ? 1 : 3;     // parts of a query
 };
+// Waves a SIMD that the registers let run without spilling, and so the largest workgroup: one a CU.
+constexpr int lb_waves(int size, int DP, int NT) {
+  return DP < 128 ? (NT == 2 ? 2 : 3) : NT == 2 ? (size == 4 ? 1 : 2) : (size == 4 ? 2 : 3);
+}
 // A reference is moved when a score passes it by more than this: weights stay below 2^8.
 constexpr float LB_LAZY = 8.f;
+constexpr long long CUS = 256;
 
 __device__ __forceinline__ int lb_position(int s, int last, int n_sink, int window) {
   return s < n_sink ? s : s + (last - s) / window * window;
@@ -42,13 +56,38 @@ template <int I> __device__ __forceinline__ unsigned fp4_pair(unsigned w, float 
 }
 template <int I> __device__ __forceinline__ float int8_at(unsigned w, float s) { return (float)(int8_t)(w >> (8 * I)) * s; }
 
+typedef __amdgpu_buffer_rsrc_t lb_rsrc;
+// `bytes` bytes from p on; loads behind them give zero.
+__device__ __forceinline__ lb_rsrc lb_buffer(const uint8_t* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000);
+}
+// N bytes at lane + row.  LB_ONCE: not kept in the caches (the values; 8 bits, one sequence of 131072 slots 54.7 -> 48.5 us,
+// with the keys too 50.9; 4 bits, 32 sequences of 4100 31.5 -> 31.0).
+constexpr int LB_ONCE = 2;
+template <int N, int AUX = 0, int W> __device__ __forceinline__ void lb_load(unsigned (&w)[W], lb_rsrc b, unsigned lane, unsigned row) {
+  static_assert(W == (N + 3) / 4, "whole dwords");
+  if constexpr (N == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(b, lane, row, AUX);
+  else if constexpr (N == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b16(b, lane, row, AUX);
+  else if constexpr (N == 4) w[0] = __builtin_amdgcn_raw_buffer_load_b32(b, lane, row, AUX);
+  else if constexpr (N == 8) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(b, lane, row, AUX);
+    w[0] = x[0], w[1] = x[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 16; ++i) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b128(b, lane + 16 * i, row, AUX);
+      w[4 * i] = x[0], w[4 * i + 1] = x[1], w[4 * i + 2] = x[2], w[4 * i + 3] = x[3];
+    }
+  }
+}
+
 union LbFrag {
   unsigned u[4];
   bf16x8 v;
 };
 
 template <typename T, int BITS, int DP, int NT, bool REL>
-__global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) {
+__global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(sizeof(T), DP, NT)) lowbit_decode_kernel(LowbitDecodeArgs a) {
   using Hd = LbHeads<T>;
   constexpr int GP = Hd::GP, QT = Hd::QT, GB = NT * GP;
   constexpr int KF = DP / 32;            // matrix instructions of a score tile; fragments of a lane's quarter row
@@ -57,13 +96,14 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
   constexpr int VB = NC * BITS / 8;      // bytes of them: 1, 2, 4 or 2, 4, 8
   constexpr int VW = (VB + 3) / 4;
   extern __shared__ __align__(16) unsigned char smem[];
-  float* s_ml = reinterpret_cast<float*>(smem);  // [4][GB][2]
-  float* s_o = s_ml + 4 * GB * 2;                // [4][GB][DP]
-  uint8_t* s_own = reinterpret_cast<uint8_t*>(s_o + 4 * GB * DP);  // [2][DP * BITS / 8] the token's own codes
+  const int waves = blockDim.x >> 6;
+  float* s_ml = reinterpret_cast<float*>(smem);  // [waves][GB][2]
+  float* s_o = s_ml + waves * GB * 2;            // [waves][GB][DP]
+  uint8_t* s_own = reinterpret_cast<uint8_t*>(s_o + waves * GB * DP);  // [2][DP * BITS / 8] the token's own codes
   uint8_t* s_exp = s_own + 2 * DP * BITS / 8;                      // [2][4]
   float* s_tab = reinterpret_cast<float*>(s_exp + 8);              // [GB][buckets]
   uint8_t* s_lut = reinterpret_cast<uint8_t*>(s_tab + (REL ? GB * a.rel.buckets() : 0));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, h = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, h = lane >> 4;
   const int G = a.H / a.Hk, nhg = (G + GB - 1) / GB;
   int x = blockIdx.x;
   const int sp = x % a.n_split;
@@ -81,6 +121,44 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
   const uint8_t* vc = a.vc.codes + b * a.vc.sb + hk * a.vc.sh;
   const uint8_t* ke = a.kc.exps + b * a.kc.esb + hk * a.kc.esh;
   const uint8_t* ve = a.vc.exps + b * a.vc.esb + hk * a.vc.esh;
+
+  const int kg = DP / 4 * h / 32, vg = n * NC / 32;   // groups of the lane's key and value elements
+  const bool kin = kg < groups, vin = vg < groups;    // (96 of 128 elements: the last quarter has none)
+  const int kge = min(kg, groups - 1), vge = min(vg, groups - 1);
+  struct Raw {
+    unsigned k[2][KW], v[8][VW];
+    unsigned ke[2], ve[2][4];
+  };
+  // Loads through buffer resources: what the block and the row have in an address is scalar, a lane adds one register, and
+  // what lies behind the last slot in use (or beside the row: 96 of 128 elements) is not read and counts as zero.
+  constexpr unsigned NOWHERE = 0xfffff000u;
+  const int kofs = h * (KW * 4), vofs = n * VB, ksn = (int)a.kc.sn, vsn = (int)a.vc.sn;
+  const int kn = 4 * (n & 3) + (n >> 2);  // the slot of a half block that the lane's row of keys is
+  const unsigned kat = kin ? kn * ksn + kofs : NOWHERE, vat = vin ? h * vsn + vofs : NOWHERE;
+  const unsigned keat = kge * (unsigned)a.kc.esg + kn, veat = vge * (unsigned)a.vc.esg;
+  const int S4 = (S + 3) & ~3;  // (a dword of exponents may reach behind the last slot)
+  const auto kexp = lb_buffer(ke, (groups - 1) * (int)a.kc.esg + S4), vexp = lb_buffer(ve, (groups - 1) * (int)a.vc.esg + S4);
+  Raw r;
+  auto load_keys = [&](int s0) {
+    const auto kb = lb_buffer(kc + s0 * a.kc.sn, min(32, end - s0) * ksn);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      lb_load<KW * 4>(r.k[u], kb, kat, 16 * u * ksn);
+      r.ke[u] = __builtin_amdgcn_raw_buffer_load_b8(kexp, keat, s0 + 16 * u, 0);
+    }
+  };
+  auto load_values = [&](int s0) {
+    const auto vb = lb_buffer(vc + s0 * a.vc.sn, min(32, end - s0) * vsn);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      lb_load<16>(r.ve[u], vexp, veat, s0 + 16 * u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lb_load<VB, LB_ONCE>(r.v[4 * u + j], vb, vat, (16 * u + 4 * j) * vsn);
+    }
+  };
+  // the first block is on its way while the token and the queries are prepared
+  const int first = begin + 32 * wave, stride = 32 * waves;
+  if (first < end) load_keys(first), load_values(first);
 
   // The token's own codes: from the call's rows into LDS, and into the cache by one workgroup.
   if (mine && wave < 2 && lane < nch) {
@@ -104,8 +182,8 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
   }
   if (REL) {
     const int nb = a.rel.buckets(), dist = a.rel.dist();
-    for (int e = threadIdx.x; e < gn * nb; e += 256) s_tab[e] = a.table[(size_t)h0 * nb + e] * LOG2E;
-    for (int e = threadIdx.x; e <= dist; e += 256) s_lut[e] = (uint8_t)rel_bucket(a.rel, -e);
+    for (int e = threadIdx.x; e < gn * nb; e += blockDim.x) s_tab[e] = a.table[(size_t)h0 * nb + e] * LOG2E;
+    for (int e = threadIdx.x; e <= dist; e += blockDim.x) s_lut[e] = (uint8_t)rel_bucket(a.rel, -e);
   }
   // The queries: lane's column n is head n % GP of a tile, elements DP / 4 * h .. of it.  They take the scale's power of
   // two, which changes none of their digits; the scores take the rest of it, a factor from 1 to 2.
@@ -135,12 +213,9 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
 
   const int term = n / GP;
   const float sel1 = term >= 1 ? -1.f : 0.f, sel2 = term >= 2 ? -1.f : 0.f;
-  const int kg = DP / 4 * h / 32, vg = n * NC / 32;   // groups of the lane's key and value elements
-  const bool kin = kg < groups, vin = vg < groups;    // (96 of 128 elements: the last quarter has none)
-  const int kge = min(kg, groups - 1), vge = min(vg, groups - 1);
   f32x4 o[NT][NC];
   float m[NT], l[NT];
-  unsigned bad = 0;
+  unsigned top = 0;  // the highest exponent in use
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     m[i] = NEG_BIG, l[i] = 0.f;
@@ -148,40 +223,13 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
     for (int c = 0; c < NC; ++c) o[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Raw {
-    unsigned k[2][KW], v[8][VW];
-    unsigned ke[2], ve[2];
-  };
-  const int kofs = h * (KW * 4), vofs = n * VB;
-  auto load = [&](Raw& r, int s0) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int s = min(s0 + 16 * u + n, end - 1);
-      const unsigned* at = reinterpret_cast<const unsigned*>(kc + s * a.kc.sn + (kin ? kofs : 0));
-#pragma unroll
-      for (int i = 0; i < KW; ++i) r.k[u][i] = at[i];
-      r.ke[u] = ke[kge * a.kc.esg + s];
-      // four slots' bytes; the last dword of a group where these would lie behind it (they are masked then)
-      const int s4 = min(s0 + 16 * u + 4 * h, (S - 1) & ~3);
-      r.ve[u] = *reinterpret_cast<const unsigned*>(ve + vge * a.vc.esg + s4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int sv = min(s0 + 16 * u + 4 * h + j, end - 1);
-        const uint8_t* p = vc + sv * a.vc.sn + (vin ? vofs : 0);
-        if constexpr (VB == 1) r.v[4 * u + j][0] = *p;
-        else if constexpr (VB == 2) r.v[4 * u + j][0] = *reinterpret_cast<const unsigned short*>(p);
-        else
-#pragma unroll
-          for (int i = 0; i < VW; ++i) r.v[4 * u + j][i] = reinterpret_cast<const unsigned*>(p)[i];
-      }
-    }
-  };
-  auto step = [&](Raw& r, int s0) {
+  f32x4 none[2] = {};  // what the scores of a block start from
+  auto step = [&](int s0) {
     if (mine && s0 <= own && own < s0 + 32) {  // the token's own slot, as its codes stand
       const int at = own - s0;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (16 * u + n == at) {
+        if (16 * u + kn == at) {
           const unsigned* p = reinterpret_cast<const unsigned*>(s_own + (kin ? kofs : 0));
 #pragma unroll
           for (int i = 0; i < KW; ++i) r.k[u][i] = p[i];
@@ -189,34 +237,37 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (16 * u + 4 * h + j == at) {
+          if (16 * u + 4 * j + h == at) {
             const uint8_t* p = s_own + DP * BITS / 8 + (vin ? vofs : 0);
             if constexpr (VB == 1) r.v[4 * u + j][0] = *p;
             else if constexpr (VB == 2) r.v[4 * u + j][0] = *reinterpret_cast<const unsigned short*>(p);
             else
 #pragma unroll
               for (int i = 0; i < VW; ++i) r.v[4 * u + j][i] = reinterpret_cast<const unsigned*>(p)[i];
-            r.ve[u] = (r.ve[u] & ~(255u << (8 * j))) | (unsigned)s_exp[4 + vge] << (8 * j);
+            r.ve[u][j] = (unsigned)s_exp[4 + vge] << (8 * h);
           }
       }
     }
-    const bool whole = s0 + 32 <= end;
-    if (!whole) {  // slots that are not in use: their exponents are not looked at
+    if (s0 + 32 > end) {  // the wave's last block: slots that are not in use score -inf, their exponents are not looked at
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (s0 + 16 * u + n >= end) r.ke[u] = 0;
-        const int left = end - (s0 + 16 * u + 4 * h);
-        if (left < 4) r.ve[u] = left <= 0 ? 0u : r.ve[u] & ((1u << (8 * left)) - 1);
+        if (s0 + 16 * u + kn >= end) r.ke[u] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = s0 + 16 * u + 4 * j + h < end;
+          none[u][j] = in ? 0.f : -INFINITY;
+          if (!in) r.ve[u][j] = 0;
+        }
       }
     }
     // scores
     f32x4 y[2][NT];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float ks = kin ? lb_scale(r.ke[u]) : 0.f;
-      bad |= kin ? (r.ke[u] + 1) & 256u : 0u;
+      const float ks = lb_scale(r.ke[u]);
+      top = max(top, r.ke[u]);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) y[u][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NT; ++i) y[u][i] = none[u];
 #pragma unroll
       for (int f = 0; f < KF; ++f) {
         LbFrag k;
@@ -235,6 +286,7 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
             y[u][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.v, q[i][p][f].v, y[u][i], 0, 0, 0);
       }
     }
+    if (s0 + stride < end) load_keys(s0 + stride);
     // weights
     LbFrag w[NT];
 #pragma unroll
@@ -244,13 +296,11 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int s = s0 + 16 * u + 4 * h + j;
           float v = y[u][i][j] * sc;
           if (REL) {
-            const int bk = s_lut[min(t - lb_position(min(s, end - 1), t, a.n_sink, a.window), a.rel.dist())];
+            const int bk = s_lut[min(t - lb_position(min(s0 + 16 * u + 4 * j + h, end - 1), t, a.n_sink, a.window), a.rel.dist())];
             v += s_tab[min(i * GP + n % GP, gn - 1) * a.rel.buckets() + bk];
           }
-          if (!whole) v = s < end ? v : -INFINITY;
           y[u][i][j] = v;
           mx = fmaxf(mx, v);
         }
@@ -290,10 +340,12 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
     float vs[8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const unsigned e = vin ? r.ve[u] : 0u;
-      bad |= (((e & 0x7f7f7f7fu) + 0x01010101u) & e) & 0x80808080u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vs[4 * u + j] = lb_scale((e >> (8 * j)) & 255u);
+      for (int j = 0; j < 4; ++j) {
+        const unsigned e = __builtin_amdgcn_ubfe(r.ve[u][j], 8 * h, 8);
+        top = max(top, e);
+        vs[4 * u + j] = lb_scale(e);
+      }
     }
     auto column = [&](int c, const LbFrag& v) {
 #pragma unroll
@@ -333,21 +385,15 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
     }
   };
   {
-    int s0 = begin + 32 * wave;
-    if (s0 < end) {
-      Raw now, next;
-      load(now, s0);
-      for (; s0 + 128 < end; s0 += 128) {
-        load(next, s0 + 128);
-        step(now, s0);
-        now = next;
-      }
-      step(now, s0);
+    // the next block's keys are loaded once this one's are used, its values likewise
+    for (int s0 = first; s0 < end; s0 += stride) {
+      step(s0);
+      if (s0 + stride < end) load_values(s0 + stride);
     }
   }
 
   // The waves' parts: weights' parts and lanes joined, then the waves in LDS.
-  const bool poison = __any(bad != 0);
+  const bool poison = __any(top == LB_NAN);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     float sum = sum_groups(l[i]);
@@ -367,18 +413,20 @@ __global__ void __launch_bounds__(256) lowbit_decode_kernel(LowbitDecodeArgs a) 
       }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < gn * DP; e += 256) {
+  for (int e = threadIdx.x; e < gn * DP; e += blockDim.x) {
     const int g = e / DP, col = e % DP;
     float mx = NEG_BIG;
+    for (int r = 0; r < waves; r += 4)  // (a multiple of 4)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s_ml[(r * GB + g) * 2]);
+      for (int k = 0; k < 4; ++k) mx = fmaxf(mx, s_ml[((r + k) * GB + g) * 2]);
     float sl = 0.f, so = 0.f;
+    for (int r = 0; r < waves; r += 4)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float al = fast_exp2(s_ml[(r * GB + g) * 2] - mx);
-      sl = __builtin_fmaf(s_ml[(r * GB + g) * 2 + 1], al, sl);
-      so = __builtin_fmaf(s_o[(r * GB + g) * DP + col], al, so);
-    }
+      for (int k = 0; k < 4; ++k) {
+        const float al = fast_exp2(s_ml[((r + k) * GB + g) * 2] - mx);
+        sl = __builtin_fmaf(s_ml[((r + k) * GB + g) * 2 + 1], al, sl);
+        so = __builtin_fmaf(s_o[((r + k) * GB + g) * DP + col], al, so);
+      }
     const size_t head = (size_t)b * a.H + h0 + g;
     if (a.n_split == 1) {
       if (col < a.d) reinterpret_cast<T*>(a.o)[head * a.d + col] = from_f32<T>(sl == 0.f ? 0.f : so / sl);
@@ -429,12 +477,12 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) lowbit_join
 template <typename T, int BITS, int DP, int NT, bool REL> static hipError_t decode_l(const LowbitDecodeArgs& a, hipStream_t s) {
   constexpr int GB = NT * LbHeads<T>::GP;
   const int G = a.H / a.Hk, nhg = (G + GB - 1) / GB;
-  const size_t lds = (size_t)4 * GB * (DP + 2) * 4 + 2 * DP * BITS / 8 + 8 +
+  const size_t lds = (size_t)a.waves * GB * (DP + 2) * 4 + 2 * DP * BITS / 8 + 8 +
                      (REL ? (size_t)GB * a.rel.buckets() * 4 + a.rel.dist() + 1 : 0);
   auto kern = lowbit_decode_kernel<T, BITS, DP, NT, REL>;
   hipError_t e = set_lds_limit((const void*)kern, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(a.B * a.Hk * nhg * a.n_split)), dim3(256), lds, s, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.B * a.Hk * nhg * a.n_split)), dim3(64 * a.waves), lds, s, a);
   if ((e = hipGetLastError()) != hipSuccess || a.n_split == 1) return e;
   hipLaunchKernelGGL((lowbit_join_kernel<T, DP>), dim3((unsigned)(a.B * a.H)), dim3(128), a.n_split * 4, s, a);
   return hipGetLastError();
@@ -451,9 +499,33 @@ hipError_t launch_lowbit_decode(const LowbitDecodeArgs& a, bool bf16_in, int bit
   if (bf16_in) return bits == 4 ? decode_b<bf16, 4>(a, DP, s) : decode_b<bf16, 8>(a, DP, s);
   return bits == 4 ? decode_b<float, 4>(a, DP, s) : decode_b<float, 8>(a, DP, s);
 }
-int lowbit_decode_heads(bool bf16_in, int G) {
-  const int gp = bf16_in ? LbHeads<bf16>::GP : LbHeads<float>::GP;
-  return G > gp ? 2 * gp : gp;
+
+// How a call is cut up.  A workgroup of 4 lb_waves waves has a CU to itself; smaller ones share it.
+//  * Caches of up to four blocks of 32 slots a wave of such a workgroup: one workgroup for all of it, whose one launch
+//    is shorter than two.
+//  * As many of these workgroups as CUs, or nearly: no split either, or as many splits as make that many.
+//  * Else workgroups of 4 waves, which fill the CUs in any number.
+LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S) {
+  const int DP = d <= 32 ? 32 : d <= 64 ? 64 : 128, G = H / Hk, gp = bf16_in ? LbHeads<bf16>::GP : LbHeads<float>::GP;
+  const int NT = G > gp ? 2 : 1, per = lb_waves(bf16_in ? 2 : 4, DP, NT), big = 4 * per, blocks = (S + 31) / 32;
+  LowbitPlan p;
+  p.heads = NT * gp;
+  const long long wg = (long long)B * Hk * ((G + p.heads - 1) / p.heads), rounds = (wg + CUS - 1) / CUS;
+  long long n = 1;
+  p.waves = big;
+  if (blocks <= 4 * big) {
+    p.waves = std::min(big, (blocks + 3) / 4 * 4);
+  } else if (wg * 5 < rounds * CUS * 4) {
+    n = CUS / wg;
+    if (n * wg * 5 < CUS * 4) {
+      p.waves = 4;
+      n = std::max(1ll, CUS * per / wg);
+    }
+    n = std::min<long long>(n, (blocks + p.waves - 1) / p.waves);
+  }
+  p.chunk = (int)((blocks + n - 1) / n) * 32;
+  p.n_split = (S + p.chunk - 1) / p.chunk;
+  return p;
 }
 
 }  // namespace dfl

@@ -42,7 +42,7 @@ def test_struct_layout_matches_c(tmp_path):
 
 def codes(**kw):
     return _lib.LowbitCache(**{**dict(codes=FAKE, exponents=FAKE, stride_b=256, stride_h=128, stride_n=64, exp_stride_b=64,
-                                      exp_stride_h=64, exp_stride_g=16), **kw})
+                                      exp_stride_h=64, exp_stride_g=8192), **kw})
 
 
 def fill_params(**kw):
@@ -83,7 +83,9 @@ CODES = [dict(bits=5), dict(bits=16), dict(k_cache=codes(codes=None)), dict(v_ca
                                            dict(bits=0, v_cache=codes(codes=None)), dict(bits=1)]),
     ("decode", decode_params, SHAPE + CODES + [dict(H=3), dict(H=0), dict(scale=0.0), dict(scale=float("nan")), dict(q=None), dict(o=None),
                                                dict(rel_table=FAKE), dict(n_edges=2), dict(n_edges=96, rel_table=FAKE, rel_edges=FAKE),
-                                               dict(n_edges=-1, rel_table=FAKE), dict(B=2**30, H=2**30, Hk=2**30)]),
+                                               dict(n_edges=-1, rel_table=FAKE), dict(B=2**30, H=2**30, Hk=2**30),
+                                               dict(k_cache=codes(stride_n=16)), dict(v_cache=codes(stride_n=1 << 26)),
+                                               dict(k_cache=codes(exp_stride_g=4096)), dict(v_cache=codes(exp_stride_g=1 << 30))]),
     ("rows", rows_params, [dict(dtype=2), dict(M=0), dict(M=2**31), dict(K=0), dict(K=2**17 + 1), dict(x=None), dict(codes=None),
                            dict(scale=None), dict(code_stride=48), dict(code_stride=72), dict(codes=FAKE + 4)]),
     ("linear", linear_params, [dict(dtype=2), dict(M=0), dict(K=0), dict(N=0), dict(M=-1), dict(K=2**17 + 1, w_stride=2**18), dict(x=None),
