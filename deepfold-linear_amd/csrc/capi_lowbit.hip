@@ -65,13 +65,16 @@ int check_shape(int dtype, int B, int H, int Hk, int d, int window, int n_sink) 
   if (n_sink < 0 || n_sink > MAX_SINK) return fail("n_sink=%d outside [0, %d]", n_sink, MAX_SINK);
   return 0;
 }
-int check_codes(const dfl_lowbit_cache& c, int bits) {
+// (Strides of dimensions of one element are not looked at.)
+int check_codes(const dfl_lowbit_cache& c, int bits, int B, int Hk, int S, int d) {
   if (bits != 4 && bits != 8) return fail("bits must be 4 or 8");
   if (!c.codes || !c.exponents) return fail("required pointer is NULL");
-  if (((uintptr_t)c.codes | (uintptr_t)c.stride_b | (uintptr_t)c.stride_h | (uintptr_t)c.stride_n) & 15)
-    return fail("a cache's codes and their strides must be multiples of 16 bytes");
-  if (((uintptr_t)c.exponents | (uintptr_t)c.exp_stride_b | (uintptr_t)c.exp_stride_h | (uintptr_t)c.exp_stride_g) & 3)
-    return fail("a cache's exponents and their strides must be multiples of 4 bytes");
+  const uintptr_t codes = (uintptr_t)c.codes | (uintptr_t)(B > 1 ? c.stride_b : 0) | (uintptr_t)(Hk > 1 ? c.stride_h : 0) |
+                          (uintptr_t)(S > 1 ? c.stride_n : 0);
+  const uintptr_t exps = (uintptr_t)c.exponents | (uintptr_t)(B > 1 ? c.exp_stride_b : 0) |
+                         (uintptr_t)(Hk > 1 ? c.exp_stride_h : 0) | (uintptr_t)(d > 32 ? c.exp_stride_g : 0);
+  if (codes & 15) return fail("a cache's codes and their strides must be multiples of 16 bytes");
+  if (exps & 3) return fail("a cache's exponents and their strides must be multiples of 4 bytes");
   return 0;
 }
 // The decode's offsets: 32 rows of codes, and a head's exponents, within 2^31 bytes; rows behind each other.
@@ -117,8 +120,8 @@ int dfl_lowbit_cache_fill(const dfl_lowbit_cache_fill_params* p, void* stream) {
   return guarded([&] {
     if (!p) return fail("params is NULL");
     if (int rc = check_shape(p->dtype, p->B, p->Hk, p->Hk, p->d, p->window, p->n_sink)) return rc;
-    if (int rc = check_codes(p->k_cache, p->bits)) return rc;
-    if (int rc = check_codes(p->v_cache, p->bits)) return rc;
+    if (int rc = check_codes(p->k_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
+    if (int rc = check_codes(p->v_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
     if (p->N <= 0 || p->N > MAX_N) return fail("N must be in [1, %lld]", MAX_N);
     if ((long long)p->B * p->Hk > 65535) return fail("B * Hk = %lld > 65535", (long long)p->B * p->Hk);
     if (!p->k || !p->v || !p->lengths) return fail("required pointer is NULL");
@@ -139,8 +142,8 @@ int dfl_window_cache_read(const dfl_window_cache_read_params* p, void* stream) {
     if (!p) return fail("params is NULL");
     if (int rc = check_shape(p->dtype, p->B, p->Hk, p->Hk, p->d, p->window, p->n_sink)) return rc;
     if (p->bits) {
-      if (int rc = check_codes(p->k_cache, p->bits)) return rc;
-      if (int rc = check_codes(p->v_cache, p->bits)) return rc;
+      if (int rc = check_codes(p->k_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
+      if (int rc = check_codes(p->v_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
     }
     if ((long long)p->B * p->Hk > 65535) return fail("B * Hk = %lld > 65535", (long long)p->B * p->Hk);
     if (!p->k_cache.codes || !p->v_cache.codes || !p->lengths || !p->k || !p->v || !p->mask)
@@ -166,8 +169,8 @@ int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t
   return guarded([&] {
     if (!p) return fail("params is NULL");
     if (int rc = check_shape(p->dtype, p->B, p->H, p->Hk, p->d, p->window, p->n_sink)) return rc;
-    if (int rc = check_codes(p->k_cache, p->bits)) return rc;
-    if (int rc = check_codes(p->v_cache, p->bits)) return rc;
+    if (int rc = check_codes(p->k_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
+    if (int rc = check_codes(p->v_cache, p->bits, p->B, p->Hk, p->window + p->n_sink, p->d)) return rc;
     const int S = p->window + p->n_sink;
     if (int rc = check_near(p->k_cache, p->bits, p->d, S)) return rc;
     if (int rc = check_near(p->v_cache, p->bits, p->d, S)) return rc;

@@ -35,7 +35,7 @@ def _no_grad(what, *tensors):
 
 def _quantize(x):
     M, K = x.shape
-    dev, xc = x.device, _unit_inner(x.detach())
+    dev, xc = x.device, _unit_inner(x)
     stride = -(-K // 16) * 16
     codes = torch.empty(M, stride, dtype=torch.int8, device=dev)
     scale = torch.empty(M, dtype=torch.float32, device=dev)
@@ -52,14 +52,11 @@ def _quantize(x):
 def _linear(x, codes, scale, bias):
     N, K = codes.shape
     dev = x.device
-    xc = x.detach()
-    if xc.dim() != 2:
-        xc = xc.reshape(-1, K)
-    xc = _unit_inner(xc)
+    xc = _unit_inner(x if x.dim() == 2 else x.reshape(-1, K))
     M = xc.shape[0]
     y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
-    b = None if bias is None else bias.detach().to(x.dtype).contiguous()
-    scale = scale.detach().contiguous()
+    b = None if bias is None else bias.to(x.dtype).contiguous()
+    scale = scale.contiguous()
     p = _lib.Int8LinearParams(_dtype_code("int8_linear", x), xc.data_ptr(), xc.stride(0), codes.data_ptr(), codes.stride(0),
                               scale.data_ptr(), _lib.ptr(b), y.data_ptr(), M, K, N)
     lib = _lib.load()

@@ -253,27 +253,40 @@ def _check_codes(what, k_cache, v_cache, B, Hk, d, n_sink):
     if bits not in (4, 8) or v_cache.bits != bits:
         raise ValueError(f"{what}: k_cache and v_cache must both hold 8 or both 4 bits, got {bits} and {v_cache.bits}")
     slots = k_cache.codes.shape[2] if k_cache.codes.dim() == 4 else 0
+    shape, exp_shape = (B, Hk, slots, groups * 4 * bits), (B, Hk, groups)
     for codes, exps, _ in (k_cache, v_cache):
         if codes.dtype != torch.uint8 or exps.dtype != torch.uint8:
             raise TypeError(f"{what}: a quantized cache's codes and exponents must be uint8")
-        if codes.shape != (B, Hk, slots, groups * 4 * bits) or exps.dim() != 4 or exps.shape[:3] != (B, Hk, groups):
-            raise ValueError(f"{what}: quantized cache {tuple(codes.shape)}, {tuple(exps.shape)} does not fit "
+        es = exps.shape
+        if codes.shape != shape or len(es) != 4 or es[:3] != exp_shape:
+            raise ValueError(f"{what}: quantized cache {tuple(codes.shape)}, {tuple(es)} does not fit "
                              f"({B}, {Hk}, *, {d}) in {bits} bits")
-        if exps.shape[3] < slots or exps.shape[3] % 4:
-            raise ValueError(f"{what}: {exps.shape[3]} exponents a group for {slots} slots: need a multiple of 4, as many at least")
-        for t, inner, unit in ((codes, codes.shape[3], 16), (exps, exps.shape[3], 4)):
+        if es[3] < slots or es[3] % 4:
+            raise ValueError(f"{what}: {es[3]} exponents a group for {slots} slots: need a multiple of 4, as many at least")
+        for t, unit in ((codes, 16), (exps, 4)):
             at = t.data_ptr()
-            if at % unit or not t.is_contiguous() and (
-                    t.stride(3) != 1 or any(s % unit for s, n in zip(t.stride(), t.shape[:3]) if n > 1)):
+            if t.is_contiguous():
+                size, fine = t.numel(), True
+            else:
+                fine = t.stride(3) == 1 and all(s % unit == 0 for s, n in zip(t.stride(), t.shape[:3]) if n > 1)
+                size = _extent(what, t, t.shape[3])
+            if at % unit or not fine:
                 raise ValueError(f"{what}: a quantized cache's rows must be contiguous, {unit}-byte aligned")
-            regions.append((at, at + _extent(what, t, inner), t))
-    for i, (a0, a1, s) in enumerate(regions):
-        for b0, b1, t in regions[i + 1:]:
-            if a0 < b1 and b0 < a1 and (s.shape != t.shape or s.stride() != t.stride() or _meet(s.shape, s.stride(), b0 - a0)):
-                raise ValueError(f"{what}: codes or exponents of the caches share memory")
+            regions.append((at, at + size, t))
+    regions.sort(key=_address)
+    if regions[0][1] > regions[1][0] or regions[1][1] > regions[2][0] or regions[2][1] > regions[3][0]:
+        for i, (a0, a1, s) in enumerate(regions):
+            for b0, b1, t in regions[i + 1:]:
+                if a0 < b1 and b0 < a1 and (s.shape != t.shape or s.stride() != t.stride() or
+                                            _meet(s.shape, s.stride(), b0 - a0)):
+                    raise ValueError(f"{what}: codes or exponents of the caches share memory")
     window = slots - n_sink
     _check_window(what, window, n_sink)
     return window
+
+
+def _address(region):
+    return region[0]
 
 
 def _same_kind(what, k_cache, v_cache):
@@ -299,8 +312,7 @@ def _no_grad_inputs(what, *tensors):
 
 
 def _codes_of(codes, exps):
-    unused = lambda t: [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]  # noqa: E731
-    return _lib.LowbitCache(codes.data_ptr(), exps.data_ptr(), *unused(codes), *unused(exps))
+    return _lib.LowbitCache(codes.data_ptr(), exps.data_ptr(), *codes.stride()[:3], *exps.stride()[:3])
 
 
 def _dtype_of(t):
@@ -332,7 +344,7 @@ def _fill_codes(K, V, lengths, starts, kc, ke, vc, ve, bits, n_sink):
     B, Hk, N, d = K.shape
     dev, at = K.device, _lengths(lengths)
     start = None if starts is None else _lengths(starts)
-    k, v = _unit_inner(K.detach()), _unit_inner(V.detach())
+    k, v = _unit_inner(K), _unit_inner(V)
     p = _lib.LowbitCacheFillParams(
         _dtype_of(K), bits, k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], at.data_ptr(), _lib.ptr(start),
         _codes_of(kc, ke), _codes_of(vc, ve), B, Hk, N, d, kc.shape[2] - n_sink, n_sink)
@@ -368,7 +380,7 @@ def _decode_codes(q, k, v, kc, ke, vc, ve, lengths, rel_table, arr, bits, n_sink
     Hk, window = k.shape[1], kc.shape[2] - n_sink
     dev, at = q.device, _lengths(lengths)
     tab = None if rel_table is None else rel_table.detach().to(torch.float32).contiguous()
-    q, k, v = _unit_inner(q.detach()), _unit_inner(k.detach()), _unit_inner(v.detach())
+    q, k, v = _unit_inner(q), _unit_inner(k), _unit_inner(v)
     o = torch.empty(B, H, d, dtype=q.dtype, device=dev)
     lib = _lib.load()
     nbytes = lib.dfl_lowbit_decode_workspace_size(B, H, Hk, d, window, n_sink)
