@@ -102,7 +102,7 @@ int linear_form(int M, int K, int N) {
   if (tiles(128) >= 256) return 5;
   return 4;
 }
-size_t code_row(int K) { return ((size_t)K + 63) / 64 * 64; }
+size_t code_row(int K) { return ((size_t)K + 127) / 128 * 128; }
 bool linear_ok(int M, int K, int N) { return M > 0 && K > 0 && N > 0 && K <= MAX_K; }
 struct LinearWs {
   size_t scale, total;

@@ -151,15 +151,18 @@ template <int N> __device__ __forceinline__ void i8_wait() {
   asm volatile("" ::: "memory");
 }
 
-// Tiles of TM tokens and TN rows of weights, WM x WN waves of 32 x 32 blocks.  K goes by in steps of 64 bytes through
-// four LDS buffers, loaded three steps ahead without passing through registers; a 64-byte row's 16-byte chunk c lies at
-// position c ^ (row / 4 % 4), so that 16 lanes reading the same chunk of 16 rows meet every bank once.
+// Tiles of TM tokens and TN rows of weights, WM x WN waves of 32 x 32 blocks.  K goes by in steps of 128 bytes, whole lines
+// of memory, through two LDS buffers that are loaded without passing through registers; a row's 16-byte chunk c lies
+// at position c ^ (row / 2 % 8), so that 16 lanes reading the same chunk of 16 rows meet every bank once.  The weights are
+// the instructions' first operand: a lane of the accumulators has one token and runs of four rows of weights, and the results
+// leave through LDS in whole lines.
 template <typename T, int TM, int TN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs a) {
-  constexpr int NT = 64 * WM * WN, BUF = 4, BK = 64, MI = TM / WM / 32, NI = TN / WN / 32;
-  constexpr int CHUNKS = (TM + TN) * 4, PER = CHUNKS / NT, STEP = NT / 4;  // rows between a thread's chunks
+  constexpr int NT = 64 * WM * WN, BK = 128, SUB = BK / 32, MI = TM / WM / 32, NI = TN / WN / 32;
+  constexpr int CHUNKS = (TM + TN) * 8, PER = CHUNKS / NT, STEP = NT / 8;  // rows between a thread's chunks
+  constexpr int TILE = (TM + TN) * BK;
   static_assert(CHUNKS % NT == 0 && STEP % 16 == 0 && TM % STEP == 0, "whole loads of one swizzle");
-  extern __shared__ __align__(16) int8_t s_tile[];  // [BUF][TM + TN][64]
+  extern __shared__ __align__(16) int8_t s_tile[];  // [2][TM + TN][128]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // neighbouring tiles on one XCD; within it columns of 8 tiles of tokens, so that few rows of weights are in use at once
   const int mt = (a.M + TM - 1) / TM, nt = (a.N + TN - 1) / TN;
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
   const int band = at / (8 * nt), rows = min(8, mt - band * 8), in = at - band * 8 * nt;
   const int m0 = (band * 8 + in % rows) * TM, n0 = in / rows * TN;
 
-  const int r0 = threadIdx.x >> 2, chunk = (threadIdx.x & 3) ^ ((r0 >> 2) & 3);
+  const int r0 = threadIdx.x >> 3, chunk = (threadIdx.x & 7) ^ ((r0 >> 1) & 7);
   const int8_t* from[PER];
   int last[PER];  // the furthest chunk that a row may be read at
 #pragma unroll
@@ -191,8 +194,7 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
   auto issue = [&](int step) {
     const int k = min(step, steps - 1) * BK + chunk * 16;
 #pragma unroll
-    for (int p = 0; p < PER; ++p)
-      i8_load_to_lds(from[p] + min(k, last[p]), to + (step % BUF) * (TM + TN) * BK + p * NT * 16);
+    for (int p = 0; p < PER; ++p) i8_load_to_lds(from[p] + min(k, last[p]), to + (step & 1) * TILE + p * NT * 16);
   };
 
   i32x16 acc[MI][NI];
@@ -201,41 +203,101 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = i32x16{};
   const int wm = wave / WN, wn = wave % WN, row = lane & 31, hi = lane >> 5;
+  const int8_t* xrow = s_tile + (wm * MI * 32 + row) * BK;
+  const int8_t* wrow = s_tile + (TM + wn * NI * 32 + row) * BK;
+  struct Part {
+    i32x4 x[MI], w[NI];
+  };
+  auto read = [&](Part& f, int step, int kk) {
+    const int pos = ((2 * kk + hi) ^ ((row >> 1) & 7)) * 16 + (step & 1) * TILE;
 #pragma unroll
-  for (int s = 0; s < BUF - 1; ++s) issue(s);
-  for (int s = 0; s < steps; ++s) {
-    i8_wait<(BUF - 2) * PER>();
-    lds_barrier();  // this step's tile is there for every wave; every wave is done with the one before it
-    issue(s + BUF - 1);
-    const int8_t* tile = s_tile + (s % BUF) * (TM + TN) * BK;
+    for (int i = 0; i < MI; ++i) f.x[i] = *reinterpret_cast<const i32x4*>(xrow + i * 32 * BK + pos);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      i32x4 x[MI], w[NI];
-      const int pos = ((2 * kk + hi) ^ ((row >> 2) & 3)) * 16;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) x[i] = *reinterpret_cast<const i32x4*>(tile + (wm * MI * 32 + i * 32 + row) * BK + pos);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) w[j] = *reinterpret_cast<const i32x4*>(tile + (TM + wn * NI * 32 + j * 32 + row) * BK + pos);
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], w[j], acc[i][j], 0, 0, 0);
-    }
-  }
-  i8_wait<0>();  // no load is left in flight when the workgroup's LDS goes to another
-  const I8Out<T> out(a);
-#pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int n = n0 + wn * NI * 32 + j * 32 + row;
-    const bool in_n = n < a.N;
-    const float wsn = in_n ? out.ws[n] : 0.f, b = in_n && out.bias ? to_f32(out.bias[n]) : 0.f;
+    for (int j = 0; j < NI; ++j) f.w[j] = *reinterpret_cast<const i32x4*>(wrow + j * 32 * BK + pos);
+  };
+  auto multiply = [&](const Part& f) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int m = m0 + wm * MI * 32 + i * 32 + 8 * (e / 4) + 4 * hi + e % 4;
-        if (in_n && m < a.M) out.y[(size_t)m * a.N + n] = out.value(acc[i][j][e], a.a_scale[m], wsn, b);
+      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[j], f.x[i], acc[i][j], 0, 0, 0);
+  };
+  // A quarter of a step is read while the one before is multiplied; before the last quarter every wave has read all of
+  // its tile, the next one is there, and the buffer is filled anew.  (Left to itself the compiler moves the reads to their
+  // use, and waits for each.)
+  issue(0);
+  issue(1);
+  i8_wait<PER>();
+  lds_barrier();
+  Part f[2];
+  read(f[0], 0, 0);
+  for (int s = 0; s < steps; ++s) {
+#pragma unroll
+    for (int kk = 0; kk < SUB; ++kk) {
+      if (kk + 1 < SUB) {
+        read(f[(kk + 1) & 1], s, kk + 1);
+      } else {
+        i8_wait<0>();
+        lds_barrier();
+        issue(s + 2);
+        read(f[0], s + 1, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(f[kk & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  i8_wait<0>();  // no load is left in flight when the buffers go to the results
+  lds_barrier();
+
+  // Results: 32 tokens of the wave at a time, rows of NI * 32 in LDS with the 16-byte chunks exchanged as above.
+  constexpr int COLS = NI * 32, RC = COLS * (int)sizeof(T) / 16;  // chunks of a row
+  auto place = [](int m, int c) { return (c ^ (RC == 16 ? m & 15 : RC == 8 ? (m >> 1) & 7 : (m >> 2) & 3)) * 16; };
+  unsigned char* mine = reinterpret_cast<unsigned char*>(s_tile) + wave * (32 * RC * 16);
+  const I8Out<T> out(a);
+  const int nw = n0 + wn * COLS;
+  const bool whole = ((size_t)a.N * sizeof(T)) % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
+  f32x4 ws[NI][4], bias[NI][4];
+#pragma unroll
+  for (int j = 0; j < NI; ++j)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = min(nw + j * 32 + 8 * g + 4 * hi + e, a.N - 1);
+        ws[j][g][e] = out.ws[n];
+        bias[j][g][e] = out.bias ? to_f32(out.bias[n]) : 0.f;
+      }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int mw = m0 + (wm * MI + i) * 32;
+    const float as = a.a_scale[min(mw + row, a.M - 1)];
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        T v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = out.value(acc[i][j][4 * g + e], as, ws[j][g][e], bias[j][g][e]);
+        const int b = (j * 32 + 8 * g + 4 * hi) * (int)sizeof(T);
+        __builtin_memcpy(__builtin_assume_aligned(mine + row * (RC * 16) + place(row, b / 16) + b % 16, sizeof(v)), v, sizeof(v));
+      }
+    wave_lds_fence();
+    if (whole) {
+#pragma unroll
+      for (int x = 0; x < RC / 2; ++x) {
+        const int m = (x * 64 + lane) / RC, c = lane % RC, n = nw + c * (16 / (int)sizeof(T));
+        if (mw + m < a.M && n < a.N)
+          *reinterpret_cast<i32x4*>(out.y + (size_t)(mw + m) * a.N + n) =
+              *reinterpret_cast<const i32x4*>(mine + m * (RC * 16) + place(m, c));
+      }
+    } else {
+      for (int x = 0; x < 32 * COLS / 64; ++x) {
+        const int m = (x * 64 + lane) / COLS, n = lane % COLS + (COLS > 64 ? x % (COLS / 64) * 64 : 0), b = n * (int)sizeof(T);
+        if (mw + m < a.M && nw + n < a.N)
+          out.y[(size_t)(mw + m) * a.N + nw + n] = *reinterpret_cast<const T*>(mine + m * (RC * 16) + place(m, b / 16) + b % 16);
+      }
+    }
+    wave_lds_fence();
   }
 }
 
@@ -258,7 +320,7 @@ hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s) 
 
 template <typename T, int TM, int TN, int WM, int WN> static hipError_t tile_t(const Int8LinearArgs& a, hipStream_t s) {
   auto kern = int8_tile_kernel<T, TM, TN, WM, WN>;
-  const size_t lds = 4 * (TM + TN) * 64;
+  const size_t lds = 2 * (TM + TN) * 128;
   const hipError_t e = set_lds_limit((const void*)kern, lds);
   if (e != hipSuccess) return e;
   const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + TN - 1) / TN);

@@ -67,7 +67,7 @@ struct RowCodesArgs {
 };
 
 struct Int8LinearArgs {
-  const int8_t* a;  // (M, as) codes of the tokens, zeros from K on; as a multiple of 64
+  const int8_t* a;  // (M, as) codes of the tokens, zeros from K on; as a multiple of 128
   const float* a_scale;
   const int8_t* w;  // (N, ws) codes of the weights
   const float* w_scale;
