@@ -58,10 +58,22 @@ template <typename T, bool FAST, int W> __global__ void __launch_bounds__(64 * W
   const float inv = 1.f / s;
   if (threadIdx.x == 0) a.scale[row] = s;
   auto put = [&](int c, const float (&v)[8]) {
-    unsigned w[2] = {0u, 0u};
-    if (fine) {
+    // 1.5 * 2^23 + x / s, nearly: a code in the low bits, and the right one where the remainder is less than half a step
+    unsigned w[2] = {0u, 0u}, u[8];
+    float far = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i / 4] |= ((unsigned)(int)i8_code(v[i], s, inv) & 255u) << (8 * (i % 4));
+    for (int i = 0; i < 8; ++i) {
+      const float y = __builtin_fmaf(v[i], inv, 12582912.f);
+      far = fmaxf(far, fabsf(__builtin_fmaf(12582912.f - y, s, v[i])));
+      u[i] = __float_as_uint(y);
+    }
+    if (fine) {
+      if (far >= 0.5f * s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = (unsigned)(int)i8_code(v[i], s, inv);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[h] = low_bytes(u[4 * h], u[4 * h + 1], u[4 * h + 2], u[4 * h + 3]);
     }
     *reinterpret_cast<uint2*>(out + c * 8) = make_uint2(w[0], w[1]);
   };

@@ -3,6 +3,7 @@
 //
 // A thread takes 8 elements of a row of the keys and the same of the values: 16 bytes of bf16 rows, 4 or 8 bytes of
 // codes, neighbouring threads neighbouring elements, so that a group's maximum is two exchanges within a quad of lanes.
+// A workgroup has whole rows (GR groups each: 64, 32, 21 or 16 of them), so that no thread divides a 64-bit index.
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 
@@ -10,34 +11,36 @@
 
 namespace dfl {
 
-// Latest position <= last that slot s holds; s <= last.  (Positions of a later chunk reach 2^31 + 2^28.)
-__device__ __forceinline__ unsigned slot_latest(unsigned s, unsigned last, unsigned n_sink, unsigned window) {
-  return s < n_sink ? s : s + (last - s) / window * window;
-}
-
-template <int BITS> __device__ __forceinline__ void store_codes(const LowbitCache& c, int b, int hk, int s, int ch,
+// Bounds: memory.  135 MB of bf16 prompts into 4 bits (32 x 8 heads, 1028 slots, d 128), 170 MB in all: 42 us from memory, 30
+// us where the prompts are in the last level of the caches; the loads alone take 34 us.  (Workgroups of 128 slots that hand
+// over whole lines of exponents, or hold four rows' loads in flight: the same.)
+template <int BITS> __device__ __forceinline__ void store_codes(const LowbitCache& q, int b, int hk, int s, int c,
                                                                 const unsigned (&w)[BITS / 4], unsigned e) {
-  uint8_t* to = c.codes + b * c.sb + hk * c.sh + s * c.sn + ch * BITS;
+  uint8_t* to = q.codes + b * q.sb + hk * q.sh + s * q.sn + c * BITS;
   if constexpr (BITS == 4) *reinterpret_cast<unsigned*>(to) = w[0];
   else *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-  if (ch % 4 == 0) c.exps[b * c.esb + hk * c.esh + ch / 4 * c.esg + s] = (uint8_t)e;
+  if (c % 4 == 0) q.exps[b * q.esb + hk * q.esh + c / 4 * q.esg + s] = (uint8_t)e;
 }
-
-template <typename T, int BITS, bool FAST> __global__ void __launch_bounds__(256) lowbit_fill_kernel(LowbitFillArgs a) {
-  const int nch = 4 * lb_groups(a.d), S = a.n_sink + a.window;
+template <typename T, int BITS, int GR, bool FAST> __global__ void __launch_bounds__(256) lowbit_fill_kernel(LowbitFillArgs a) {
+  constexpr int NCH = 4 * GR, ROWS = 256 / NCH;
+  const int S = a.n_sink + a.window;
   const int bh = blockIdx.y, b = bh / a.Hk, hk = bh % a.Hk;
   const int n = min(a.lengths[b], a.N), start = a.starts ? a.starts[b] : 0;
   if (n <= 0 || start < 0) return;
-  const unsigned last = (unsigned)start + (unsigned)n - 1;
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (slot, 8 elements)
-  const int s = (int)(e / nch), c = (int)(e % nch);
-  if (s >= S || (unsigned)s > last) return;
-  const unsigned p = slot_latest(s, last, a.n_sink, a.window);
+  const unsigned last = (unsigned)start + (unsigned)n - 1;  // at most 2^31 + 2^28
+  // Latest position that a slot holds: past the first tokens, turn `turns` of the window up to the slot of `last`, one
+  // turn less behind it.
+  const unsigned past = last >= (unsigned)a.n_sink ? last - a.n_sink : 0u, turns = past / a.window, rest = past - turns * a.window;
+  const int s = blockIdx.x * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
+  if ((int)threadIdx.x >= ROWS * NCH || s >= S || (unsigned)s > last) return;
+  const unsigned o = (unsigned)(s - a.n_sink), back = o > rest;
+  if (s >= a.n_sink && turns < back) return;
+  const unsigned p = s < a.n_sink ? (unsigned)s : a.n_sink + o + (turns - back) * a.window;
   if (p < (unsigned)start) return;
   const size_t row = p - (unsigned)start;
-  float k[8], v[8];
-  load8<T, FAST>(reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + row * a.ksn, c, a.d, k);
-  load8<T, FAST>(reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + row * a.vsn, c, a.d, v);
+  Eight<T> k, v;
+  load8<FAST>(k, reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh + row * a.ksn, c, a.d);
+  load8<FAST>(v, reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh + row * a.vsn, c, a.d);
   unsigned kw[BITS / 4], vw[BITS / 4];
   const unsigned ke = lb_encode<BITS>(k, kw), ve = lb_encode<BITS>(v, vw);
   store_codes<BITS>(a.kc, b, hk, s, c, kw, ke);
@@ -61,13 +64,13 @@ __device__ __forceinline__ void read_row(const LowbitCache& c, T* out, int b, in
   store8<T, FAST>(out, ch, d, x);
 }
 
-template <typename T, int BITS, bool FAST> __global__ void __launch_bounds__(256) cache_read_kernel(CacheReadArgs a) {
-  const int nch = (a.d + 7) / 8, S = a.n_sink + a.window;
+template <typename T, int BITS, int GR, bool FAST> __global__ void __launch_bounds__(256) cache_read_kernel(CacheReadArgs a) {
+  constexpr int NCH = 4 * GR, ROWS = 256 / NCH;
+  const int S = a.n_sink + a.window;
   const int bh = blockIdx.y, b = bh / a.Hk, hk = bh % a.Hk;
   const int len = a.lengths[b];
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (row, 8 elements)
-  const int j = (int)(e / nch), c = (int)(e % nch);
-  if (j >= S) return;
+  const int j = blockIdx.x * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
+  if ((int)threadIdx.x >= ROWS * NCH || j >= S || c * 8 >= a.d) return;
   const int p = j < a.n_sink ? j : max(len, 0) - S + j;  // S < 2^29: no overflow
   const bool held = j < a.n_sink ? j < len : p >= a.n_sink;
   const size_t at = ((size_t)bh * S + j) * a.d;
@@ -91,28 +94,44 @@ template <typename T> static bool aligned16(const void* p, std::initializer_list
   return ok;
 }
 
-template <typename T, int BITS> static hipError_t fill_b(const LowbitFillArgs& a, hipStream_t s) {
+template <typename T, int BITS, int GR> static hipError_t fill_g(const LowbitFillArgs& a, hipStream_t s) {
   const bool fast = a.d % 8 == 0 && aligned16<T>(a.k, {a.ksb, a.ksh, a.ksn}) && aligned16<T>(a.v, {a.vsb, a.vsh, a.vsn});
-  const long long per = (long long)(a.n_sink + a.window) * 4 * lb_groups(a.d);
-  const dim3 grid((unsigned)((per + 255) / 256), a.B * a.Hk);
-  if (fast) hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, false>), grid, dim3(256), 0, s, a);
+  constexpr int ROWS = 256 / (4 * GR);
+  const dim3 grid((a.n_sink + a.window + ROWS - 1) / ROWS, a.B * a.Hk);
+  if (fast) hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
+}
+template <typename T, int BITS> static hipError_t fill_b(const LowbitFillArgs& a, hipStream_t s) {
+  switch (lb_groups(a.d)) {
+    case 1: return fill_g<T, BITS, 1>(a, s);
+    case 2: return fill_g<T, BITS, 2>(a, s);
+    case 3: return fill_g<T, BITS, 3>(a, s);
+    default: return fill_g<T, BITS, 4>(a, s);
+  }
 }
 hipError_t launch_lowbit_fill(const LowbitFillArgs& a, bool bf16_in, int bits, hipStream_t s) {
   if (bf16_in) return bits == 4 ? fill_b<bf16, 4>(a, s) : fill_b<bf16, 8>(a, s);
   return bits == 4 ? fill_b<float, 4>(a, s) : fill_b<float, 8>(a, s);
 }
 
-template <typename T, int BITS> static hipError_t read_b(const CacheReadArgs& a, hipStream_t s) {
+template <typename T, int BITS, int GR> static hipError_t read_g(const CacheReadArgs& a, hipStream_t s) {
   bool fast = a.d % 8 == 0 && aligned16<T>(a.k, {}) && aligned16<T>(a.v, {});
   if (BITS == 0)
     fast = fast && aligned16<T>(a.kc.codes, {a.kc.sb, a.kc.sh, a.kc.sn}) && aligned16<T>(a.vc.codes, {a.vc.sb, a.vc.sh, a.vc.sn});
-  const long long per = (long long)(a.n_sink + a.window) * ((a.d + 7) / 8);
-  const dim3 grid((unsigned)((per + 255) / 256), a.B * a.Hk);
-  if (fast) hipLaunchKernelGGL((cache_read_kernel<T, BITS, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((cache_read_kernel<T, BITS, false>), grid, dim3(256), 0, s, a);
+  constexpr int ROWS = 256 / (4 * GR);
+  const dim3 grid((a.n_sink + a.window + ROWS - 1) / ROWS, a.B * a.Hk);
+  if (fast) hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
+}
+template <typename T, int BITS> static hipError_t read_b(const CacheReadArgs& a, hipStream_t s) {
+  switch (lb_groups(a.d)) {
+    case 1: return read_g<T, BITS, 1>(a, s);
+    case 2: return read_g<T, BITS, 2>(a, s);
+    case 3: return read_g<T, BITS, 3>(a, s);
+    default: return read_g<T, BITS, 4>(a, s);
+  }
 }
 template <typename T> static hipError_t read_t(const CacheReadArgs& a, int bits, hipStream_t s) {
   return bits == 4 ? read_b<T, 4>(a, s) : bits == 8 ? read_b<T, 8>(a, s) : read_b<T, 0>(a, s);

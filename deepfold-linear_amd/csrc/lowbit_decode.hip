@@ -164,9 +164,9 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
   if (mine && wave < 2 && lane < nch) {
     const T* row = wave ? reinterpret_cast<const T*>(a.v) + b * a.vsb + hk * a.vsh
                         : reinterpret_cast<const T*>(a.k) + b * a.ksb + hk * a.ksh;
-    float e[8];
+    Eight<T> e;
     unsigned w[BITS / 4];
-    load8<T, false>(row, lane, a.d, e);
+    load8<false>(e, row, lane, a.d);
     const unsigned ex = lb_encode<BITS>(e, w);
     unsigned* at = reinterpret_cast<unsigned*>(s_own + wave * (DP * BITS / 8) + lane * BITS);
 #pragma unroll
