@@ -18,6 +18,7 @@ hipError_t launch_cache_read(const CacheReadArgs& a, bool bf16_out, int bits, hi
 hipError_t launch_lowbit_decode(const LowbitDecodeArgs& a, bool bf16_in, int bits, int DP, hipStream_t s);
 LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S);
 hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s);
+int int8_linear_form(int M, int K, int N);
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s);
 }  // namespace dfl
 
@@ -91,17 +92,6 @@ dfl::LowbitCache cache(const dfl_lowbit_cache& c) {
           c.exp_stride_b, c.exp_stride_h, c.exp_stride_g};
 }
 
-// Which kernel a product takes.
-int linear_form(int M, int K, int N) {
-  (void)K;
-  auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
-  if (M <= 16) return 1;
-  if (M <= 32) return 2;
-  if (M <= 64) return 3;
-  if (tiles(256) >= 256) return 6;
-  if (tiles(128) >= 256) return 5;
-  return 4;
-}
 size_t code_row(int K) { return ((size_t)K + 127) / 128 * 128; }
 bool linear_ok(int M, int K, int N) { return M > 0 && K > 0 && N > 0 && K <= MAX_K; }
 struct LinearWs {
@@ -224,7 +214,9 @@ int dfl_quantize_rows(const dfl_quantize_rows_params* p, void* stream) {
   });
 }
 
-size_t dfl_int8_linear_workspace_size(int M, int K, int N) { return linear_ok(M, K, N) ? LinearWs(M, K).total : 0; }
+size_t dfl_int8_linear_workspace_size(int M, int K, int N) {
+  return linear_ok(M, K, N) && dfl::int8_linear_form(M, K, N) != 0 ? LinearWs(M, K).total : 0;
+}
 
 int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t workspace_bytes, void* stream) {
   return guarded([&] {
@@ -234,18 +226,24 @@ int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t wor
     if (!p->x || !p->w || !p->w_scale || !p->y) return fail("required pointer is NULL");
     if (p->w_stride < p->K || ((uintptr_t)p->w | (uintptr_t)p->w_stride) & 15)
       return fail("w and w_stride must be multiples of 16 bytes, w_stride at least K");
-    const LinearWs ws(p->M, p->K);
-    if (!workspace || workspace_bytes < ws.total) return fail("workspace too small: need %zu bytes", ws.total);
-    if ((uintptr_t)workspace & 15) return fail("workspace must be 16-byte aligned");
-    const int form = linear_form(p->M, p->K, p->N);
+    const int form = dfl::int8_linear_form(p->M, p->K, p->N);
     if (form >= 4 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
-    unsigned char* at = static_cast<unsigned char*>(workspace);
-    const dfl::RowCodesArgs r = {p->x, p->x_stride, reinterpret_cast<int8_t*>(at), (long long)code_row(p->K),
-                                 reinterpret_cast<float*>(at + ws.scale), p->M, p->K};
-    hipError_t e = dfl::launch_row_codes(r, p->dtype == DFL_BF16, (hipStream_t)stream);
-    if (e != hipSuccess) return dfl::capi_hip_fail(e, "row quantisation launch");
-    const dfl::Int8LinearArgs a = {r.codes, r.scale, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,
-                                   r.cs, p->w_stride, p->M, p->K, p->N};
+    dfl::Int8LinearArgs a = {p->x, p->x_stride, nullptr, nullptr, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,
+                             0, p->w_stride, p->M, p->K, p->N};
+    hipError_t e;
+    if (form != 0) {
+      const LinearWs ws(p->M, p->K);
+      if (!workspace || workspace_bytes < ws.total) return fail("workspace too small: need %zu bytes", ws.total);
+      if ((uintptr_t)workspace & 15) return fail("workspace must be 16-byte aligned");
+      unsigned char* at = static_cast<unsigned char*>(workspace);
+      const dfl::RowCodesArgs r = {p->x, p->x_stride, reinterpret_cast<int8_t*>(at), (long long)code_row(p->K),
+                                   reinterpret_cast<float*>(at + ws.scale), p->M, p->K};
+      e = dfl::launch_row_codes(r, p->dtype == DFL_BF16, (hipStream_t)stream);
+      if (e != hipSuccess) return dfl::capi_hip_fail(e, "row quantisation launch");
+      a.a = r.codes;
+      a.a_scale = r.scale;
+      a.as = r.cs;
+    }
     e = dfl::launch_int8_linear(a, p->dtype == DFL_BF16, form, (hipStream_t)stream);
     return e == hipSuccess ? 0 : dfl::capi_hip_fail(e, "8-bit product launch");
   });

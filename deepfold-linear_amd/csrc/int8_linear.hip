@@ -23,6 +23,32 @@ __device__ __forceinline__ float i8_code(float x, float s, float inv) {
   return q;
 }
 
+// The scale of a row by its largest magnitude's bits: NaN where that is no finite number.
+__device__ __forceinline__ float i8_scale(unsigned top) {
+  return top < 0x7f800000u ? fmaxf(__uint_as_float(top) / 127.f, I8_MIN_SCALE) : __builtin_nanf("");
+}
+// 8 codes; zeros where the scale is NaN.
+__device__ __forceinline__ void i8_codes(const float (&v)[8], float s, float inv, unsigned (&w)[2]) {
+  // 1.5 * 2^23 + x / s, nearly: a code in the low bits, and the right one where the remainder is less than half a step
+  unsigned u[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __builtin_fmaf(v[i], inv, 12582912.f);
+    far = fmaxf(far, fabsf(__builtin_fmaf(12582912.f - y, s, v[i])));
+    u[i] = __float_as_uint(y);
+  }
+  w[0] = w[1] = 0u;
+  if (s == s) {
+    if (far >= 0.5f * s) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = (unsigned)(int)i8_code(v[i], s, inv);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = low_bytes(u[4 * h], u[4 * h + 1], u[4 * h + 2], u[4 * h + 3]);
+  }
+}
+
 // A row a workgroup of 64 W threads, its elements in registers where they fit.
 constexpr int I8_KEEP = 4;  // 8 elements each
 template <typename T, bool FAST, int W> __global__ void __launch_bounds__(64 * W) row_codes_kernel(RowCodesArgs a) {
@@ -53,28 +79,11 @@ template <typename T, bool FAST, int W> __global__ void __launch_bounds__(64 * W
 #pragma unroll
     for (int w = 0; w < W; ++w) top = max(top, s_top[w]);
   }
-  const bool fine = top < 0x7f800000u;
-  const float s = fine ? fmaxf(__uint_as_float(top) / 127.f, I8_MIN_SCALE) : __builtin_nanf("");
-  const float inv = 1.f / s;
+  const float s = i8_scale(top), inv = 1.f / s;
   if (threadIdx.x == 0) a.scale[row] = s;
   auto put = [&](int c, const float (&v)[8]) {
-    // 1.5 * 2^23 + x / s, nearly: a code in the low bits, and the right one where the remainder is less than half a step
-    unsigned w[2] = {0u, 0u}, u[8];
-    float far = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __builtin_fmaf(v[i], inv, 12582912.f);
-      far = fmaxf(far, fabsf(__builtin_fmaf(12582912.f - y, s, v[i])));
-      u[i] = __float_as_uint(y);
-    }
-    if (fine) {
-      if (far >= 0.5f * s) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = (unsigned)(int)i8_code(v[i], s, inv);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) w[h] = low_bytes(u[4 * h], u[4 * h + 1], u[4 * h + 2], u[4 * h + 3]);
-    }
+    unsigned w[2];
+    i8_codes(v, s, inv, w);
     *reinterpret_cast<uint2*>(out + c * 8) = make_uint2(w[0], w[1]);
   };
 #pragma unroll
@@ -103,34 +112,104 @@ template <typename T> struct I8Out {
 };
 
 // Few tokens: the weights go by once.  A workgroup has 16 rows of weights and MT tiles of 16 tokens; its waves share K,
-// in steps of 64 bytes, straight from memory into the operands: lane l holds row l % 16 and a quarter l / 16 of the step.
-template <typename T, int MT> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
-  constexpr int WAVES = 8, U = 4;
+// in steps of 128 bytes, straight from memory into the operands: lane l holds row l % 16 and the 32 bytes l / 16 of a step
+// (any order of the bytes will do, as long as weights and tokens have the same).
+// OWN: up to I8_OWN tokens, whose codes each workgroup forms itself while its first weights arrive: one launch, and no
+// workspace.
+constexpr int I8_OWN = 4, I8_OWN_K = 8192;
+template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
+  constexpr int WAVES = 8, U = MT == 4 ? 2 : 4;  // steps in flight
   __shared__ int s_sum[WAVES][MT][16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, h = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+  __shared__ float s_scale[OWN ? I8_OWN : 1];
+  extern __shared__ __align__(16) int8_t s_x[];  // OWN: [M][steps * 128] codes
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, h = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = OWN ? 0 : blockIdx.y * (16 * MT);
   const int8_t* w = a.w + (long long)min(n0 + r, a.N - 1) * a.ws;
-  const int8_t* x[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) x[i] = a.a + (long long)min(m0 + 16 * i + r, a.M - 1) * a.as;
-  const int steps = (a.K + 63) / 64, tail = ((a.K + 15) & ~15) - 16;  // last 16 bytes of a row of weights
+  const int steps = (a.K + 127) / 128, tail = ((a.K + 15) & ~15) - 16;  // last 16 bytes of a row of weights
+  auto weights = [&](i32x4 (&v)[2], int s) {
+    const int k = s * 128 + 32 * h;  // (past the row's end: tokens are zero there)
+    v[0] = *reinterpret_cast<const i32x4*>(w + min(k, tail));
+    v[1] = *reinterpret_cast<const i32x4*>(w + min(k + 16, tail));
+  };
   i32x4 sum[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) sum[i] = i32x4{0, 0, 0, 0};
-  for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
-    i32x4 wv[U], xv[U][MT];
+  if constexpr (OWN) {
+    i32x4 wv[U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = min(s0 + u * WAVES, steps - 1) * 64 + 16 * h;
-      wv[u] = *reinterpret_cast<const i32x4*>(w + min(k, tail));  // (past the row's end: tokens are zero there)
+    for (int u = 0; u < U; ++u) weights(wv[u], min(wave + u * WAVES, steps - 1));
+    __shared__ unsigned s_top[I8_OWN][WAVES];
+    constexpr int KEEP = I8_OWN_K / (512 * 8);
+    float e[I8_OWN][KEEP][8];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xv[u][i] = *reinterpret_cast<const i32x4*>(x[i] + k);
+    for (int m = 0; m < I8_OWN; ++m)
+      if (m < a.M) {
+        unsigned top = 0;
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+          load8<T, FAST>(reinterpret_cast<const T*>(a.x) + m * a.xs, threadIdx.x + k * 512, a.K, e[m][k]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(e[m][k][i]) & 0x7fffffffu);
+        }
+        top = wave_max_u32(top);
+        if (lane == 0) s_top[m][wave] = top;
+      }
+    lds_barrier();
+#pragma unroll
+    for (int m = 0; m < I8_OWN; ++m)
+      if (m < a.M) {
+        unsigned top = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) top = max(top, s_top[m][v]);
+        const float s = i8_scale(top), inv = 1.f / s;
+        if (threadIdx.x == 0) s_scale[m] = s;
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+          const int c = threadIdx.x + k * 512;
+          unsigned q[2];
+          i8_codes(e[m][k], s, inv, q);
+          if (c < steps * 16) *reinterpret_cast<uint2*>(s_x + m * steps * 128 + c * 8) = make_uint2(q[0], q[1]);
+        }
+      }
+    lds_barrier();
+    const int8_t* x = s_x + min(r, a.M - 1) * steps * 128 + 32 * h;
+    for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + u * WAVES;
+        if (s < steps) {
+          const i32x4* xv = reinterpret_cast<const i32x4*>(x + s * 128);
+          sum[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][0], xv[0], sum[0], 0, 0, 0);
+          sum[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][1], xv[1], sum[0], 0, 0, 0);
+        }
+        if (s + WAVES * U < steps) weights(wv[u], s + WAVES * U);
+      }
     }
+  } else {
+    const int8_t* x[MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s0 + u * WAVES < steps) {
+    for (int i = 0; i < MT; ++i) x[i] = a.a + (long long)min(m0 + 16 * i + r, a.M - 1) * a.as;
+    for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
+      i32x4 wv[U][2], xv[U][MT][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u], xv[u][i], sum[i], 0, 0, 0);
+      for (int u = 0; u < U; ++u) {
+        const int s = min(s0 + u * WAVES, steps - 1);
+        weights(wv[u], s);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const i32x4* at = reinterpret_cast<const i32x4*>(x[i] + s * 128 + 32 * h);
+          xv[u][i][0] = at[0], xv[u][i][1] = at[1];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s0 + u * WAVES < steps) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][0], xv[u][i][0], sum[i], 0, 0, 0);
+            sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][1], xv[u][i][1], sum[i], 0, 0, 0);
+          }
+        }
       }
     }
   }
@@ -146,8 +225,8 @@ template <typename T, int MT> __global__ void __launch_bounds__(512) int8_few_ke
     int t = 0;
 #pragma unroll
     for (int v = 0; v < WAVES; ++v) t += s_sum[v][m >> 4][m & 15][c];
-    const float b = out.bias ? to_f32(out.bias[n0 + c]) : 0.f;
-    out.y[(size_t)(m0 + m) * a.N + n0 + c] = out.value(t, a.a_scale[m0 + m], out.ws[n0 + c], b);
+    const float b = out.bias ? to_f32(out.bias[n0 + c]) : 0.f, as = OWN ? s_scale[m] : a.a_scale[m0 + m];
+    out.y[(size_t)(m0 + m) * a.N + n0 + c] = out.value(t, as, out.ws[n0 + c], b);
   }
 }
 
@@ -341,11 +420,19 @@ template <typename T, int TM, int TN, int WM, int WN> static hipError_t tile_t(c
 }
 template <typename T, int MT> static hipError_t few_t(const Int8LinearArgs& a, hipStream_t s) {
   const dim3 grid((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT));
-  hipLaunchKernelGGL((int8_few_kernel<T, MT>), grid, dim3(512), 0, s, a);
+  hipLaunchKernelGGL((int8_few_kernel<T, MT, false, false>), grid, dim3(512), 0, s, a);
+  return hipGetLastError();
+}
+template <typename T> static hipError_t own_t(const Int8LinearArgs& a, hipStream_t s) {
+  const bool fast = a.K % 8 == 0 && aligned16<T>(a.x, {a.xs});
+  const size_t lds = (size_t)a.M * ((a.K + 127) / 128 * 128);
+  if (fast) hipLaunchKernelGGL((int8_few_kernel<T, 1, true, true>), dim3((a.N + 15) / 16), dim3(512), lds, s, a);
+  else hipLaunchKernelGGL((int8_few_kernel<T, 1, true, false>), dim3((a.N + 15) / 16), dim3(512), lds, s, a);
   return hipGetLastError();
 }
 template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int form, hipStream_t s) {
   switch (form) {
+    case 0: return own_t<T>(a, s);
     case 1: return few_t<T, 1>(a, s);
     case 2: return few_t<T, 2>(a, s);
     case 3: return few_t<T, 4>(a, s);
@@ -356,6 +443,18 @@ template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int fo
 }
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s) {
   return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
+}
+
+// Which kernel a product takes (0: forms the codes itself and needs no workspace).
+int int8_linear_form(int M, int K, int N) {
+  auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
+  if (M <= I8_OWN && K <= I8_OWN_K) return 0;
+  if (M <= 16) return 1;
+  if (M <= 32) return 2;
+  if (M <= 64) return 3;
+  if (tiles(256) >= 256) return 6;
+  if (tiles(128) >= 256) return 5;
+  return 4;
 }
 
 }  // namespace dfl

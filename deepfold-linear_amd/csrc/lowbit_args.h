@@ -67,6 +67,8 @@ struct RowCodesArgs {
 };
 
 struct Int8LinearArgs {
+  const void* x;    // (M,K) tokens, element stride (the form that makes the codes itself)
+  long long xs;
   const int8_t* a;  // (M, as) codes of the tokens, zeros from K on; as a multiple of 128
   const float* a_scale;
   const int8_t* w;  // (N, ws) codes of the weights

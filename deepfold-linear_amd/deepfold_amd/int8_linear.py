@@ -62,10 +62,10 @@ def _linear(x, codes, scale, bias):
     lib = _lib.load()
     # the tokens' codes, in a workspace of the call's own: calls on other streams and captured graphs cannot share it
     nbytes = lib.dfl_int8_linear_workspace_size(M, K, N)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _lib.on_device(dev):
         rc = _lib.timed_launch("int8_linear", dev, lambda: lib.dfl_int8_linear(
-            ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
     _lib.check(rc, "dfl_int8_linear")
     return y
 

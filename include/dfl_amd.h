@@ -702,6 +702,7 @@ int dfl_lowbit_cache_fill(const dfl_lowbit_cache_fill_params* p, void* stream);
 size_t dfl_lowbit_decode_workspace_size(int B, int H, int Hk, int d, int window, int n_sink);
 int dfl_lowbit_decode(const dfl_lowbit_decode_params* p, void* workspace, size_t workspace_bytes, void* stream);
 int dfl_quantize_rows(const dfl_quantize_rows_params* p, void* stream);
+/* 0 where the kernel forms the tokens' codes itself (few tokens): the workspace may then be NULL. */
 size_t dfl_int8_linear_workspace_size(int M, int K, int N);
 int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -124,10 +124,12 @@ def test_workspaces():
     assert lib.dfl_lowbit_decode(ctypes.byref(decode_params()), FAKE, need - 1, None) < 0
     assert b"workspace too small" in lib.dfl_last_error()
     assert lib.dfl_lowbit_decode(ctypes.byref(decode_params()), None, need, None) < 0
-    need = lib.dfl_int8_linear_workspace_size(4, 60, 8)
-    assert lib.dfl_int8_linear(ctypes.byref(linear_params()), FAKE, need - 1, None) < 0
+    assert lib.dfl_int8_linear_workspace_size(4, 60, 8) == 0  # (few tokens: none is needed)
+    need = lib.dfl_int8_linear_workspace_size(9, 60, 8)
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), FAKE, need - 1, None) < 0
     assert b"workspace too small" in lib.dfl_last_error()
-    assert lib.dfl_int8_linear(ctypes.byref(linear_params()), FAKE + 8, need, None) < 0
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), FAKE + 8, need, None) < 0
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), None, need, None) < 0
 
 
 class Launches:
