@@ -227,7 +227,7 @@ int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t wor
     if (p->w_stride < p->K || ((uintptr_t)p->w | (uintptr_t)p->w_stride) & 15)
       return fail("w and w_stride must be multiples of 16 bytes, w_stride at least K");
     const int form = dfl::int8_linear_form(p->M, p->K, p->N);
-    if (form >= 4 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
+    if (form >= 3 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
     dfl::Int8LinearArgs a = {p->x, p->x_stride, nullptr, nullptr, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,
                              0, p->w_stride, p->M, p->K, p->N};
     hipError_t e;

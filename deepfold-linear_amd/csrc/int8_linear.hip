@@ -118,7 +118,7 @@ template <typename T> struct I8Out {
 // workspace.
 constexpr int I8_OWN = 4, I8_OWN_K = 8192;
 template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
-  constexpr int WAVES = 8, U = MT == 4 ? 2 : 4;  // steps in flight
+  constexpr int WAVES = 8, U = 4;  // steps in flight
   __shared__ int s_sum[WAVES][MT][16][17];
   __shared__ float s_scale[OWN ? I8_OWN : 1];
   extern __shared__ __align__(16) int8_t s_x[];  // OWN: [M][steps * 128] codes
@@ -243,17 +243,17 @@ template <int N> __device__ __forceinline__ void i8_wait() {
 }
 
 // Tiles of TM tokens and TN rows of weights, WM x WN waves of 32 x 32 blocks.  K goes by in steps of 128 bytes, whole lines
-// of memory, through two LDS buffers that are loaded without passing through registers; a row's 16-byte chunk c lies
+// of memory, through BUF LDS buffers that are loaded without passing through registers; a row's 16-byte chunk c lies
 // at position c ^ (row / 2 % 8), so that 16 lanes reading the same chunk of 16 rows meet every bank once.  The weights are
 // the instructions' first operand: a lane of the accumulators has one token and runs of four rows of weights, and the results
 // leave through LDS in whole lines.
-template <typename T, int TM, int TN, int WM, int WN>
+template <typename T, int TM, int TN, int WM, int WN, int BUF>
 __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs a) {
   constexpr int NT = 64 * WM * WN, BK = 128, SUB = BK / 32, MI = TM / WM / 32, NI = TN / WN / 32;
   constexpr int CHUNKS = (TM + TN) * 8, PER = CHUNKS / NT, STEP = NT / 8;  // rows between a thread's chunks
   constexpr int TILE = (TM + TN) * BK;
   static_assert(CHUNKS % NT == 0 && STEP % 16 == 0 && TM % STEP == 0, "whole loads of one swizzle");
-  extern __shared__ __align__(16) int8_t s_tile[];  // [2][TM + TN][128]
+  extern __shared__ __align__(16) int8_t s_tile[];  // [BUF][TM + TN][128]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // neighbouring tiles on one XCD; within it columns of 8 tiles of tokens, so that few rows of weights are in use at once
   const int mt = (a.M + TM - 1) / TM, nt = (a.N + TN - 1) / TN;
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
   auto issue = [&](int step) {
     const int k = min(step, steps - 1) * BK + chunk * 16;
 #pragma unroll
-    for (int p = 0; p < PER; ++p) i8_load_to_lds(from[p] + min(k, last[p]), to + (step & 1) * TILE + p * NT * 16);
+    for (int p = 0; p < PER; ++p) i8_load_to_lds(from[p] + min(k, last[p]), to + (step % BUF) * TILE + p * NT * 16);
   };
 
   i32x16 acc[MI][NI];
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
     i32x4 x[MI], w[NI];
   };
   auto read = [&](Part& f, int step, int kk) {
-    const int pos = ((2 * kk + hi) ^ ((row >> 1) & 7)) * 16 + (step & 1) * TILE;
+    const int pos = ((2 * kk + hi) ^ ((row >> 1) & 7)) * 16 + (step % BUF) * TILE;
 #pragma unroll
     for (int i = 0; i < MI; ++i) f.x[i] = *reinterpret_cast<const i32x4*>(xrow + i * 32 * BK + pos);
 #pragma unroll
@@ -315,9 +315,9 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
   // A quarter of a step is read while the one before is multiplied; before the last quarter every wave has read all of
   // its tile, the next one is there, and the buffer is filled anew.  (Left to itself the compiler moves the reads to their
   // use, and waits for each.)
-  issue(0);
-  issue(1);
-  i8_wait<PER>();
+#pragma unroll
+  for (int s = 0; s < BUF; ++s) issue(s);
+  i8_wait<(BUF - 1) * PER>();
   lds_barrier();
   Part f[2];
   read(f[0], 0, 0);
@@ -327,9 +327,9 @@ __global__ void __launch_bounds__(64 * WM * WN) int8_tile_kernel(Int8LinearArgs 
       if (kk + 1 < SUB) {
         read(f[(kk + 1) & 1], s, kk + 1);
       } else {
-        i8_wait<0>();
+        i8_wait<(BUF - 2) * PER>();
         lds_barrier();
-        issue(s + 2);
+        issue(s + BUF);
         read(f[0], s + 1, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -409,9 +409,9 @@ hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s) 
   return wide ? codes_w<float, 4>(a, s) : codes_w<float, 1>(a, s);
 }
 
-template <typename T, int TM, int TN, int WM, int WN> static hipError_t tile_t(const Int8LinearArgs& a, hipStream_t s) {
-  auto kern = int8_tile_kernel<T, TM, TN, WM, WN>;
-  const size_t lds = 2 * (TM + TN) * 128;
+template <typename T, int TM, int TN, int WM, int WN, int BUF> static hipError_t tile_t(const Int8LinearArgs& a, hipStream_t s) {
+  auto kern = int8_tile_kernel<T, TM, TN, WM, WN, BUF>;
+  const size_t lds = BUF * (TM + TN) * 128;
   const hipError_t e = set_lds_limit((const void*)kern, lds);
   if (e != hipSuccess) return e;
   const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + TN - 1) / TN);
@@ -435,26 +435,34 @@ template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int fo
     case 0: return own_t<T>(a, s);
     case 1: return few_t<T, 1>(a, s);
     case 2: return few_t<T, 2>(a, s);
-    case 3: return few_t<T, 4>(a, s);
-    case 4: return tile_t<T, 64, 64, 2, 2>(a, s);
-    case 5: return tile_t<T, 128, 128, 2, 2>(a, s);
-    default: return tile_t<T, 256, 256, 2, 4>(a, s);
+    case 3: return tile_t<T, 64, 64, 2, 2, 4>(a, s);
+    case 4: return tile_t<T, 128, 128, 2, 2, 2>(a, s);
+    default: return tile_t<T, 256, 256, 2, 4, 2>(a, s);
   }
 }
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s) {
   return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
 }
 
-// Which kernel a product takes (0: forms the codes itself and needs no workspace).
+// Which kernel a product takes (0: forms the codes itself and needs no workspace).  Calls (us, codes and product, in a
+// graph) of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and 256 x 256 tiles:
+//   M 16, K 4096, N 4096     10.1  10.3  12.3  25.0  50.4
+//   32, 4096, 4096              -  11.9  12.5  25.4  50.5
+//   64, 4096, 4096              -  17.4  12.8  25.9  50.5
+//   97, 512, 512                -   6.4   6.8   9.7  13.8
+//   200, 6000, 500              -  15.8  18.9  37.6  77.0
+//   65, 6000, 6000              -  44.9  18.5  41.3  70.9
+//   512, 4096, 4096             -  93.2  23.3  29.5  55.0
+//   1024, 4096, 4096            -   179  41.4  34.7  56.9
+//   2048, 4096, 4096            -   352  72.8  51.0  61.5
+//   4096, 4096, 4096            -   694   128   102  81.9
+// So: few tokens, or too few tiles to go round, the first; the largest tiles of which there is about one a CU.
 int int8_linear_form(int M, int K, int N) {
   auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
   if (M <= I8_OWN && K <= I8_OWN_K) return 0;
   if (M <= 16) return 1;
-  if (M <= 32) return 2;
-  if (M <= 64) return 3;
-  if (tiles(256) >= 256) return 6;
-  if (tiles(128) >= 256) return 5;
-  return 4;
+  if (M <= 32 || tiles(64) < 48) return 2;
+  return tiles(256) >= 224 ? 5 : tiles(128) >= 224 ? 4 : 3;
 }
 
 }  // namespace dfl

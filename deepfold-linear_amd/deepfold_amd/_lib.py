@@ -416,6 +416,8 @@ SIGNATURES = [
 def load(path: str = LIB_PATH):
     """Load (once) and return the ctypes handle; raise if the library is absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(path):
@@ -487,7 +489,7 @@ class on_device:
         self.index = device.index
 
     def __enter__(self):
-        self.back = torch.cuda.current_device()
+        self.back = torch._C._cuda_getDevice()
         if self.back != self.index:
             torch.cuda.set_device(self.index)
 

@@ -44,7 +44,7 @@ def _quantize(x):
     lib = _lib.load()
     with _lib.on_device(dev):
         rc = _lib.timed_launch("quantize_rows", dev, lambda: lib.dfl_quantize_rows(
-            ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), _lib.stream_handle(dev)))
     _lib.check(rc, "dfl_quantize_rows")
     return codes[:, :K], scale
 
@@ -65,7 +65,7 @@ def _linear(x, codes, scale, bias):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _lib.on_device(dev):
         rc = _lib.timed_launch("int8_linear", dev, lambda: lib.dfl_int8_linear(
-            ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), _lib.ptr(ws), nbytes, _lib.stream_handle(dev)))
     _lib.check(rc, "dfl_int8_linear")
     return y
 

@@ -351,7 +351,7 @@ def _fill_codes(K, V, lengths, starts, kc, ke, vc, ve, bits, n_sink):
     lib = _lib.load()
     with _lib.on_device(dev):
         rc = _lib.timed_launch("window_cache_fill", dev, lambda: lib.dfl_lowbit_cache_fill(
-            ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), _lib.stream_handle(dev)))
     _lib.check(rc, "dfl_lowbit_cache_fill")
     torch.autograd.graph.increment_version((kc, ke, vc, ve))
 
@@ -370,7 +370,7 @@ def _read(lengths, kc, ke, vc, ve, bits, d, n_sink, dtype):
     lib = _lib.load()
     with _lib.on_device(dev):
         rc = _lib.timed_launch("window_cache_read", dev, lambda: lib.dfl_window_cache_read(
-            ctypes.byref(p), ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), _lib.stream_handle(dev)))
     _lib.check(rc, "dfl_window_cache_read")
     return k, v, mask
 
@@ -392,7 +392,7 @@ def _decode_codes(q, k, v, kc, ke, vc, ve, lengths, rel_table, arr, bits, n_sink
         scale, o.data_ptr())
     with _lib.on_device(dev):
         rc = _lib.timed_launch("window_decode_attn", dev, lambda: lib.dfl_lowbit_decode(
-            ctypes.byref(p), ctypes.c_void_p(_lib.ptr(ws)), nbytes, ctypes.c_void_p(_lib.stream_handle(dev))))
+            ctypes.byref(p), _lib.ptr(ws), nbytes, _lib.stream_handle(dev)))
     _lib.check(rc, "dfl_lowbit_decode")
     torch.autograd.graph.increment_version((kc, ke, vc, ve))
     return o

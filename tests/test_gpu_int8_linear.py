@@ -59,7 +59,8 @@ def test_linear(M, K, N, dtype):
     case(M, K, N, dtype, bias=(M + K + N) % 2 == 0)
 
 
-@pytest.mark.parametrize("M,K,N", [(2048, 192, 2048), (2049, 80, 2177), (4096, 64, 4096), (4100, 130, 4099)])
+@pytest.mark.parametrize("M,K,N", [(500, 100, 450), (513, 2100, 449), (3100, 33, 60), (66, 700, 1600), (2048, 192, 2048),
+                                   (2049, 80, 2177), (4096, 64, 4096), (4100, 130, 4099)])
 def test_linear_large_tiles(M, K, N):
     """Products of enough tiles for the larger ones, whole and with ragged edges."""
     case(M, K, N, BF)
@@ -80,6 +81,19 @@ def test_largest_sums(M):
     y = int8_linear(x.to(DEV), codes.to(DEV), scale.to(DEV))
     holds(y, *ref.linear(x, codes, scale, None, F32))
     assert not y[:, 2].any() and (y[:, 0] > 2.6e7).all()
+
+
+@pytest.mark.parametrize("M,N", [(385, 449), (2048, 2048)])
+def test_largest_sums_in_tiles(M, N):
+    from deepfold_amd import int8_linear
+
+    K = 2**17 if M < 2048 else 2**12
+    codes = torch.full((N, K), 127, dtype=torch.int8, device=DEV)
+    codes[1::2] = -127
+    y = int8_linear(torch.full((M, K), 2.0, dtype=BF, device=DEV), codes, torch.ones(N, device=DEV))
+    want = torch.full((M, N), 127.0 * 127 * K * float(torch.tensor(2.0 / 127)), dtype=torch.float64)
+    want[:, 1::2] *= -1
+    holds(y, want, want.abs() * (2.0**-9 + 2.0**-20))
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
