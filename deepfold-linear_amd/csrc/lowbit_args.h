@@ -45,6 +45,7 @@ struct LowbitDecodeArgs {
   RelSpec rel;
   int B, H, Hk, d, window, n_sink;
   float scale;
+  bool q_fast;  // the queries' rows are 16-byte aligned, d a multiple of 8
   void* o;      // (B,H,d) contiguous
   float* part;  // [B*H][n_split][2 + DP]: reference, sum, output of a split (n_split > 1)
   int waves;           // of a workgroup

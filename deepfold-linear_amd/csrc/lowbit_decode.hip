@@ -40,8 +40,10 @@ constexpr int lb_waves(int size, int DP, int NT) {
 constexpr float LB_LAZY = 8.f;
 constexpr long long CUS = 256;
 
-__device__ __forceinline__ int lb_position(int s, int last, int n_sink, int window) {
-  return s < n_sink ? s : s + (last - s) / window * window;
+// Distance of the token, `rest` slots behind the first one of the window, to the position that slot s in use holds.
+__device__ __forceinline__ int lb_distance(int s, int t, int n_sink, int window, int rest) {
+  const int back = rest - (s - n_sink);
+  return s < n_sink ? t - s : back + (back < 0 ? window : 0);
 }
 __device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {  // upper halves: exact where the values have 8 bits
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
@@ -194,11 +196,13 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
     const int g = i * GP + n % GP;
     const T* row = reinterpret_cast<const T*>(a.q) + b * a.qsb + (h0 + min(g, gn - 1)) * a.qsh;
 #pragma unroll
-    for (int f = 0; f < KF; ++f)
+    for (int f = 0; f < KF; ++f) {
+      float x[8];
+      if (a.q_fast) load8<T, true>(row, KF * h + f, a.d, x);
+      else load8<T, false>(row, KF * h + f, a.d, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int at = DP / 4 * h + 8 * f + e;
-        float rest = g < gn && at < a.d ? to_f32(row[at]) * two : 0.f;
+        float rest = g < gn ? x[e] * two : 0.f;
 #pragma unroll
         for (int p = 0; p < QT; ++p) {
           // parts cut off, not rounded: a finite query has no infinite part
@@ -208,8 +212,9 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
           rest = fine ? rest - part : 0.f;
         }
       }
+    }
   }
-  __syncthreads();
+  lds_barrier();  // (not __syncthreads, which would wait for the block's loads)
 
   const int term = n / GP;
   const float sel1 = term >= 1 ? -1.f : 0.f, sel2 = term >= 2 ? -1.f : 0.f;
@@ -298,7 +303,8 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
         for (int j = 0; j < 4; ++j) {
           float v = y[u][i][j] * sc;
           if (REL) {
-            const int bk = s_lut[min(t - lb_position(min(s0 + 16 * u + 4 * j + h, end - 1), t, a.n_sink, a.window), a.rel.dist())];
+            const int at = min(s0 + 16 * u + 4 * j + h, end - 1);
+            const int bk = s_lut[min(lb_distance(at, t, a.n_sink, a.window, own - a.n_sink), a.rel.dist())];
             v += s_tab[min(i * GP + n % GP, gn - 1) * a.rel.buckets() + bk];
           }
           y[u][i][j] = v;
@@ -487,7 +493,8 @@ template <typename T, int BITS, int DP, int NT, bool REL> static hipError_t deco
   hipLaunchKernelGGL((lowbit_join_kernel<T, DP>), dim3((unsigned)(a.B * a.H)), dim3(128), a.n_split * 4, s, a);
   return hipGetLastError();
 }
-template <typename T, int BITS, int DP> static hipError_t decode_d(const LowbitDecodeArgs& a, hipStream_t s) {
+template <typename T, int BITS, int DP> static hipError_t decode_d(LowbitDecodeArgs a, hipStream_t s) {
+  a.q_fast = a.d % 8 == 0 && (((uintptr_t)a.q | (uintptr_t)(a.qsb * (long long)sizeof(T)) | (uintptr_t)(a.qsh * (long long)sizeof(T))) & 15) == 0;
   const bool two = a.H / a.Hk > LbHeads<T>::GP;
   if (a.table) return two ? decode_l<T, BITS, DP, 2, true>(a, s) : decode_l<T, BITS, DP, 1, true>(a, s);
   return two ? decode_l<T, BITS, DP, 2, false>(a, s) : decode_l<T, BITS, DP, 1, false>(a, s);
