@@ -114,9 +114,9 @@ template <typename T> struct I8Out {
 // Few tokens: the weights go by once.  A workgroup has 16 rows of weights and MT tiles of 16 tokens; its waves share K,
 // in steps of 128 bytes, straight from memory into the operands: lane l holds row l % 16 and the 32 bytes l / 16 of a step
 // (any order of the bytes will do, as long as weights and tokens have the same).
-// OWN: up to I8_OWN tokens, whose codes each workgroup forms itself while its first weights arrive: one launch, and no
-// workspace.
-constexpr int I8_OWN = 4, I8_OWN_K = 8192;
+// OWN: up to I8_OWN short tokens, whose codes each workgroup forms itself, a token a wave, while its first weights arrive:
+// one launch, and no workspace.
+constexpr int I8_OWN = 8, I8_OWN_K = 4096, I8_OWN_N = 4096;
 template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
   constexpr int WAVES = 8, U = 4;  // steps in flight
   __shared__ int s_sum[WAVES][MT][16][17];
@@ -138,39 +138,34 @@ template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_boun
     i32x4 wv[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) weights(wv[u], min(wave + u * WAVES, steps - 1));
-    __shared__ unsigned s_top[I8_OWN][WAVES];
-    constexpr int KEEP = I8_OWN_K / (512 * 8);
-    float e[I8_OWN][KEEP][8];
+    // a token a wave: its largest magnitude, its scale, its codes
+    constexpr int KEEP = I8_OWN_K / (64 * 8);
+    for (int m = wave; m < a.M; m += WAVES) {
+      const T* row = reinterpret_cast<const T*>(a.x) + m * a.xs;
+      Eight<T> e[KEEP];
+      unsigned top = 0;
+      auto look = [&](const Eight<T>& v) {
+        float f[8];
+        lb_floats(v, f);
 #pragma unroll
-    for (int m = 0; m < I8_OWN; ++m)
-      if (m < a.M) {
-        unsigned top = 0;
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+      };
 #pragma unroll
-        for (int k = 0; k < KEEP; ++k) {
-          load8<T, FAST>(reinterpret_cast<const T*>(a.x) + m * a.xs, threadIdx.x + k * 512, a.K, e[m][k]);
+      for (int k = 0; k < KEEP; ++k) load8<FAST>(e[k], row, lane + 64 * k, a.K);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(e[m][k][i]) & 0x7fffffffu);
-        }
-        top = wave_max_u32(top);
-        if (lane == 0) s_top[m][wave] = top;
-      }
-    lds_barrier();
+      for (int k = 0; k < KEEP; ++k) look(e[k]);
+      const float s = i8_scale(wave_max_u32(top)), inv = 1.f / s;
+      if (lane == 0) s_scale[m] = s;
+      auto put = [&](int c, const Eight<T>& v) {
+        float f[8];
+        unsigned q[2];
+        lb_floats(v, f);
+        i8_codes(f, s, inv, q);
+        if (c < steps * 16) *reinterpret_cast<uint2*>(s_x + m * steps * 128 + c * 8) = make_uint2(q[0], q[1]);
+      };
 #pragma unroll
-    for (int m = 0; m < I8_OWN; ++m)
-      if (m < a.M) {
-        unsigned top = 0;
-#pragma unroll
-        for (int v = 0; v < WAVES; ++v) top = max(top, s_top[m][v]);
-        const float s = i8_scale(top), inv = 1.f / s;
-        if (threadIdx.x == 0) s_scale[m] = s;
-#pragma unroll
-        for (int k = 0; k < KEEP; ++k) {
-          const int c = threadIdx.x + k * 512;
-          unsigned q[2];
-          i8_codes(e[m][k], s, inv, q);
-          if (c < steps * 16) *reinterpret_cast<uint2*>(s_x + m * steps * 128 + c * 8) = make_uint2(q[0], q[1]);
-        }
-      }
+      for (int k = 0; k < KEEP; ++k) put(lane + 64 * k, e[k]);
+    }
     lds_barrier();
     const int8_t* x = s_x + min(r, a.M - 1) * steps * 128 + 32 * h;
     for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
@@ -444,8 +439,11 @@ hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, 
   return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
 }
 
-// Which kernel a product takes (0: forms the codes itself and needs no workspace).  Calls (us, codes and product, in a
-// graph) of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and 256 x 256 tiles:
+// Which kernel a product takes (0: forms the codes itself and needs no workspace).  Calls in a graph (us, M x K x N) that
+// form the codes themselves and that take a kernel for them: 1 x 4096 x 4096 7.2, 7.8; 8 x 4096 x 4096 7.2, 9.1; 16 x 4096 x
+// 4096 12.7, 10.1; 1 x 4096 x 11008 15.1, 13.0; 1 x 8192 x 4096 13.2, 11.7; 8 x 512 x 512 5.7, 5.1; 8 x 1024 x 2048 6.3, 6.5.  (A
+// launch less saves 3 us of the caller's time.)  Codes and product of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and
+// 256 x 256 tiles:
 //   M 16, K 4096, N 4096     10.1  10.3  12.3  25.0  50.4
 //   32, 4096, 4096              -  11.9  12.5  25.4  50.5
 //   64, 4096, 4096              -  17.4  12.8  25.9  50.5
@@ -459,7 +457,7 @@ hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, 
 // So: few tokens, or too few tiles to go round, the first; the largest tiles of which there is about one a CU.
 int int8_linear_form(int M, int K, int N) {
   auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
-  if (M <= I8_OWN && K <= I8_OWN_K) return 0;
+  if (M <= I8_OWN && K <= I8_OWN_K && N <= I8_OWN_N) return 0;
   if (M <= 16) return 1;
   if (M <= 32 || tiles(64) < 48) return 2;
   return tiles(256) >= 224 ? 5 : tiles(128) >= 224 ? 4 : 3;
