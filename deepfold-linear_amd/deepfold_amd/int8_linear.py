@@ -20,6 +20,7 @@ from . import _lib
 from ._attn import _unit_inner
 
 MAX_IN = 1 << 17  # a sum of so many products of two codes stays below 2^31
+MAX_ROWS = 1 << 31  # rows of tokens or weights are counted in 32 bits
 
 
 def _dtype_code(what, t):
@@ -57,8 +58,8 @@ def _linear(x, codes, scale, bias):
     y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
     b = None if bias is None else bias.to(x.dtype).contiguous()
     scale = scale.contiguous()
-    p = _lib.Int8LinearParams(_dtype_code("int8_linear", x), xc.data_ptr(), xc.stride(0), codes.data_ptr(), codes.stride(0),
-                              scale.data_ptr(), _lib.ptr(b), y.data_ptr(), M, K, N)
+    row = codes.stride(0) if N > 1 else -(-K // 16) * 16
+    p = _lib.Int8LinearParams(_dtype_code("int8_linear", x), xc.data_ptr(), xc.stride(0), codes.data_ptr(), row, scale.data_ptr(), _lib.ptr(b), y.data_ptr(), M, K, N)
     lib = _lib.load()
     # the tokens' codes, in a workspace of the call's own: calls on other streams and captured graphs cannot share it
     nbytes = lib.dfl_int8_linear_workspace_size(M, K, N)
@@ -132,8 +133,8 @@ def int8_linear(
     _dtype_code(what, x)
     _no_grad(what, x, scale, bias)
     _lib.require_gpu(x, codes, scale, bias)
-    if x.numel() == 0:
-        raise ValueError(f"{what}: no tokens")
+    if x.numel() == 0 or x.numel() // K >= MAX_ROWS or N >= MAX_ROWS:
+        raise ValueError(f"{what}: no tokens, or 2^31 of them or of the weights' rows")
     stride = codes.stride()
     if N == 1:
         stride = (-(-K // 16) * 16, stride[1])

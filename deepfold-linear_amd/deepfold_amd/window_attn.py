@@ -45,6 +45,7 @@ from .rel_pos_bias import edge_array
 
 MAX_HEAD_DIM = 128
 MAX_SINK = 128
+MAX_SLOTS = 1 << 28  # window and rows of a chunk of caches in few bits
 EXACT_KEYS = 256  # rows of at most this many keys need no remainder of o (csrc/window_geometry.h)
 
 
@@ -282,6 +283,8 @@ def _check_codes(what, k_cache, v_cache, B, Hk, d, n_sink):
                     raise ValueError(f"{what}: codes or exponents of the caches share memory")
     window = slots - n_sink
     _check_window(what, window, n_sink)
+    if window > MAX_SLOTS:
+        raise ValueError(f"{what}: window={window} above {MAX_SLOTS}")
     return window
 
 
@@ -494,8 +497,8 @@ def window_cache_fill(
         _lib.require_gpu(K, V, lengths, starts, kc, ke, vc, ve)
         if V.dtype != K.dtype or K.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"{what}: K and V must both be bf16 or both fp32, got {K.dtype} and {V.dtype}")
-        if not 1 <= d <= MAX_HEAD_DIM or N < 1:
-            raise ValueError(f"{what}: K {tuple(K.shape)} is empty, or its head dim above {MAX_HEAD_DIM}")
+        if not 1 <= d <= MAX_HEAD_DIM or not 1 <= N <= MAX_SLOTS:
+            raise ValueError(f"{what}: K {tuple(K.shape)} is empty, or its head dim above {MAX_HEAD_DIM} or rows above {MAX_SLOTS}")
         _check_codes(what, k_cache, v_cache, B, Hk, d, n_sink)
     else:
         _no_grad_inputs(what, K, V, k_cache, v_cache)

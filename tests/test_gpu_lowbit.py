@@ -111,7 +111,7 @@ def test_fill(Hk, N, d, window, n_sink, layout, bits, dtype):
 
     lengths = torch.tensor([N, 0, 1, max(1, N - 5), N + 7, -3, N, N, N, 1], dtype=torch.int64)
     starts = torch.tensor([0, 5, 0, 3, n_sink, 2, -1, 1000, 2**31 + 5, n_sink + window - 1], dtype=torch.int64)
-    starts[8] = 2**31 - 1 if N == 1 else 10**6  # (the last position of all, and one far on)
+    starts[8] = 2**31 - 1 if N == 1 else 2**31 - N // 2  # (the last position that a start can be, positions behind it)
     B = len(lengths)
     k, v = (odd_rows(B, N, Hk, d, s, dtype).transpose(1, 2) for s in (1, 2))
     for start in (None, starts):

@@ -251,6 +251,10 @@ def test_wrappers_refuse(launches):
         (ValueError, lambda: df.window_cache_fill(K, V, LENGTHS, kc, vc, n_sink=1, starts=LENGTHS.float())),
         (ValueError, lambda: df.window_cache_fill(K, V[:, :, :1], LENGTHS, kc, vc, n_sink=1)),
         (ValueError, lambda: df.window_cache_fill(K[:, :, :0], V[:, :, :0], LENGTHS, kc, vc, n_sink=1)),
+        (ValueError, lambda: df.window_cache_fill(*[K[:, :, :1].expand(B, Hk, 2**32 + 5, D)] * 2, LENGTHS, kc, vc, n_sink=1)),
+        (ValueError, lambda: df.window_cache_read(*[df.QuantizedCache(
+            torch.empty(1, 1, 1, 16, dtype=torch.uint8).expand(1, 1, 2**32 + 5, 16),
+            torch.empty(1, 1, 1, 1, dtype=torch.uint8).expand(1, 1, 1, 2**32 + 8), 4)] * 2, LENGTHS[:1], 8)),
         (TypeError, lambda: df.window_cache_fill(K, V.to(BF), LENGTHS, kc, vc, n_sink=1)),
         (TypeError, lambda: df.window_cache_fill(K.half(), V.half(), LENGTHS, kc, vc, n_sink=1)),
         (RuntimeError, lambda: df.window_cache_fill(K.clone().requires_grad_(), V, LENGTHS, kc, vc, n_sink=1)),
@@ -296,6 +300,7 @@ def test_int8_wrappers_refuse(launches):
         (ValueError, lambda: df.int8_linear(x, torch.zeros(20, dtype=torch.int8)[None], s[:1])),
         (ValueError, lambda: df.int8_linear(x, w.t()[:20].t()[:, ::1].t().contiguous().t(), s)),
         (RuntimeError, lambda: df.int8_linear(x.clone().requires_grad_(), w[:, :20], s)),
+        (ValueError, lambda: df.int8_linear(x[:1].expand(2**31, 20), w[:, :20], s)),
         (RuntimeError, lambda: df.int8_linear(x, w[:, :20], s, torch.ones(4).requires_grad_())),
     ]
     for i, (error, call) in enumerate(calls):
@@ -307,6 +312,7 @@ def test_int8_wrappers_refuse(launches):
     assert df.int8_linear(torch.ones(2, 3, 32), w, s).shape == (2, 3, 4)
     assert df.int8_linear(x, torch.zeros(1, 32, dtype=torch.int8)[:, :20], s[:1]).shape == (3, 1)
     assert df.int8_linear(x[0], w[:, :20], s).shape == (4,)
+    assert df.int8_linear(x, w.flatten()[:20].view(1, 20), s[:1]).shape == (3, 1)  # (one row in a longer storage)
     codes, scale = df.quantize_rows(x)
     assert codes.shape == (3, 20) and codes.stride() == (32, 1) and scale.shape == (3,)
     assert df.int8_linear(torch.ones(5, 20), codes, scale).shape == (5, 3)
