@@ -215,7 +215,7 @@ int dfl_quantize_rows(const dfl_quantize_rows_params* p, void* stream) {
 }
 
 size_t dfl_int8_linear_workspace_size(int M, int K, int N) {
-  return linear_ok(M, K, N) && dfl::int8_linear_form(M, K, N) != 0 ? LinearWs(M, K).total : 0;
+  return linear_ok(M, K, N) && dfl::int8_linear_form(M, K, N) > dfl::I8_OWN_32 ? LinearWs(M, K).total : 0;
 }
 
 int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -227,11 +227,11 @@ int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t wor
     if (p->w_stride < p->K || ((uintptr_t)p->w | (uintptr_t)p->w_stride) & 15)
       return fail("w and w_stride must be multiples of 16 bytes, w_stride at least K");
     const int form = dfl::int8_linear_form(p->M, p->K, p->N);
-    if (form >= 3 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
+    if (form >= dfl::I8_TILE_64 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
     dfl::Int8LinearArgs a = {p->x, p->x_stride, nullptr, nullptr, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,
                              0, p->w_stride, p->M, p->K, p->N};
     hipError_t e;
-    if (form != 0) {
+    if (form > dfl::I8_OWN_32) {
       const LinearWs ws(p->M, p->K);
       if (!workspace || workspace_bytes < ws.total) return fail("workspace too small: need %zu bytes", ws.total);
       if ((uintptr_t)workspace & 15) return fail("workspace must be 16-byte aligned");

@@ -7,6 +7,7 @@
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace dfl {
@@ -118,16 +119,16 @@ template <typename T> struct I8Out {
 // Few tokens: the weights go by once.  A workgroup has 16 rows of weights and MT tiles of 16 tokens; its waves share K,
 // in steps of 128 bytes, straight from memory into the operands: lane l holds row l % 16 and the 32 bytes l / 16 of a step
 // (any order of the bytes will do, as long as weights and tokens have the same).
-// OWN: up to I8_OWN short tokens, whose codes each workgroup forms itself, a token a wave, while its first weights arrive:
-// one launch, and no workspace.
-constexpr int I8_OWN = 8, I8_OWN_K = 4096, I8_OWN_N = 4096;
-template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
+// OWN: each workgroup forms its tokens' codes itself, OWN tokens a wave, while its first weights arrive: one launch, and no
+// workspace.  A wave keeps I8_OWN elements: 1 token of 4096, 2 of 2048 or 4 of 1024.
+constexpr int I8_OWN = 4096, I8_OWN_N = 12288;
+template <typename T, int MT, int OWN, bool FAST> __global__ void __launch_bounds__(512) int8_few_kernel(Int8LinearArgs a) {
   constexpr int WAVES = 8, U = 4;  // steps in flight
   __shared__ int s_sum[WAVES][MT][16][17];
-  __shared__ float s_scale[OWN ? I8_OWN : 1];
-  extern __shared__ __align__(16) int8_t s_x[];  // OWN: [M][steps * 128] codes
+  __shared__ float s_scale[16 * MT];
+  extern __shared__ __align__(16) int8_t s_x[];  // OWN: [tokens][steps * 128 + 16] codes
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, h = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = OWN ? 0 : blockIdx.y * (16 * MT);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
   const int8_t* w = a.w + (long long)min(n0 + r, a.N - 1) * a.ws;
   const int steps = (a.K + 127) / 128, tail = ((a.K + 15) & ~15) - 16;  // last 16 bytes of a row of weights
   auto weights = [&](i32x4 (&v)[2], int s) {
@@ -142,44 +143,55 @@ template <typename T, int MT, bool OWN, bool FAST> __global__ void __launch_boun
     i32x4 wv[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) weights(wv[u], min(wave + u * WAVES, steps - 1));
-    // a token a wave: its largest magnitude, its scale, its codes
-    constexpr int KEEP = I8_OWN_K / (64 * 8);
-    for (int m = wave; m < a.M; m += WAVES) {
-      const T* row = reinterpret_cast<const T*>(a.x) + m * a.xs;
-      Eight<T> e[KEEP];
+    // OWN tokens a wave: the largest magnitude, the scale, the codes of each
+    constexpr int KEEP = I8_OWN / OWN / (64 * 8);
+    const int tokens = min(a.M - m0, 16 * MT), stride = steps * 128 + 16;
+    Eight<T> e[OWN][KEEP];
+#pragma unroll
+    for (int t = 0; t < OWN; ++t) {  // (a wave without a token takes the last one, and stores nothing)
+      const T* row = reinterpret_cast<const T*>(a.x) + (m0 + min(wave + t * WAVES, tokens - 1)) * a.xs;
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k) load8<FAST>(e[t][k], row, lane + 64 * k, a.K);
+    }
+#pragma unroll
+    for (int t = 0; t < OWN; ++t) {
+      const int m = wave + t * WAVES;
+      if (m >= tokens) continue;
       unsigned top = 0;
-      auto look = [&](const Eight<T>& v) {
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k) {
         float f[8];
-        lb_floats(v, f);
+        lb_floats(e[t][k], f);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-      };
-#pragma unroll
-      for (int k = 0; k < KEEP; ++k) load8<FAST>(e[k], row, lane + 64 * k, a.K);
-#pragma unroll
-      for (int k = 0; k < KEEP; ++k) look(e[k]);
+      }
       const float s = i8_scale(wave_max_u32(top)), inv = 1.f / s;
       if (lane == 0) s_scale[m] = s;
-      auto put = [&](int c, const Eight<T>& v) {
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k) {
+        const int c = lane + 64 * k;
         float f[8];
         unsigned q[2];
-        lb_floats(v, f);
+        lb_floats(e[t][k], f);
         i8_codes(f, s, inv, q);
-        if (c < steps * 16) *reinterpret_cast<uint2*>(s_x + m * steps * 128 + c * 8) = make_uint2(q[0], q[1]);
-      };
-#pragma unroll
-      for (int k = 0; k < KEEP; ++k) put(lane + 64 * k, e[k]);
+        if (c < steps * 16) *reinterpret_cast<uint2*>(s_x + m * stride + c * 8) = make_uint2(q[0], q[1]);
+      }
     }
     lds_barrier();
-    const int8_t* x = s_x + min(r, a.M - 1) * steps * 128 + 32 * h;
+    const int8_t* x[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = s_x + min(16 * i + r, tokens - 1) * stride + 32 * h;
     for (int s0 = wave; s0 < steps; s0 += WAVES * U) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int s = s0 + u * WAVES;
         if (s < steps) {
-          const i32x4* xv = reinterpret_cast<const i32x4*>(x + s * 128);
-          sum[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][0], xv[0], sum[0], 0, 0, 0);
-          sum[0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][1], xv[1], sum[0], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const i32x4* xv = reinterpret_cast<const i32x4*>(x[i] + s * 128);
+            sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][0], xv[0], sum[i], 0, 0, 0);
+            sum[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][1], xv[1], sum[i], 0, 0, 0);
+          }
         }
         if (s + WAVES * U < steps) weights(wv[u], s + WAVES * U);
       }
@@ -419,23 +431,26 @@ template <typename T, int TM, int TN, int WM, int WN, int BUF> static hipError_t
 }
 template <typename T, int MT> static hipError_t few_t(const Int8LinearArgs& a, hipStream_t s) {
   const dim3 grid((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT));
-  hipLaunchKernelGGL((int8_few_kernel<T, MT, false, false>), grid, dim3(512), 0, s, a);
+  hipLaunchKernelGGL((int8_few_kernel<T, MT, 0, false>), grid, dim3(512), 0, s, a);
   return hipGetLastError();
 }
-template <typename T> static hipError_t own_t(const Int8LinearArgs& a, hipStream_t s) {
+template <typename T, int MT, int OWN> static hipError_t own_t(const Int8LinearArgs& a, hipStream_t s) {
   const bool fast = a.K % 8 == 0 && aligned16<T>(a.x, {a.xs});
-  const size_t lds = (size_t)a.M * ((a.K + 127) / 128 * 128);
-  if (fast) hipLaunchKernelGGL((int8_few_kernel<T, 1, true, true>), dim3((a.N + 15) / 16), dim3(512), lds, s, a);
-  else hipLaunchKernelGGL((int8_few_kernel<T, 1, true, false>), dim3((a.N + 15) / 16), dim3(512), lds, s, a);
+  const size_t lds = (size_t)std::min(a.M, 16 * MT) * ((a.K + 127) / 128 * 128 + 16);
+  const dim3 grid((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT));
+  if (fast) hipLaunchKernelGGL((int8_few_kernel<T, MT, OWN, true>), grid, dim3(512), lds, s, a);
+  else hipLaunchKernelGGL((int8_few_kernel<T, MT, OWN, false>), grid, dim3(512), lds, s, a);
   return hipGetLastError();
 }
 template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int form, hipStream_t s) {
   switch (form) {
-    case 0: return own_t<T>(a, s);
-    case 1: return few_t<T, 1>(a, s);
-    case 2: return few_t<T, 2>(a, s);
-    case 3: return tile_t<T, 64, 64, 2, 2, 4>(a, s);
-    case 4: return tile_t<T, 128, 128, 2, 2, 2>(a, s);
+    case I8_OWN_8: return own_t<T, 1, 1>(a, s);
+    case I8_OWN_16: return own_t<T, 1, 2>(a, s);
+    case I8_OWN_32: return own_t<T, 2, 4>(a, s);
+    case I8_FEW_16: return few_t<T, 1>(a, s);
+    case I8_FEW_32: return few_t<T, 2>(a, s);
+    case I8_TILE_64: return tile_t<T, 64, 64, 2, 2, 4>(a, s);
+    case I8_TILE_128: return tile_t<T, 128, 128, 2, 2, 2>(a, s);
     default: return tile_t<T, 256, 256, 2, 4, 2>(a, s);
   }
 }
@@ -443,11 +458,11 @@ hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, 
   return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
 }
 
-// Which kernel a product takes (0: forms the codes itself and needs no workspace).  Calls in a graph (us, M x K x N) that
-// form the codes themselves and that take a kernel for them: 1 x 4096 x 4096 7.2, 7.8; 8 x 4096 x 4096 7.2, 9.1; 16 x 4096 x
-// 4096 12.7, 10.1; 1 x 4096 x 11008 15.1, 13.0; 1 x 8192 x 4096 13.2, 11.7; 8 x 512 x 512 5.7, 5.1; 8 x 1024 x 2048 6.3, 6.5.  (A
-// launch less saves 3 us of the caller's time.)  Codes and product of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and
-// 256 x 256 tiles:
+// Which kernel a product takes.  Calls in a graph (us, M x K x N) that form the codes in the product's workgroups and that take a
+// kernel for them: 1 x 4096 x 4096 5.6, 7.4; 8 x 4096 x 4096 8.2, 9.0; 8 x 2048 x 4096 6.2, 9.0; 16 x 2048 x 4096 8.0, 9.7;
+// 16 x 512 x 512 6.1, 5.4; 32 x 1024 x 4096 7.7, 8.9; 300 x 1024 x 300 8.4, 9.5; 97 x 64 x 64 5.8, 5.4; 1 x 4096 x 11008 11.4, 12.5;
+// 8 x 4096 x 11008 16.6, 15.6; 4 x 512 x 32768 20.6, 12.1.  (A launch less saves 3 us of the caller's time besides.)
+// Codes and product of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and 256 x 256 tiles:
 //   M 16, K 4096, N 4096     10.1  10.3  12.3  25.0  50.4
 //   32, 4096, 4096              -  11.9  12.5  25.4  50.5
 //   64, 4096, 4096              -  17.4  12.8  25.9  50.5
@@ -461,10 +476,13 @@ hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, 
 // So: few tokens, or too few tiles to go round, the first; the largest tiles of which there is about one a CU.
 int int8_linear_form(int M, int K, int N) {
   auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
-  if (M <= I8_OWN && K <= I8_OWN_K && N <= I8_OWN_N) return 0;
-  if (M <= 16) return 1;
-  if (M <= 32 || tiles(64) < 48) return 2;
-  return tiles(256) >= 224 ? 5 : tiles(128) >= 224 ? 4 : 3;
+  if (M <= 32 || tiles(64) < 48) {
+    if (N <= I8_OWN_N && M <= 8 && K <= I8_OWN) return I8_OWN_8;
+    if (N <= I8_OWN_N && M <= 16 && K <= I8_OWN / 2) return I8_OWN_16;
+    if (N <= I8_OWN_N && M > 16 && K <= I8_OWN / 4) return I8_OWN_32;
+    return M <= 16 ? I8_FEW_16 : I8_FEW_32;
+  }
+  return tiles(256) >= 224 ? I8_TILE_256 : tiles(128) >= 224 ? I8_TILE_128 : I8_TILE_64;
 }
 
 }  // namespace dfl

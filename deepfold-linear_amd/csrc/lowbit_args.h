@@ -67,8 +67,11 @@ struct RowCodesArgs {
   int K;
 };
 
+// Kernels of the product: codes formed in it, or by a kernel before; tiles of 16 or 32 tokens and 16 rows of weights, or square.
+enum Int8Form { I8_OWN_8, I8_OWN_16, I8_OWN_32, I8_FEW_16, I8_FEW_32, I8_TILE_64, I8_TILE_128, I8_TILE_256 };
+
 struct Int8LinearArgs {
-  const void* x;    // (M,K) tokens, element stride (the form that makes the codes itself)
+  const void* x;    // (M,K) tokens, element stride (I8_OWN_*)
   long long xs;
   const int8_t* a;  // (M, as) codes of the tokens, zeros from K on; as a multiple of 128
   const float* a_scale;

@@ -55,7 +55,9 @@ def case(M, K, N, dtype, bias=True, x=None, seed=1):
 @pytest.mark.parametrize("M,K,N", [(1, 1, 1), (1, 64, 16), (2, 15, 17), (3, 16, 33), (15, 17, 1), (16, 63, 64), (17, 65, 100), (31, 127, 48),
                                    (32, 128, 15), (33, 200, 70), (48, 1000, 31), (64, 512, 129), (65, 48, 64), (65, 513, 200), (97, 512, 512),
                                    (128, 100, 65), (129, 64, 63), (200, 2100, 130), (1, 4097, 20), (5, 9000, 18), (70, 8200, 66),
-                                   (5, 4096, 40), (8, 4095, 33), (7, 520, 300), (9, 4096, 17), (6, 100, 4097), (8, 64, 4096)])
+                                   (5, 4096, 40), (8, 4095, 33), (7, 520, 300), (9, 4096, 17), (6, 100, 4097), (8, 64, 4096), (9, 2048, 50),
+                                   (16, 2049, 33), (13, 2047, 4096), (16, 1000, 97), (33, 1024, 40), (17, 1025, 40), (100, 1023, 300),
+                                   (2, 20, 12289), (24, 8, 12289), (700, 640, 200)])
 def test_linear(M, K, N, dtype):
     case(M, K, N, dtype, bias=(M + K + N) % 2 == 0)
 

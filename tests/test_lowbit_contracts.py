@@ -125,11 +125,15 @@ def test_workspaces():
     assert b"workspace too small" in lib.dfl_last_error()
     assert lib.dfl_lowbit_decode(ctypes.byref(decode_params()), None, need, None) < 0
     assert lib.dfl_int8_linear_workspace_size(4, 60, 8) == 0  # (few tokens: none is needed)
-    need = lib.dfl_int8_linear_workspace_size(9, 60, 8)
-    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), FAKE, need - 1, None) < 0
+    for a in ((8, 4096, 8), (16, 2048, 8), (100, 1024, 8)):
+        assert lib.dfl_int8_linear_workspace_size(*a) == 0, a
+    for a in ((8, 4097, 8), (9, 2049, 8), (17, 1025, 8), (1, 64, 2**20)):
+        assert lib.dfl_int8_linear_workspace_size(*a) > 0, a
+    need = lib.dfl_int8_linear_workspace_size(9, 4100, 8)
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9, K=4100, x_stride=4104, w_stride=4112)), FAKE, need - 1, None) < 0
     assert b"workspace too small" in lib.dfl_last_error()
-    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), FAKE + 8, need, None) < 0
-    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9)), None, need, None) < 0
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9, K=4100, x_stride=4104, w_stride=4112)), FAKE + 8, need, None) < 0
+    assert lib.dfl_int8_linear(ctypes.byref(linear_params(M=9, K=4100, x_stride=4104, w_stride=4112)), None, need, None) < 0
 
 
 class Launches:
