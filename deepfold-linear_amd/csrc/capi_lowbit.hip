@@ -46,6 +46,7 @@ template <class F> int guarded(F f) {
 constexpr long long MAX_N = 1ll << 28;   // positions and their differences stay well inside 32 bits
 constexpr long long MAX_BH = 1ll << 22;
 constexpr int MAX_SINK = 128, MAX_K = 1 << 17;  // 2^17 products of two codes: below 2^31
+constexpr int MAX_ROWS = 0x7fffff00;  // tokens, rows of weights: a tile that begins below it ends below 2^31
 
 int pad_dim(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 size_t r256(size_t n) { return (n + 255) / 256 * 256; }
@@ -226,6 +227,7 @@ int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t wor
     if (!p->x || !p->w || !p->w_scale || !p->y) return fail("required pointer is NULL");
     if (p->w_stride < p->K || ((uintptr_t)p->w | (uintptr_t)p->w_stride) & 15)
       return fail("w and w_stride must be multiples of 16 bytes, w_stride at least K");
+    if (p->M > MAX_ROWS || p->N > MAX_ROWS) return fail("M=%d, N=%d: at most %d", p->M, p->N, MAX_ROWS);
     const int form = dfl::int8_linear_form(p->M, p->K, p->N);
     if (form >= dfl::I8_TILE_64 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
     dfl::Int8LinearArgs a = {p->x, p->x_stride, nullptr, nullptr, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,

@@ -475,7 +475,7 @@ hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, 
 //   4096, 4096, 4096            -   694   128   102  81.9
 // So: few tokens, or too few tiles to go round, the first; the largest tiles of which there is about one a CU.
 int int8_linear_form(int M, int K, int N) {
-  auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
+  auto tiles = [&](int t) { return ((M + t - 1ll) / t) * ((N + t - 1ll) / t); };
   if (M <= 32 || tiles(64) < 48) {
     if (N <= I8_OWN_N && M <= 8 && K <= I8_OWN) return I8_OWN_8;
     if (N <= I8_OWN_N && M <= 16 && K <= I8_OWN / 2) return I8_OWN_16;

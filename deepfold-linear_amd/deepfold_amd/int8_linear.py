@@ -20,7 +20,7 @@ from . import _lib
 from ._attn import _unit_inner
 
 MAX_IN = 1 << 17  # a sum of so many products of two codes stays below 2^31
-MAX_ROWS = 1 << 31  # rows of tokens or weights are counted in 32 bits
+MAX_ROWS = (1 << 31) - 256  # rows of tokens or weights, and the ends of their tiles, are counted in 32 bits
 
 
 def _dtype_code(what, t):
@@ -133,8 +133,8 @@ def int8_linear(
     _dtype_code(what, x)
     _no_grad(what, x, scale, bias)
     _lib.require_gpu(x, codes, scale, bias)
-    if x.numel() == 0 or x.numel() // K >= MAX_ROWS or N >= MAX_ROWS:
-        raise ValueError(f"{what}: no tokens, or 2^31 of them or of the weights' rows")
+    if x.numel() == 0 or x.numel() // K > MAX_ROWS or N > MAX_ROWS:
+        raise ValueError(f"{what}: no tokens, or above {MAX_ROWS} of them or of the weights' rows")
     stride = codes.stride()
     if N == 1:
         stride = (-(-K // 16) * 16, stride[1])

@@ -25,6 +25,10 @@ single-token form, on MI355X.
       window_cache_fill(K, V, chunk, k_cache, v_cache, n_sink=s, starts=lengths)   # chunk: rows of each sample
       lengths += chunk
 
+  Chunks of at most ``window`` rows are right from any lengths on (0 too); longer ones where the caches hold the n_sink
+  first tokens already: those that come with a chunk stand at its rows, not at the first n_sink, and are seen no further
+  than the window.
+
 Where ``flash_atom_attn`` has fixed windows of 32 queries and 128 keys, here the window
 moves with the query.  The reference has no counterpart.  bf16 runs on bf16 MFMA with fp32
 sums, any other type in fp32, as in the other attention ops; CPU tensors raise.
@@ -533,7 +537,8 @@ def window_cache_read(
     j, any other row position lengths[b] - (n_sink + window) + j: the last ``window`` positions end with the last row.  Rows
     that have no such position (short sequences, lengths below 1) are zero and masked: 0.  The caches may be tensors
     (``dtype`` is theirs) or in few bits (``dtype`` bf16 or fp32, by default bf16, in which every code is
-    exact).  Distances between the first tokens and the others are those of the rows, not of the positions: a table of
+    exact).  The rows that follow may be more than ``window`` only where
+    lengths[b] >= n_sink (module docstring).  Distances between the first tokens and the others are those of the rows, not of the positions: a table of
     relative biases that goes on beyond the window sees them nearer.  No gradient."""
     what = "window_cache_read"
     n_sink = int(n_sink)

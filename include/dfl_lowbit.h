@@ -93,7 +93,7 @@ typedef struct dfl_quantize_rows_params {
 
 /* y (M,N) contiguous in `dtype`: y[m,n] = (sum_k a[m,k] w[n,k]) s[m] w_scale[n] + bias[n] with a, s the codes and
  * scale of x's rows as in dfl_quantize_rows and w (N,K) int8 codes; bias in `dtype` or NULL.  The sum is exact (K at
- * most 131072).  w and its row stride (bytes) are multiples of 16, and a row's bytes up to the next multiple of 16 from K
+ * most 131072; M and N at most 2^31 - 256).  w and its row stride (bytes) are multiples of 16, and a row's bytes up to the next multiple of 16 from K
  * on are read, whatever they hold. */
 typedef struct dfl_int8_linear_params {
   int dtype;

@@ -374,6 +374,33 @@ def test_a_long_cache():
     assert all(torch.equal(x, y) for x, y in zip(*out))
 
 
+def test_chunks_before_the_first_tokens():
+    """Chunks as long as the window for samples without, with a part of and with all of the first tokens, then a longer one."""
+    from deepfold_amd import flash_window_attn, quantized_cache, window_cache_fill, window_cache_read
+
+    B, H, Hk, d, window, n_sink, bits = 4, 4, 2, 32, 20, 4, 8
+    kc, vc = (quantized_cache(B, Hk, n_sink + window, d, bits=bits, device=DEV) for _ in range(2))
+    held = [[torch.zeros(Hk, 0, d) for _ in range(B)] for _ in range(2)]
+    lengths = torch.zeros(B, dtype=torch.int32, device=DEV)
+    for step, rows in enumerate(([0, 2, 3, 4], [window] * 4, [2 * window + 1, 2 * window + 1, 7, 0])):
+        n = max(rows)
+        q, k, v = (rnd(B, h, n, d, seed=20 * step + i) for i, h in enumerate((H, Hk, Hk)))
+        chunk = torch.tensor(rows, device=DEV, dtype=torch.int32)
+        mine = (torch.arange(n, device=DEV)[None] < chunk[:, None]).float()
+        kp, vp, m = window_cache_read(kc, vc, lengths, d, n_sink=n_sink, dtype=F32)
+        o = flash_window_attn(q.to(DEV), torch.cat((kp, k.to(DEV)), 2), torch.cat((vp, v.to(DEV)), 2), torch.cat((m, mine), 1),
+                              window=window, n_sink=n_sink)
+        window_cache_fill(k.to(DEV), v.to(DEV), chunk, kc, vc, n_sink=n_sink, starts=lengths)
+        for b in range(B):
+            if rows[b]:
+                whole = [torch.cat((h[b], x[b, :, :rows[b]]), 1)[None] for h, x in zip(held, (k, v))]
+                want = plain_ref.attention(q[b:b + 1, :, :rows[b]], *whole, window=window, n_sink=n_sink, operand=F32, result=F32)["o"]
+                holds("chunk", o[b:b + 1, :, :rows[b]], *want)
+            for h, x in zip(held, (k, v)):
+                h[b] = torch.cat((h[b], ref.values(*ref.encode(x[b], bits), d, bits)[:, :rows[b]].to(F32)), 1)
+        lengths += chunk
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_chunks_then_tokens(dtype, bits):

@@ -90,7 +90,7 @@ CODES = [dict(bits=5), dict(bits=16), dict(k_cache=codes(codes=None)), dict(v_ca
                            dict(scale=None), dict(code_stride=48), dict(code_stride=72), dict(codes=FAKE + 4)]),
     ("linear", linear_params, [dict(dtype=2), dict(M=0), dict(K=0), dict(N=0), dict(M=-1), dict(K=2**17 + 1, w_stride=2**18), dict(x=None),
                                dict(w=None), dict(w_scale=None), dict(y=None), dict(w_stride=48), dict(w_stride=72),
-                               dict(w=FAKE + 8), dict(M=2**31 - 1, N=2**31 - 1)]),
+                               dict(w=FAKE + 8), dict(M=2**31 - 1, N=2**31 - 1), dict(M=2**31 - 255), dict(N=2**31 - 1)]),
 ])
 def test_entries_refuse(entry, make, bad):
     """Every refusal comes before any launch (the pointers are no memory)."""
