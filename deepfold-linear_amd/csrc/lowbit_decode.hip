@@ -508,10 +508,14 @@ hipError_t launch_lowbit_decode(const LowbitDecodeArgs& a, bool bf16_in, int bit
 }
 
 // How a call is cut up.  A workgroup of 4 lb_waves waves has a CU to itself; smaller ones share it.
-//  * Caches of up to four blocks of 32 slots a wave of such a workgroup: one workgroup for all of it, whose one launch
+//  * More workgroups than CUs: of 4 waves, so that one's first loads and last sums pass beside another's work (4 bits, 64 x
+//    16 / 16 heads of 2052 slots, d 64, 47.4 us with workgroups of 12 and 38.9 of 4; of 300 slots 25.5, 12.2; 64 x 32 / 8, 8200
+//    slots, d 128 104.6, 101.4), unless the cache is long and its last round would leave a fifth of the CUs idle (below).
+//  * Else caches of up to four blocks of 32 slots a wave of a large workgroup: one workgroup for all of it, whose one launch
 //    is shorter than two.
-//  * As many of these workgroups as CUs, or nearly: no split either, or as many splits as make that many.
-//  * Else workgroups of 4 waves, which fill the CUs in any number.
+//  * As many of the large workgroups as CUs, or nearly: no split either (32 x 32 / 8 heads of 4100 slots, d 128 29.2 us, of 4
+//    waves 39.0), or as many splits as make that many.
+//  * Else splits in workgroups of 4 waves, which fill the CUs in any number (48 x 32 / 8 heads 42.7 us, not split 47.4).
 LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S) {
   const int DP = d <= 32 ? 32 : d <= 64 ? 64 : 128, G = H / Hk, gp = bf16_in ? LbHeads<bf16>::GP : LbHeads<float>::GP;
   const int NT = G > gp ? 2 : 1, per = lb_waves(bf16_in ? 2 : 4, DP, NT), big = 4 * per, blocks = (S + 31) / 32;
@@ -520,9 +524,12 @@ LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S) 
   const long long wg = (long long)B * Hk * ((G + p.heads - 1) / p.heads), rounds = (wg + CUS - 1) / CUS;
   long long n = 1;
   p.waves = big;
-  if (blocks <= 4 * big) {
+  const bool uneven = wg * 5 < rounds * CUS * 4;
+  if (wg > CUS && (blocks <= 4 * big || !uneven)) {
+    p.waves = 4;
+  } else if (blocks <= 4 * big) {
     p.waves = std::min(big, (blocks + 3) / 4 * 4);
-  } else if (wg * 5 < rounds * CUS * 4) {
+  } else if (uneven) {
     n = CUS / wg;
     if (n * wg * 5 < CUS * 4) {
       p.waves = 4;

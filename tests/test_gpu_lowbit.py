@@ -261,6 +261,15 @@ def test_decode_lengths(bits, dtype):
         decode_case(4, 2, 64, window, n_sink, False, bits, dtype, "own", lengths[lengths < 3 * S])
 
 
+@pytest.mark.parametrize("dtype,bits", [(BF, 4), (F32, 8)])
+@pytest.mark.parametrize("B,H,Hk,d,window,n_sink", [(129, 4, 2, 24, 45, 3), (86, 3, 3, 64, 300, 0), (100, 3, 3, 8, 1600, 1),
+                                                    (150, 6, 3, 8, 1600, 0)])
+def test_decode_many_sequences(B, H, Hk, d, window, n_sink, bits, dtype):
+    """More samples and key heads than CUs, with short and long caches, as many as fill the CUs again and fewer."""
+    lengths = torch.randint(-1, 3 * window, (B,), generator=torch.Generator().manual_seed(B))
+    decode_case(H, Hk, d, window, n_sink, False, bits, dtype, "own", lengths)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_decode_sharp_scores(bits, dtype):
