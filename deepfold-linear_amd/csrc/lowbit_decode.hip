@@ -45,7 +45,7 @@ __device__ __forceinline__ int lb_distance(int s, int t, int n_sink, int window,
   const int back = rest - (s - n_sink);
   return s < n_sink ? t - s : back + (back < 0 ? window : 0);
 }
-__device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {  // upper halves: exact where the values have 8 bits
+__device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {  // upper halves: exact where the values have 8 bits, else cut off
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
@@ -200,16 +200,17 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
       float x[8];
       if (a.q_fast) load8<T, true>(row, KF * h + f, a.d, x);
       else load8<T, false>(row, KF * h + f, a.d, x);
+      // Parts cut off, not rounded: a finite query has no infinite part.  (x * two is a quiet NaN where x is one, and stays
+      // one cut off.)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float rest = g < gn ? x[e] * two : 0.f;
+      for (int e = 0; e < 8; e += 2) {
+        float lo = x[e] * two, hi = x[e + 1] * two;
+        const bool finite_lo = fabsf(lo) < INFINITY, finite_hi = fabsf(hi) < INFINITY;
 #pragma unroll
         for (int p = 0; p < QT; ++p) {
-          // parts cut off, not rounded: a finite query has no infinite part
-          const bool fine = fabsf(rest) < INFINITY;
-          const float part = fine ? __uint_as_float(__float_as_uint(rest) & 0xffff0000u) : rest;
-          q[i][p][f].v[e] = (bf16)part;
-          rest = fine ? rest - part : 0.f;
+          q[i][p][f].u[e / 2] = g < gn ? bf16_pair(lo, hi) : 0u;
+          lo = finite_lo ? lo - __uint_as_float(__float_as_uint(lo) & 0xffff0000u) : 0.f;
+          hi = finite_hi ? hi - __uint_as_float(__float_as_uint(hi) & 0xffff0000u) : 0.f;
         }
       }
     }
