@@ -420,27 +420,38 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
       }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < gn * DP; e += blockDim.x) {
-    const int g = e / DP, col = e % DP;
+  // (A thread's columns: of many heads four, so that no thread does this twice: 16 x 16 / 1 heads of 8196 slots 18.6 -> 16.9 us;
+  // of few one, 1 x 16 / 4 heads 9.2 and 9.4 with four.)
+  constexpr int CW = NT == 2 ? 4 : 1;
+  typedef __attribute__((__vector_size__(CW * sizeof(float)))) float cols;
+  for (int e = threadIdx.x; e < gn * (DP / CW); e += blockDim.x) {
+    const int g = e / (DP / CW), col = e % (DP / CW) * CW;
     float mx = NEG_BIG;
     for (int r = 0; r < waves; r += 4)  // (a multiple of 4)
 #pragma unroll
       for (int k = 0; k < 4; ++k) mx = fmaxf(mx, s_ml[((r + k) * GB + g) * 2]);
-    float sl = 0.f, so = 0.f;
+    float sl = 0.f;
+    cols so = {};
     for (int r = 0; r < waves; r += 4)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float al = fast_exp2(s_ml[((r + k) * GB + g) * 2] - mx);
+        const cols v = *reinterpret_cast<const cols*>(s_o + ((r + k) * GB + g) * DP + col);
         sl = __builtin_fmaf(s_ml[((r + k) * GB + g) * 2 + 1], al, sl);
-        so = __builtin_fmaf(s_o[((r + k) * GB + g) * DP + col], al, so);
+#pragma unroll
+        for (int c = 0; c < CW; ++c) so[c] = __builtin_fmaf(v[c], al, so[c]);
       }
     const size_t head = (size_t)b * a.H + h0 + g;
     if (a.n_split == 1) {
-      if (col < a.d) reinterpret_cast<T*>(a.o)[head * a.d + col] = from_f32<T>(sl == 0.f ? 0.f : so / sl);
+      T* o = reinterpret_cast<T*>(a.o) + head * a.d + col;
+#pragma unroll
+      for (int c = 0; c < CW; ++c)
+        if (col + c < a.d) o[c] = from_f32<T>(sl == 0.f ? 0.f : so[c] / sl);
     } else {
       float* part = a.part + (head * a.n_split + sp) * (DP + 2);
       if (col == 0) part[0] = mx, part[1] = sl;
-      part[2 + col] = so;
+#pragma unroll
+      for (int c = 0; c < CW; ++c) part[2 + col + c] = so[c];
     }
   }
 }
