@@ -1,5 +1,6 @@
-// Issue-rate and exchange probes behind the forward's roofline figures (a separate
-// library, libdfl_peaks.so, loaded only by bench.py --workload peaks; nothing in the
+// Issue-rate and exchange probes behind the forward's roofline figures, and a probe of
+// what a buffer load takes to be out of range (a separate library, libdfl_peaks.so,
+// loaded only by bench.py --workload peaks and by that rule's test; nothing in the
 // product calls it).  Every probe runs one 512-thread workgroup per CU (the dynamic
 // LDS request keeps a second one off the CU), i.e. two waves per SIMD as in the
 // Sinkhorn kernels, on `blocks` workgroups.
@@ -114,6 +115,32 @@ hipError_t lds_limit(K kern) {
 // multiple of 8, one group per XCD slot), `iters` rounds (<= 4000).
 // Writes the launch's event time (ms) and workgroup 0's clock64() span; returns a
 // hipError_t, or 1000 + 2 if an exchange wait expired.
+namespace dfl {
+namespace {
+// A load of 16 bytes and one of a byte at each of 64 lane offsets and one scalar offset a workgroup.
+__global__ void __launch_bounds__(64) buffer_range_kernel(const unsigned char* base, int bytes, const unsigned* lanes,
+                                                          const unsigned* scalars, unsigned* out) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(base), 0, bytes, 0x00020000);
+  const unsigned lane = lanes[threadIdx.x], scalar = __builtin_amdgcn_readfirstlane(scalars[blockIdx.x]);
+  const auto x = __builtin_amdgcn_raw_buffer_load_b128(r, lane, scalar, 0);
+  unsigned* to = out + (blockIdx.x * 64 + threadIdx.x) * 5;
+  to[0] = x[0], to[1] = x[1], to[2] = x[2], to[3] = x[3];
+  to[4] = __builtin_amdgcn_raw_buffer_load_b8(r, lane, scalar, 0);
+}
+}  // namespace
+}  // namespace dfl
+
+// A resource of `bytes` bytes from base on, n workgroups: out (n,64,5), the 16 bytes and the byte of each load.  The memory
+// at base + lanes[i] + scalars[j] .. + 15 must be there for every pair, whatever the rule.  (All pointers on the device.)
+extern "C" int dfl_probe_buffer_range(const void* base, int bytes, const unsigned* lanes, const unsigned* scalars, int n,
+                                      unsigned* out) {
+  if (!base || bytes < 0 || !lanes || !scalars || n <= 0 || n > 65535 || !out) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL(dfl::buffer_range_kernel, dim3(n), dim3(64), 0, 0, static_cast<const unsigned char*>(base), bytes, lanes,
+                     scalars, out);
+  const hipError_t e = hipGetLastError();
+  return (int)(e != hipSuccess ? e : hipDeviceSynchronize());
+}
+
 extern "C" int dfl_peak_run(int mode, int blocks, int iters, float* out_ms, long long* out_clk) {
   using namespace dfl;
   if (blocks <= 0 || iters <= 0 || mode < 0 || mode > 4) return (int)hipErrorInvalidValue;
