@@ -36,8 +36,17 @@ template <typename T> struct LbHeads {
 constexpr int lb_waves(int size, int DP, int NT) {
   return DP < 128 ? (NT == 2 ? 2 : 3) : NT == 2 ? (size == 4 ? 1 : 2) : (size == 4 ? 2 : 3);
 }
+// Small workgroups overlap on a CU (lowbit_decode_plan): of bf16 rows of at most 64 elements the registers are held down to
+// four waves a SIMD (64 x 16 / 16 heads of 2052 slots, 4 bits 51 us with three).
+constexpr int lb_least_waves(int size, int DP, int NT) { return size == 2 && DP < 128 && NT == 1 ? 4 : lb_waves(size, DP, NT); }
 // A reference is moved when a score passes it by more than this: weights stay below 2^8.
 constexpr float LB_LAZY = 8.f;
+// With S <= 2^c slots, sums of weights times values stay below 2^126 as long as the values' exponents lie below 239 - c (a
+// code has 7 bits).  A wave that has met a higher one goes through its slots again with a reference c + 10 above the largest
+// score: values below 2^128 then make no more of a sum either, and the join needs to know nothing of it.  (Weights below
+// 2^(c - 116) of the largest vanish there.)
+__device__ __forceinline__ int lb_lift(int S) { return 42 - __clz(S - 1); }
+__device__ __forceinline__ unsigned lb_high(int S) { return 249u - lb_lift(S); }
 constexpr long long CUS = 256;
 
 // Distance of the token, `rest` slots behind the first one of the window, to the position that slot s in use holds.
@@ -89,7 +98,8 @@ union LbFrag {
 };
 
 template <typename T, int BITS, int DP, int NT, bool REL>
-__global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(sizeof(T), DP, NT)) lowbit_decode_kernel(LowbitDecodeArgs a) {
+__global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_least_waves(sizeof(T), DP, NT))
+    lowbit_decode_kernel(LowbitDecodeArgs a) {
   using Hd = LbHeads<T>;
   constexpr int GP = Hd::GP, QT = Hd::QT, GB = NT * GP;
   constexpr int KF = DP / 32;            // matrix instructions of a score tile; fragments of a lane's quarter row
@@ -234,6 +244,7 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
   }
 
   f32x4 none[2] = {};  // what the scores of a block start from
+  float slack = LB_LAZY;
   auto step = [&](int s0) {
     if (mine && s0 <= own && own < s0 + 32) {  // the token's own slot, as its codes stand
       const int at = own - s0;
@@ -315,8 +326,8 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
           y[u][i][j] = v;
           mx = fmaxf(mx, v);
         }
-      if (__any(mx > m[i] + LB_LAZY)) {
-        mx = max_groups(fmaxf(mx, m[i]));
+      if (__any(mx > m[i] + slack)) {
+        mx = max_groups(fmaxf(mx + (LB_LAZY - slack), m[i]));
         const float al = fast_exp2(m[i] - mx);
         m[i] = mx;
         l[i] *= al;
@@ -395,12 +406,22 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_waves(si
       }
     }
   };
-  {
+  for (;;) {
     // the next block's keys are loaded once this one's are used, its values likewise
     for (int s0 = first; s0 < end; s0 += stride) {
       step(s0);
       if (s0 + stride < end) load_values(s0 + stride);
     }
+    if (slack != LB_LAZY || !__any(top >= lb_high(S)) || __any(top == LB_NAN)) break;
+    slack = LB_LAZY - (float)lb_lift(S);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      m[i] = NEG_BIG, l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) o[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    none[0] = none[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    load_keys(first), load_values(first);  // (top is not 0: the wave has slots)
   }
 
   // The waves' parts: weights' parts and lanes joined, then the waves in LDS.

@@ -58,7 +58,9 @@ typedef struct dfl_window_cache_read_params {
 } dfl_window_cache_read_params;
 
 /* As dfl_window_decode, over such caches: the token's own key and value enter them, and count, as their codes stand.
- * A sample and key head with a group of E = 255 among its slots in use: zero divided by zero in every output. */
+ * A sample and key head with a group of E = 255 among its slots in use: zero divided by zero in every output.  Values up to
+ * the largest that a group holds are weighted without passing fp32 on the way (weights below 2^-90 or so of the largest
+ * vanish beside such values, else those below 2^-125). */
 typedef struct dfl_lowbit_decode_params {
   int dtype, bits;
   const void* q;
