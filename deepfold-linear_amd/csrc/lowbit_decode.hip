@@ -202,8 +202,9 @@ __global__ void __launch_bounds__(256 * lb_waves(sizeof(T), DP, NT), lb_least_wa
     for (int e = threadIdx.x; e <= dist; e += blockDim.x) s_lut[e] = (uint8_t)rel_bucket(a.rel, -e);
   }
   // The queries: lane's column n is head n % GP of a tile, elements DP / 4 * h .. of it.  They take the scale's power of
-  // two, which changes none of their digits; the scores take the rest of it, a factor from 1 to 2.
-  const float sc0 = a.scale * LOG2E, two = __uint_as_float(__float_as_uint(sc0) & 0x7f800000u), sc = sc0 / two;
+  // two, which changes none of their digits, where it is below 1 (above, a query may have no room for it); the scores take
+  // the rest of the scale.
+  const float sc0 = a.scale * LOG2E, two = fminf(__uint_as_float(__float_as_uint(sc0) & 0x7f800000u), 1.f), sc = sc0 / two;
   LbFrag q[NT][QT][KF];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {

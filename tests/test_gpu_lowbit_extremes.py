@@ -91,3 +91,30 @@ def test_large_values_with_a_table():
         table[2, 1] = -float("inf")
         values = rnd(B, Hk, S, d, seed=5).clamp(-1, 1) * BIG
         check(q, k, v.clamp(-1, 1) * BIG, rnd(B, Hk, S, d, seed=4), values, 8, [399, 1000], n_sink=3, table=table, edges=(1, 7, 32, 100))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("scale", [1.5, 4.0, 2.0**20, 1e30])
+def test_queries_times_a_large_scale(scale, bits, dtype):
+    """Scores within reach whose queries, times the scale, are not."""
+    B, H, Hk, d, S = 2, 4, 1, 64, 100
+    q, k, v = token(B, H, Hk, d, 1, dtype)
+    keys, values = rnd(B, Hk, S, d, seed=4), rnd(B, Hk, S, d, seed=5)
+    small = 2.0**-126  # of the keys; queries as large as bf16 and fp32 have them, if the scale lets the scores stay below 100
+    size = min(3.3e38, 2.0**126 / scale)
+    check(q.clamp(-1, 1) * size, k * small, v, keys * small, values, bits, [70, 1000], scale=scale)
+    check(q.clamp(-1, 1) * 2.0**60, k / 2.0**60 / scale, v, keys / 2.0**60 / scale, values, bits, [70, 1000], scale=scale)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_the_largest_finite_query(bits):
+    """A query's largest element at the end of fp32, its head held to the bound of the others."""
+    H, d, S = 4, 32, 60
+    q, k, v = token(1, H, 1, d, 1, F32)
+    q[0, 1] = 0
+    q[0, 1, 0] = torch.finfo(F32).max
+    q[0, 2] = -torch.finfo(F32).max
+    check(q, k, v, rnd(1, 1, S, d, seed=4), rnd(1, 1, S, d, seed=5), bits, [40], scale=1e-30)
+    check(q, k * 1e-38, v, rnd(1, 1, S, d, seed=4) * 1e-38, rnd(1, 1, S, d, seed=5), bits, [40], scale=1.0)
+    check(q, k * 1e-38, v, rnd(1, 1, S, d, seed=4) * 1e-38, rnd(1, 1, S, d, seed=5), bits, [40], scale=4.0)
