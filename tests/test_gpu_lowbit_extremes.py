@@ -118,3 +118,25 @@ def test_the_largest_finite_query(bits):
     check(q, k, v, rnd(1, 1, S, d, seed=4), rnd(1, 1, S, d, seed=5), bits, [40], scale=1e-30)
     check(q, k * 1e-38, v, rnd(1, 1, S, d, seed=4) * 1e-38, rnd(1, 1, S, d, seed=5), bits, [40], scale=1.0)
     check(q, k * 1e-38, v, rnd(1, 1, S, d, seed=4) * 1e-38, rnd(1, 1, S, d, seed=5), bits, [40], scale=4.0)
+
+
+@pytest.mark.parametrize("dtype,bits,d", [(BF, 4, 32), (F32, 8, 16)])
+def test_one_head_in_many_splits(dtype, bits, d):
+    """One key head of so many slots that its splits (250) pass the join's workgroup: all of them, some without a slot, one
+    with a group that is no number."""
+    from deepfold_amd import window_decode_attn
+    from test_gpu_lowbit import cache
+
+    S = 120000
+    q, k, v = token(1, 1, 1, d, 1, dtype)
+    kc, vc = (cache(1, 1, S, d, bits, s, odd=False) for s in (4, 5))
+    q = q * 4  # (so that the splits' references differ)
+    for n in (3 * S + 11, 100001, 62000, 477):
+        lengths = torch.tensor([n])
+        want, bound, _, _ = ref.decode(q, k, v, kc, vc, lengths, 0, result=dtype)
+        o = window_decode_attn(q.to(DEV), k.to(DEV), v.to(DEV), onto(kc), onto(vc), lengths.to(DEV))
+        holds(str(n), o, want, bound)
+    vc.exponents[0, 0, 0, 100001] = 255
+    for n, spoilt in ((100000, False), (100002, True)):
+        o = window_decode_attn(q.to(DEV), k.to(DEV), v.to(DEV), onto(kc), onto(vc), torch.tensor([n], device=DEV))
+        assert bool(o.isnan().all()) == spoilt and bool(o.isnan().any()) == spoilt
