@@ -19,6 +19,7 @@ hipError_t launch_lowbit_decode(const LowbitDecodeArgs& a, bool bf16_in, int bit
 LowbitPlan lowbit_decode_plan(bool bf16_in, int B, int H, int Hk, int d, int S);
 hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s);
 int int8_linear_form(int M, int K, int N);
+bool int8_linear_fits(int M, int N);
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s);
 }  // namespace dfl
 
@@ -123,6 +124,7 @@ int dfl_lowbit_cache_fill(const dfl_lowbit_cache_fill_params* p, void* stream) {
     a.lengths = p->lengths; a.starts = p->starts;
     a.kc = cache(p->k_cache); a.vc = cache(p->v_cache);
     a.B = p->B; a.Hk = p->Hk; a.N = p->N; a.d = p->d; a.window = p->window; a.n_sink = p->n_sink;
+    a.first = 0;
     const hipError_t e = dfl::launch_lowbit_fill(a, p->dtype == DFL_BF16, p->bits, (hipStream_t)stream);
     return e == hipSuccess ? 0 : dfl::capi_hip_fail(e, "few-bit cache fill launch");
   });
@@ -144,6 +146,7 @@ int dfl_window_cache_read(const dfl_window_cache_read_params* p, void* stream) {
     a.lengths = p->lengths;
     a.k = p->k; a.v = p->v; a.mask = p->mask;
     a.B = p->B; a.Hk = p->Hk; a.d = p->d; a.window = p->window; a.n_sink = p->n_sink;
+    a.first = 0;
     const hipError_t e = dfl::launch_cache_read(a, p->dtype == DFL_BF16, p->bits, (hipStream_t)stream);
     return e == hipSuccess ? 0 : dfl::capi_hip_fail(e, "cache read launch");
   });
@@ -229,9 +232,9 @@ int dfl_int8_linear(const dfl_int8_linear_params* p, void* workspace, size_t wor
       return fail("w and w_stride must be multiples of 16 bytes, w_stride at least K");
     if (p->M > MAX_ROWS || p->N > MAX_ROWS) return fail("M=%d, N=%d: at most %d", p->M, p->N, MAX_ROWS);
     const int form = dfl::int8_linear_form(p->M, p->K, p->N);
-    if (form >= dfl::I8_TILE_64 && (long long)((p->M + 63) / 64) * ((p->N + 63) / 64) >= (1ll << 31)) return fail("M * N is too large");
+    if (!dfl::int8_linear_fits(p->M, p->N)) return fail("M * N is too large");
     dfl::Int8LinearArgs a = {p->x, p->x_stride, nullptr, nullptr, static_cast<const int8_t*>(p->w), p->w_scale, p->bias, p->y,
-                             0, p->w_stride, p->M, p->K, p->N};
+                             0, p->w_stride, p->M, p->K, p->N, 0};
     hipError_t e;
     if (form > dfl::I8_OWN_32) {
       const LinearWs ws(p->M, p->K);

@@ -272,6 +272,7 @@ int dfl_window_cache_append(const dfl_window_cache_fill_params* p, const int* st
     a.vsb = p->v_stride_b; a.vsh = p->v_stride_h; a.vsn = p->v_stride_n;
     a.lengths = p->lengths;
     a.starts = starts;
+    a.first = 0;
     a.kc = p->k_cache; a.vc = p->v_cache;
     a.kcsb = p->kc_stride_b; a.kcsh = p->kc_stride_h; a.kcsn = p->kc_stride_n;
     a.vcsb = p->vc_stride_b; a.vcsh = p->vc_stride_h; a.vcsn = p->vc_stride_n;

@@ -4,6 +4,7 @@
 // Bounds: large products the matrix instructions at the clock that they leave (8192 x 4096 x 4096: 130-144 us, 1900-2110 TOP/s,
 // where a library's product in 8-bit integers reaches 2150 and the same loop without its loads 2180-2550), the codes memory (19
 // us for 100 MB); few tokens the weights' bytes and latency (1 x 4096 x 4096: 5.8 us, 32: 4.5 + 8.4).
+#include "launch_slices.h"
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 
@@ -128,7 +129,7 @@ template <typename T, int MT, int OWN, bool FAST> __global__ void __launch_bound
   __shared__ float s_scale[16 * MT];
   extern __shared__ __align__(16) int8_t s_x[];  // OWN: [tokens][steps * 128 + 16] codes
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, h = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
+  const int n0 = (a.first + blockIdx.x) * 16, m0 = blockIdx.y * (16 * MT);
   const int8_t* w = a.w + (long long)min(n0 + r, a.N - 1) * a.ws;
   const int steps = (a.K + 127) / 128, tail = ((a.K + 15) & ~15) - 16;  // last 16 bytes of a row of weights
   auto weights = [&](i32x4 (&v)[2], int s) {
@@ -410,9 +411,15 @@ template <typename T> static bool aligned16(const void* p, std::initializer_list
 }
 template <typename T, int W> static hipError_t codes_w(const RowCodesArgs& a, hipStream_t s) {
   const bool fast = a.K % 8 == 0 && aligned16<T>(a.x, {a.xs});
-  if (fast) hipLaunchKernelGGL((row_codes_kernel<T, true, W>), dim3((unsigned)a.M), dim3(64 * W), 0, s, a);
-  else hipLaunchKernelGGL((row_codes_kernel<T, false, W>), dim3((unsigned)a.M), dim3(64 * W), 0, s, a);
-  return hipGetLastError();
+  return launch_slices(a.M, 64 * W, [&](long long first, long long count) {
+    RowCodesArgs r = a;
+    r.x = reinterpret_cast<const T*>(a.x) + first * a.xs;
+    r.codes = a.codes + first * a.cs;
+    r.scale = a.scale + first;
+    if (fast) hipLaunchKernelGGL((row_codes_kernel<T, true, W>), dim3((unsigned)count), dim3(64 * W), 0, s, r);
+    else hipLaunchKernelGGL((row_codes_kernel<T, false, W>), dim3((unsigned)count), dim3(64 * W), 0, s, r);
+    return hipGetLastError();
+  });
 }
 hipError_t launch_row_codes(const RowCodesArgs& a, bool bf16_in, hipStream_t s) {
   const bool wide = a.K > 64 * 8 * I8_KEEP;
@@ -425,14 +432,17 @@ template <typename T, int TM, int TN, int WM, int WN, int BUF> static hipError_t
   const size_t lds = BUF * (TM + TN) * 128;
   const hipError_t e = set_lds_limit((const void*)kern, lds);
   if (e != hipSuccess) return e;
-  const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + TN - 1) / TN);
+  const long long tiles = (long long)((a.M + TM - 1) / TM) * ((a.N + TN - 1) / TN);  // (below 2^23: int8_linear_fits)
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(64 * WM * WN), lds, s, a);
   return hipGetLastError();
 }
-template <typename T, int MT> static hipError_t few_t(const Int8LinearArgs& a, hipStream_t s) {
-  const dim3 grid((a.N + 15) / 16, (a.M + 16 * MT - 1) / (16 * MT));
-  hipLaunchKernelGGL((int8_few_kernel<T, MT, 0, false>), grid, dim3(512), 0, s, a);
-  return hipGetLastError();
+template <typename T, int MT> static hipError_t few_t(Int8LinearArgs a, hipStream_t s) {
+  return launch_slices((a.N + 15) / 16, 512, [&](long long first, long long count) {
+    const dim3 grid((unsigned)count, (a.M + 16 * MT - 1) / (16 * MT));
+    a.first = (int)first;
+    hipLaunchKernelGGL((int8_few_kernel<T, MT, 0, false>), grid, dim3(512), 0, s, a);
+    return hipGetLastError();
+  });
 }
 template <typename T, int MT, int OWN> static hipError_t own_t(const Int8LinearArgs& a, hipStream_t s) {
   const bool fast = a.K % 8 == 0 && aligned16<T>(a.x, {a.xs});
@@ -457,6 +467,9 @@ template <typename T> static hipError_t linear_t(const Int8LinearArgs& a, int fo
 hipError_t launch_int8_linear(const Int8LinearArgs& a, bool bf16_out, int form, hipStream_t s) {
   return bf16_out ? linear_t<bf16>(a, form, s) : linear_t<float>(a, form, s);
 }
+
+// Whether the largest tiles of a product fit one launch: y has at least 500 GB where they do not.
+bool int8_linear_fits(int M, int N) { return ((M + 255ll) / 256) * ((N + 255ll) / 256) <= launch_most(512); }
 
 // Which kernel a product takes.  Calls in a graph (us, M x K x N) that form the codes in the product's workgroups and that take a
 // kernel for them: 1 x 4096 x 4096 5.6, 7.4; 8 x 4096 x 4096 8.2, 9.0; 8 x 2048 x 4096 6.2, 9.0; 16 x 2048 x 4096 8.0, 9.7;

@@ -23,6 +23,7 @@ struct LowbitFillArgs {
   const int* starts;   // (B) position of row 0, or null: 0
   LowbitCache kc, vc;
   int B, Hk, N, d, window, n_sink;
+  int first;  // workgroup of the launch's first (launch_slices.h)
 };
 
 struct CacheReadArgs {
@@ -32,6 +33,7 @@ struct CacheReadArgs {
   void* v;
   float* mask;  // (B,S)
   int B, Hk, d, window, n_sink;
+  int first;
 };
 
 struct LowbitDecodeArgs {
@@ -81,6 +83,7 @@ struct Int8LinearArgs {
   void* y;           // (M,N)
   long long as, ws;
   int M, K, N;
+  int first;  // 16 rows of weights of the launch's first workgroup (I8_OWN_*, I8_FEW_*)
 };
 
 }  // namespace dfl

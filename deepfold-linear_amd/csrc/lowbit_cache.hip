@@ -4,6 +4,7 @@
 // A thread takes 8 elements of a row of the keys and the same of the values: 16 bytes of bf16 rows, 4 or 8 bytes of
 // codes, neighbouring threads neighbouring elements, so that a group's maximum is two exchanges within a quad of lanes.
 // A workgroup has whole rows (GR groups each: 64, 32, 21 or 16 of them), so that no thread divides a 64-bit index.
+#include "launch_slices.h"
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 
@@ -31,7 +32,7 @@ template <typename T, int BITS, int GR, bool FAST> __global__ void __launch_boun
   // Latest position that a slot holds: past the first tokens, turn `turns` of the window up to the slot of `last`, one
   // turn less behind it.
   const unsigned past = last >= (unsigned)a.n_sink ? last - a.n_sink : 0u, turns = past / a.window, rest = past - turns * a.window;
-  const int s = blockIdx.x * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
+  const int s = (a.first + blockIdx.x) * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
   if ((int)threadIdx.x >= ROWS * NCH || s >= S || (unsigned)s > last) return;
   const unsigned o = (unsigned)(s - a.n_sink), back = o > rest;
   if (s >= a.n_sink && turns < back) return;
@@ -69,7 +70,7 @@ template <typename T, int BITS, int GR, bool FAST> __global__ void __launch_boun
   const int S = a.n_sink + a.window;
   const int bh = blockIdx.y, b = bh / a.Hk, hk = bh % a.Hk;
   const int len = a.lengths[b];
-  const int j = blockIdx.x * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
+  const int j = (a.first + blockIdx.x) * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
   if ((int)threadIdx.x >= ROWS * NCH || j >= S || c * 8 >= a.d) return;
   const int p = j < a.n_sink ? j : max(len, 0) - S + j;  // S < 2^29: no overflow
   const bool held = j < a.n_sink ? j < len : p >= a.n_sink;
@@ -94,13 +95,16 @@ template <typename T> static bool aligned16(const void* p, std::initializer_list
   return ok;
 }
 
-template <typename T, int BITS, int GR> static hipError_t fill_g(const LowbitFillArgs& a, hipStream_t s) {
+template <typename T, int BITS, int GR> static hipError_t fill_g(LowbitFillArgs a, hipStream_t s) {
   const bool fast = a.d % 8 == 0 && aligned16<T>(a.k, {a.ksb, a.ksh, a.ksn}) && aligned16<T>(a.v, {a.vsb, a.vsh, a.vsn});
   constexpr int ROWS = 256 / (4 * GR);
-  const dim3 grid((a.n_sink + a.window + ROWS - 1) / ROWS, a.B * a.Hk);
-  if (fast) hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_slices((a.n_sink + a.window + ROWS - 1) / ROWS, 256, [&](long long first, long long count) {
+    const dim3 grid((unsigned)count, a.B * a.Hk);
+    a.first = (int)first;
+    if (fast) hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((lowbit_fill_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  });
 }
 template <typename T, int BITS> static hipError_t fill_b(const LowbitFillArgs& a, hipStream_t s) {
   switch (lb_groups(a.d)) {
@@ -115,15 +119,18 @@ hipError_t launch_lowbit_fill(const LowbitFillArgs& a, bool bf16_in, int bits, h
   return bits == 4 ? fill_b<float, 4>(a, s) : fill_b<float, 8>(a, s);
 }
 
-template <typename T, int BITS, int GR> static hipError_t read_g(const CacheReadArgs& a, hipStream_t s) {
+template <typename T, int BITS, int GR> static hipError_t read_g(CacheReadArgs a, hipStream_t s) {
   bool fast = a.d % 8 == 0 && aligned16<T>(a.k, {}) && aligned16<T>(a.v, {});
   if (BITS == 0)
     fast = fast && aligned16<T>(a.kc.codes, {a.kc.sb, a.kc.sh, a.kc.sn}) && aligned16<T>(a.vc.codes, {a.vc.sb, a.vc.sh, a.vc.sn});
   constexpr int ROWS = 256 / (4 * GR);
-  const dim3 grid((a.n_sink + a.window + ROWS - 1) / ROWS, a.B * a.Hk);
-  if (fast) hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_slices((a.n_sink + a.window + ROWS - 1) / ROWS, 256, [&](long long first, long long count) {
+    const dim3 grid((unsigned)count, a.B * a.Hk);
+    a.first = (int)first;
+    if (fast) hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((cache_read_kernel<T, BITS, GR, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  });
 }
 template <typename T, int BITS> static hipError_t read_b(const CacheReadArgs& a, hipStream_t s) {
   switch (lb_groups(a.d)) {

@@ -52,6 +52,7 @@ struct CacheFillArgs {
   void* vc;
   long long kcsb, kcsh, kcsn, vcsb, vcsh, vcsn;
   int B, Hk, N, d, window, n_sink;
+  int first;  // workgroup of the launch's first (launch_slices.h)
 };
 
 struct DecodeArgs {

@@ -7,6 +7,7 @@
 // sequences of 4100 slots, 32 / 4 heads, d 128, bf16, 67 MB: 38 us).  32 sequences of 4100 slots, 32 / 8 heads, d 128,
 // bf16, 537 MB: 106 us, 5.0 TB/s of the 6.2-6.4 that a copy or read reaches (join 5 us more); 270 MB of prompts into 32
 // caches: 43 us, 6.2 TB/s.  One sequence of 1028 slots, 16 / 4 heads, d 64: 7 + 3.6 us, both of them latency.
+#include "launch_slices.h"
 #include "window_engine.h"
 
 #include <algorithm>
@@ -26,7 +27,7 @@ template <typename T, bool FAST> __global__ void __launch_bounds__(256) cache_fi
   const int n = min(a.lengths[b], a.N), start = a.starts ? a.starts[b] : 0;
   if (n <= 0 || start < 0) return;
   const unsigned last = (unsigned)start + (unsigned)n - 1;  // at most 2^31 + 2^28
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;  // (slot, chunk)
+  const long long e = ((long long)a.first + blockIdx.x) * 256 + threadIdx.x;  // (slot, chunk)
   const int s = (int)(e / nch), c = (int)(e % nch);
   if (s >= S || (unsigned)s > last) return;
   const unsigned p = s < a.n_sink ? s : s + (last - s) / a.window * a.window;  // latest position that the slot holds
@@ -237,15 +238,18 @@ template <typename T> static bool aligned(const void* p, std::initializer_list<l
   return ok;
 }
 
-template <typename T> static hipError_t fill_t(const CacheFillArgs& a, hipStream_t s) {
+template <typename T> static hipError_t fill_t(CacheFillArgs a, hipStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const bool fast = a.d % VEC == 0 && aligned<T>(a.k, {a.ksb, a.ksh, a.ksn}) && aligned<T>(a.v, {a.vsb, a.vsh, a.vsn}) &&
                     aligned<T>(a.kc, {a.kcsb, a.kcsh, a.kcsn}) && aligned<T>(a.vc, {a.vcsb, a.vcsh, a.vcsn});
   const long long per = (long long)(a.n_sink + a.window) * ((a.d + VEC - 1) / VEC);
-  const dim3 grid((unsigned)((per + 255) / 256), a.B * a.Hk);
-  if (fast) hipLaunchKernelGGL((cache_fill_kernel<T, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((cache_fill_kernel<T, false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_slices((per + 255) / 256, 256, [&](long long first, long long count) {
+    const dim3 grid((unsigned)count, a.B * a.Hk);
+    a.first = (int)first;
+    if (fast) hipLaunchKernelGGL((cache_fill_kernel<T, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((cache_fill_kernel<T, false>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  });
 }
 hipError_t launch_cache_fill(const CacheFillArgs& a, bool bf16_in, hipStream_t s) {
   return bf16_in ? fill_t<bf16>(a, s) : fill_t<float>(a, s);
