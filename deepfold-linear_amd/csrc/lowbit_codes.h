@@ -38,9 +38,12 @@ template <bool FAST> __device__ __forceinline__ void load8(Eight<bf16>& e, const
 }
 template <bool FAST> __device__ __forceinline__ void load8(Eight<float>& e, const float* row, int c, int d) {
   if (FAST) {
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f), *at = reinterpret_cast<const float4*>(row + c * 8);
-    const float4 u = c * 8 < d ? at[0] : zero, v = c * 8 < d ? at[1] : zero;
-    e.x[0] = u.x, e.x[1] = u.y, e.x[2] = u.z, e.x[3] = u.w, e.x[4] = v.x, e.x[5] = v.y, e.x[6] = v.z, e.x[7] = v.w;
+    // (vectors of the language: of two float4 objects to choose from the compiler loads each element by itself)
+    typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f4;
+    f4 u = {}, v = {};
+    if (c * 8 < d) u = reinterpret_cast<const f4*>(row + c * 8)[0], v = reinterpret_cast<const f4*>(row + c * 8)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e.x[i] = u[i], e.x[4 + i] = v[i];
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e.x[i] = c * 8 + i < d ? row[c * 8 + i] : 0.f;
