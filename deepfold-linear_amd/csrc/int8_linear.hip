@@ -3,7 +3,7 @@
 //
 // Bounds: large products the matrix instructions at the clock that they leave (8192 x 4096 x 4096: 130-144 us, 1900-2110 TOP/s,
 // where a library's product in 8-bit integers reaches 2150 and the same loop without its loads 2180-2550), the codes memory (19
-// us for 100 MB); few tokens the weights' bytes and latency (1 x 4096 x 4096: 5.8 us, 32: 4.5 + 8.4).
+// us for 100 MB); few tokens the weights' bytes and latency (1 x 4096 x 4096: 5.8-6.2 us, 32: 4.6 + 8.8).
 #include "launch_slices.h"
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
@@ -474,7 +474,9 @@ bool int8_linear_fits(int M, int N) { return ((M + 255ll) / 256) * ((N + 255ll) 
 // Which kernel a product takes.  Calls in a graph (us, M x K x N) that form the codes in the product's workgroups and that take a
 // kernel for them: 1 x 4096 x 4096 5.6, 7.4; 8 x 4096 x 4096 8.2, 9.0; 8 x 2048 x 4096 6.2, 9.0; 16 x 2048 x 4096 8.0, 9.7;
 // 16 x 512 x 512 6.1, 5.4; 32 x 1024 x 4096 7.7, 8.9; 300 x 1024 x 300 8.4, 9.5; 97 x 64 x 64 5.8, 5.4; 1 x 4096 x 11008 11.4, 12.5;
-// 8 x 4096 x 11008 16.6, 15.6; 4 x 512 x 32768 20.6, 12.1.  (A launch less saves 3 us of the caller's time besides.)
+// 8 x 4096 x 11008 16.6, 15.6; 4 x 512 x 32768 20.6, 12.1.  fp32 tokens: 1 x 4096 x 4096 5.8, 7.5; 8 x 4096 x 4096 7.8, 8.5; 16 x
+// 2048 x 4096 6.8, 8.7; 32 x 1024 x 4096 7.5, 8.5; 97 x 512 x 512 6.6, 6.3; 16 x 512 x 512 5.8, 5.4.  (A launch less saves 3 to
+// 4 us of the caller's time besides: that is what decides where the kernels are even or a little behind.)
 // Codes and product of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and 256 x 256 tiles:
 //   M 16, K 4096, N 4096     10.1  10.3  12.3  25.0  50.4
 //   32, 4096, 4096              -  11.9  12.5  25.4  50.5

@@ -12,9 +12,12 @@
 
 namespace dfl {
 
-// Bounds: memory.  135 MB of bf16 prompts into 4 bits (32 x 8 heads, 1028 slots, d 128), 170 MB in all: 34.5 us from memory,
-// 30 where the prompts are in the last level of the caches; the loads alone take 34.  (Workgroups of 128 slots that hand over
-// whole lines of exponents, with two or four rows' loads in flight: 37.)  Reading these caches back: 28.5 us, 6.0 TB/s.
+// Bounds: memory.  135 MB of bf16 prompts into 4 bits (32 x 8 heads, 1028 slots, d 128), 170 MB in all: 44 us (3.9 TB/s)
+// between readings of the caches, which leave nothing of the prompts in the last level of the caches; 35.5 in a row of fills
+// of two batches in turn, of which that level holds a part (and workgroups of 128 slots that hand over whole lines of
+// exponents, with two or four rows' loads in flight, 37).  What takes the time between readings is not settled: 8 bits, 204 MB,
+// take 37 us, 5.5 TB/s.  fp32 prompts 57.5 and 62.6 us.  Reading back: 4 bits 29 us, 5.9 TB/s, 8 bits 37, 5.5, plain caches 44,
+// 6.1.
 template <int BITS> __device__ __forceinline__ void store_codes(const LowbitCache& q, int b, int hk, int s, int c,
                                                                 const unsigned (&w)[BITS / 4], unsigned e) {
   uint8_t* to = q.codes + b * q.sb + hk * q.sh + s * q.sn + c * BITS;

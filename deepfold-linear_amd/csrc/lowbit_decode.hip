@@ -13,10 +13,10 @@
 // it), fp32 results three (24 bits), so no weight is rounded to 8 bits and the matrix rows would be idle otherwise.  fp32
 // queries are three bf16 numbers, products of their own.  Sums, references and outputs are fp32.
 //
-// Bounds: the cache's bytes, and about 230 vector instructions a block of 4 bits.  32 sequences of 4100 slots, 32 / 8 heads,
-// d 128, 4 bits, 143 MB: 29 us, 4.9 TB/s of the 6.2 that a copy reaches (bf16 caches, 537 MB: 106 us).  One sequence of 131072
-// slots, the same heads, 8 bits, 276 MB: 46.6 us, 5.9 TB/s, and 4.6 us for joining the splits.  One sequence of 1028 slots,
-// 16 / 4 heads, d 64, 4 bits: 9.7 us, latency.  Registers: the keys' are free for the next block once the scores are
+// Bounds: the cache's bytes, and about 230 vector instructions a block of 4 bits.  Kernels in a trace: 32 sequences of 4100
+// slots, 32 / 8 heads, d 128, 4 bits, 143 MB: 28.9 us, 4.9 TB/s of the 6.2 that a copy reaches (bf16 caches, 537 MB: 106 us).
+// One sequence of 131072 slots, the same heads, 8 bits, 276 MB: 47-48 us, 5.8 TB/s, and 4.1-4.6 us for joining the splits.
+// One sequence of 1028 slots, 16 / 4 heads, d 64, 4 bits: 9.3 us, latency.  Registers: the keys' are free for the next block once the scores are
 // formed, the values' once the outputs are, so that one set lets three waves a SIMD run (two sets, two waves: 33.7 us); loads go
 // through buffer resources (with 64-bit addresses a lane and clamped rows 36 us).
 #include "lowbit_args.h"

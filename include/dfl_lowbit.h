@@ -21,7 +21,7 @@
 /* A rolling cache of S = n_sink + window slots: codes (B,Hk,S,G * 4 * bits bytes), G = ceil(d / 32) groups,
  * and exponent bytes (B,Hk,G,S'), a group's slots side by side, S' a multiple of 4 from S on (the bytes
  * behind the last slot may be read, never used).  Strides in bytes: the codes' and their pointer multiples of 16,
- * the exponents' of 4. */
+ * the exponents' of 4.  The decode takes row strides below 2^26 and group strides of at most 2^28 + 192 bytes. */
 typedef struct dfl_lowbit_cache {
   void* codes;
   void* exponents;
@@ -59,7 +59,7 @@ typedef struct dfl_window_cache_read_params {
 
 /* As dfl_window_decode, over such caches: the token's own key and value enter them, and count, as their codes stand.
  * A sample and key head with a group of E = 255 among its slots in use: zero divided by zero in every output.  Values up to
- * the largest that a group holds are weighted without passing fp32 on the way (weights below 2^-90 or so of the largest
+ * the largest that a group holds are weighted without passing fp32 on the way (weights below 2^-88 of the largest may
  * vanish beside such values, else those below 2^-125). */
 typedef struct dfl_lowbit_decode_params {
   int dtype, bits;
@@ -95,8 +95,8 @@ typedef struct dfl_quantize_rows_params {
 
 /* y (M,N) contiguous in `dtype`: y[m,n] = (sum_k a[m,k] w[n,k]) s[m] w_scale[n] + bias[n] with a, s the codes and
  * scale of x's rows as in dfl_quantize_rows and w (N,K) int8 codes; bias in `dtype` or NULL.  The sum is exact (K at
- * most 131072; M and N at most 2^31 - 256).  w and its row stride (bytes) are multiples of 16, and a row's bytes up to the next multiple of 16 from K
- * on are read, whatever they hold. */
+ * most 131072; M and N at most 2^31 - 256, and ceil(M / 256) ceil(N / 256) below 2^23).  w and its row stride (bytes) are
+ * multiples of 16, and a row's bytes up to the next multiple of 16 from K on are read, whatever they hold. */
 typedef struct dfl_int8_linear_params {
   int dtype;
   const void* x;
