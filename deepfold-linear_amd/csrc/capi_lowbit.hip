@@ -208,7 +208,8 @@ int dfl_quantize_rows(const dfl_quantize_rows_params* p, void* stream) {
   return guarded([&] {
     if (!p) return fail("params is NULL");
     if (p->dtype != DFL_F32 && p->dtype != DFL_BF16) return fail("dtype must be DFL_F32 or DFL_BF16");
-    if (p->M <= 0 || p->M >= (1ll << 31) || p->K <= 0 || p->K > MAX_K) return fail("M=%lld, K=%d: need 0 < M < 2^31, 0 < K <= %d", p->M, p->K, MAX_K);
+    if (p->M <= 0 || p->M >= (1ll << 31) || p->K <= 0 || p->K > MAX_K)
+      return fail("M=%lld, K=%d: need 0 < M < 2^31, 0 < K <= %d", p->M, p->K, MAX_K);
     if (!p->x || !p->codes || !p->scale) return fail("required pointer is NULL");
     if (p->code_stride < p->K || ((uintptr_t)p->codes | (uintptr_t)p->code_stride) & 15)
       return fail("codes and code_stride must be multiples of 16 bytes, code_stride at least K");

@@ -473,8 +473,8 @@ bool int8_linear_fits(int M, int N) { return ((M + 255ll) / 256) * ((N + 255ll) 
 
 // Which kernel a product takes.  Calls in a graph (us, M x K x N) that form the codes in the product's workgroups and that take a
 // kernel for them: 1 x 4096 x 4096 5.6, 7.4; 8 x 4096 x 4096 8.2, 9.0; 8 x 2048 x 4096 6.2, 9.0; 16 x 2048 x 4096 8.0, 9.7;
-// 16 x 512 x 512 6.1, 5.4; 32 x 1024 x 4096 7.7, 8.9; 300 x 1024 x 300 8.4, 9.5; 97 x 64 x 64 5.8, 5.4; 1 x 4096 x 11008 11.4, 12.5;
-// 8 x 4096 x 11008 16.6, 15.6; 4 x 512 x 32768 20.6, 12.1.  fp32 tokens: 1 x 4096 x 4096 5.8, 7.5; 8 x 4096 x 4096 7.8, 8.5; 16 x
+// 16 x 512 x 512 6.1, 5.4; 32 x 1024 x 4096 7.7, 8.9; 300 x 1024 x 300 8.4, 9.5; 97 x 64 x 64 5.8, 5.4;
+// 1 x 4096 x 11008 11.4, 12.5; 8 x 4096 x 11008 16.6, 15.6; 4 x 512 x 32768 20.6, 12.1.  fp32 tokens: 1 x 4096 x 4096 5.8, 7.5; 8 x 4096 x 4096 7.8, 8.5; 16 x
 // 2048 x 4096 6.8, 8.7; 32 x 1024 x 4096 7.5, 8.5; 97 x 512 x 512 6.6, 6.3; 16 x 512 x 512 5.8, 5.4.  (A launch less saves 3 to
 // 4 us of the caller's time besides: that is what decides where the kernels are even or a little behind.)
 // Codes and product of 1 / 2 tiles of 16 tokens and of 64 x 64, 128 x 128 and 256 x 256 tiles:

@@ -34,7 +34,8 @@ template <typename T, int BITS, int GR, bool FAST> __global__ void __launch_boun
   const unsigned last = (unsigned)start + (unsigned)n - 1;  // at most 2^31 + 2^28
   // Latest position that a slot holds: past the first tokens, turn `turns` of the window up to the slot of `last`, one
   // turn less behind it.
-  const unsigned past = last >= (unsigned)a.n_sink ? last - a.n_sink : 0u, turns = past / a.window, rest = past - turns * a.window;
+  const unsigned past = last >= (unsigned)a.n_sink ? last - a.n_sink : 0u, turns = past / a.window;
+  const unsigned rest = past - turns * a.window;
   const int s = (a.first + blockIdx.x) * ROWS + threadIdx.x / NCH, c = threadIdx.x % NCH;
   if ((int)threadIdx.x >= ROWS * NCH || s >= S || (unsigned)s > last) return;
   const unsigned o = (unsigned)(s - a.n_sink), back = o > rest;

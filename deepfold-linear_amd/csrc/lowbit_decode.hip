@@ -16,9 +16,10 @@
 // Bounds: the cache's bytes, and about 230 vector instructions a block of 4 bits.  Kernels in a trace: 32 sequences of 4100
 // slots, 32 / 8 heads, d 128, 4 bits, 143 MB: 28.9 us, 4.9 TB/s of the 6.2 that a copy reaches (bf16 caches, 537 MB: 106 us).
 // One sequence of 131072 slots, the same heads, 8 bits, 276 MB: 47-48 us, 5.8 TB/s, and 4.1-4.6 us for joining the splits.
-// One sequence of 1028 slots, 16 / 4 heads, d 64, 4 bits: 9.3 us, latency.  Registers: the keys' are free for the next block once the scores are
-// formed, the values' once the outputs are, so that one set lets three waves a SIMD run (two sets, two waves: 33.7 us); loads go
-// through buffer resources (with 64-bit addresses a lane and clamped rows 36 us).
+// One sequence of 1028 slots, 16 / 4 heads, d 64, 4 bits: 9.3 us, latency.
+// Registers: the keys' are free for the next block once the scores are formed, the values' once the outputs are, so that one
+// set lets three waves a SIMD run (two sets, two waves: 33.7 us); loads go through buffer resources (with 64-bit addresses a
+// lane and clamped rows 36 us).
 #include "lowbit_args.h"
 #include "lowbit_codes.h"
 #include "window_engine.h"
@@ -54,7 +55,8 @@ __device__ __forceinline__ int lb_distance(int s, int t, int n_sink, int window,
   const int back = rest - (s - n_sink);
   return s < n_sink ? t - s : back + (back < 0 ? window : 0);
 }
-__device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {  // upper halves: exact where the values have 8 bits, else cut off
+// Upper halves: exact where the values have 8 bits, else cut off.
+__device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
@@ -75,7 +77,8 @@ __device__ __forceinline__ lb_rsrc lb_buffer(const uint8_t* p, int bytes) {
 // N bytes at lane + row.  LB_ONCE: not kept in the caches (the values; 8 bits, one sequence of 131072 slots 54.7 -> 48.5 us,
 // with the keys too 50.9; 4 bits, 32 sequences of 4100 31.5 -> 31.0).
 constexpr int LB_ONCE = 2;
-template <int N, int AUX = 0, int W> __device__ __forceinline__ void lb_load(unsigned (&w)[W], lb_rsrc b, unsigned lane, unsigned row) {
+template <int N, int AUX = 0, int W>
+__device__ __forceinline__ void lb_load(unsigned (&w)[W], lb_rsrc b, unsigned lane, unsigned row) {
   static_assert(W == (N + 3) / 4, "whole dwords");
   if constexpr (N == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(b, lane, row, AUX);
   else if constexpr (N == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b16(b, lane, row, AUX);
@@ -532,7 +535,8 @@ template <typename T, int BITS, int DP, int NT, bool REL> static hipError_t deco
   return hipGetLastError();
 }
 template <typename T, int BITS, int DP> static hipError_t decode_d(LowbitDecodeArgs a, hipStream_t s) {
-  a.q_fast = a.d % 8 == 0 && (((uintptr_t)a.q | (uintptr_t)(a.qsb * (long long)sizeof(T)) | (uintptr_t)(a.qsh * (long long)sizeof(T))) & 15) == 0;
+  const long long size = sizeof(T);
+  a.q_fast = a.d % 8 == 0 && (((uintptr_t)a.q | (uintptr_t)(a.qsb * size) | (uintptr_t)(a.qsh * size)) & 15) == 0;
   const bool two = a.H / a.Hk > LbHeads<T>::GP;
   if (a.table) return two ? decode_l<T, BITS, DP, 2, true>(a, s) : decode_l<T, BITS, DP, 1, true>(a, s);
   return two ? decode_l<T, BITS, DP, 2, false>(a, s) : decode_l<T, BITS, DP, 1, false>(a, s);

@@ -59,7 +59,8 @@ def _linear(x, codes, scale, bias):
     b = None if bias is None else bias.to(x.dtype).contiguous()
     scale = scale.contiguous()
     row = codes.stride(0) if N > 1 else -(-K // 16) * 16
-    p = _lib.Int8LinearParams(_dtype_code("int8_linear", x), xc.data_ptr(), xc.stride(0), codes.data_ptr(), row, scale.data_ptr(), _lib.ptr(b), y.data_ptr(), M, K, N)
+    p = _lib.Int8LinearParams(_dtype_code("int8_linear", x), xc.data_ptr(), xc.stride(0), codes.data_ptr(), row, scale.data_ptr(),
+                              _lib.ptr(b), y.data_ptr(), M, K, N)
     lib = _lib.load()
     # the tokens' codes, in a workspace of the call's own: calls on other streams and captured graphs cannot share it
     nbytes = lib.dfl_int8_linear_workspace_size(M, K, N)

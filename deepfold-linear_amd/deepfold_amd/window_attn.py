@@ -502,7 +502,8 @@ def window_cache_fill(
         if V.dtype != K.dtype or K.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"{what}: K and V must both be bf16 or both fp32, got {K.dtype} and {V.dtype}")
         if not 1 <= d <= MAX_HEAD_DIM or not 1 <= N <= MAX_SLOTS:
-            raise ValueError(f"{what}: K {tuple(K.shape)} is empty, or its head dim above {MAX_HEAD_DIM} or rows above {MAX_SLOTS}")
+            raise ValueError(f"{what}: K {tuple(K.shape)} is empty, or its head dim above {MAX_HEAD_DIM} or rows above "
+                             f"{MAX_SLOTS}")
         _check_codes(what, k_cache, v_cache, B, Hk, d, n_sink)
     else:
         _no_grad_inputs(what, K, V, k_cache, v_cache)
@@ -537,9 +538,9 @@ def window_cache_read(
     j, any other row position lengths[b] - (n_sink + window) + j: the last ``window`` positions end with the last row.  Rows
     that have no such position (short sequences, lengths below 1) are zero and masked: 0.  The caches may be tensors
     (``dtype`` is theirs) or in few bits (``dtype`` bf16 or fp32, by default bf16, in which every code is
-    exact).  The rows that follow may be more than ``window`` only where
-    lengths[b] >= n_sink (module docstring).  Distances between the first tokens and the others are those of the rows, not of the positions: a table of
-    relative biases that goes on beyond the window sees them nearer.  No gradient."""
+    exact).  The rows that follow may be more than ``window`` only where lengths[b] >= n_sink (module docstring).  Distances
+    between the first tokens and the others are those of the rows, not of the positions: a table of relative biases that
+    goes on beyond the window sees them nearer.  No gradient."""
     what = "window_cache_read"
     n_sink = int(n_sink)
     if _same_kind(what, k_cache, v_cache):
@@ -585,8 +586,8 @@ def window_decode_attn(
     q (B,H,D); k, v (B,Hk,D) the token's own key and value, which enter k_cache, v_cache (B,Hk,n_sink + window,D) in
     place at position lengths[b], the number of tokens that the sample's cache has taken so far; lengths (B,) int32 or
     int64, below 2^31 (above counts as 2^31 - 1), on the device, not changed by the call; a sample with
-    lengths[b] < 0 has no token: its output is zero and its caches stay as they are.  All of q, k, v and the caches in bf16 or all in fp32.  The table has one direction
-    (len(rel_edges) + 1 buckets).  No gradient.  Returns o (B,H,D).
+    lengths[b] < 0 has no token: its output is zero and its caches stay as they are.  All of q, k, v and the caches in bf16
+    or all in fp32.  The table has one direction (len(rel_edges) + 1 buckets).  No gradient.  Returns o (B,H,D).
 
     Both caches may be in 8 or 4 bits (``quantized_cache``): the token's own key and value are rounded to codes and
     enter, and count, as their codes stand; q, k and v are bf16 or fp32 and only the result is rounded to their type.

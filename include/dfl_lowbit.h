@@ -80,8 +80,9 @@ typedef struct dfl_lowbit_decode_params {
 } dfl_lowbit_decode_params;
 
 /* Rows x (M,K), row stride x_stride, as codes (M,K) int8 with row stride code_stride >= K (a multiple of 16, as the
- * pointer is; the bytes from K on are written as zeros) and scale (M) fp32: scale = max(max |x| / 127 rounded to fp32, 2^-100), code the
- * integer nearest to x / scale, ties to even.  A row that holds an infinity or NaN has scale NaN and codes 0. */
+ * pointer is; the bytes from K on are written as zeros) and scale (M) fp32: scale = max(max |x| / 127 rounded to fp32,
+ * 2^-100), code the integer nearest to x / scale, ties to even.  A row that holds an infinity or NaN has scale NaN and
+ * codes 0. */
 typedef struct dfl_quantize_rows_params {
   int dtype;
   const void* x;
